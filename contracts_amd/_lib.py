@@ -125,7 +125,60 @@ EXPORTS = {
     "ce_last_error": (C.c_char_p, [C.c_void_p]),
 }
 
+# ---- libcontracts_policy.so (include/contracts_policy.h): a library of its own, loaded when a policy operator is first used ----
+POLICY_LIB_PATH = os.path.join(HERE, "csrc", "libcontracts_policy.so")
+POLICY_ABI_VERSION = 1
+F32, BF16, F16, F64, U8, I32, I64 = range(7)  # enum ce_dtype
+SCAN_REVERSE, SCAN_SAVED_STEPS, ADV_DONE_PER_AGENT = 1, 16, 1
+
+
+class CeScan(C.Structure):
+    _fields_ = [("abi_version", C.c_uint32), ("device", C.c_int32), ("dtype", C.c_uint32), ("gate_dtype", C.c_uint32), ("flags", C.c_uint32),
+                ("reserved", C.c_uint32), ("steps", C.c_uint64), ("rows", C.c_uint64), ("channels", C.c_uint64), ("heads", C.c_uint64),
+                ("x_step", C.c_int64), ("x_row", C.c_int64), ("gate_step", C.c_int64), ("gate_row", C.c_int64), ("done_step", C.c_int64),
+                ("done_row", C.c_int64), ("decay", C.c_double), ("x", _P), ("gate", _P), ("done", _P), ("state", _P), ("y", _P), ("last", _P),
+                ("saved", _P), ("workspace", _P), ("workspace_bytes", C.c_uint64)]
+
+
+class CeScanGrad(C.Structure):
+    _fields_ = [("dy", _P), ("dlast", _P), ("dx", _P), ("dgate", _P), ("dstate", _P)]
+
+
+class CeAdvantage(C.Structure):
+    _fields_ = [("abi_version", C.c_uint32), ("device", C.c_int32), ("reward_dtype", C.c_uint32), ("value_dtype", C.c_uint32), ("flags", C.c_uint32),
+                ("first_plane", C.c_uint32), ("planes", C.c_uint64), ("rows", C.c_uint64), ("agents", C.c_uint64), ("gamma", C.c_double),
+                ("lam", C.c_double), ("reward", _P), ("value", _P), ("last_value", _P), ("done", _P), ("advantage", _P), ("ret", _P)]
+
+
+class CeLogits(C.Structure):
+    _fields_ = [("abi_version", C.c_uint32), ("device", C.c_int32), ("dtype", C.c_uint32), ("out_dtype", C.c_uint32), ("token_dtype", C.c_uint32),
+                ("bias_dtype", C.c_uint32), ("mask_dtype", C.c_uint32), ("reserved", C.c_uint32), ("rows", C.c_uint64), ("vocab", C.c_uint64),
+                ("history", C.c_uint64), ("logits_row", C.c_int64), ("out_row", C.c_int64), ("token_row", C.c_int64), ("token_step", C.c_int64),
+                ("bias_rows", C.c_uint64), ("mask_rows", C.c_uint64), ("repetition_all", C.c_double), ("presence_all", C.c_double),
+                ("frequency_all", C.c_double), ("logits", _P), ("tokens", _P), ("lengths", _P), ("prompt_lengths", _P), ("repetition", _P),
+                ("presence", _P), ("frequency", _P), ("bias", _P), ("mask", _P), ("mask_index", _P), ("out", _P), ("workspace", _P),
+                ("workspace_bytes", C.c_uint64)]
+
+
+class CeLogitsGrad(C.Structure):
+    _fields_ = [("dout", _P), ("dout_row", C.c_int64), ("dlogits", _P), ("dbias", _P)]
+
+
+POLICY_EXPORTS = {
+    "ce_policy_abi_version": (C.c_int, []),
+    "ce_policy_error": (C.c_char_p, []),
+    "ce_linear_scan_workspace": (C.c_int, [C.POINTER(CeScan), C.POINTER(C.c_uint64)]),
+    "ce_linear_scan": (C.c_int, [C.POINTER(CeScan), C.c_void_p]),
+    "ce_linear_scan_backward_workspace": (C.c_int, [C.POINTER(CeScan), C.POINTER(CeScanGrad), C.POINTER(C.c_uint64)]),
+    "ce_linear_scan_backward": (C.c_int, [C.POINTER(CeScan), C.POINTER(CeScanGrad), C.c_void_p]),
+    "ce_advantages": (C.c_int, [C.POINTER(CeAdvantage), C.c_void_p]),
+    "ce_process_logits": (C.c_int, [C.POINTER(CeLogits), C.c_void_p]),
+    "ce_process_logits_backward_workspace": (C.c_int, [C.POINTER(CeLogits), C.POINTER(CeLogitsGrad), C.POINTER(C.c_uint64)]),
+    "ce_process_logits_backward": (C.c_int, [C.POINTER(CeLogits), C.POINTER(CeLogitsGrad), C.c_void_p]),
+}
+
 _lib = None
+_policy = None
 
 
 class EngineError(RuntimeError):
@@ -157,6 +210,31 @@ def load():
         raise EngineError("ABI version mismatch")
     _lib = L
     return L
+
+
+def load_policy():
+    """Loads the policy operators.  Raises if they have not been built (python -m contracts_amd.build)."""
+    global _policy
+    if _policy is not None:
+        return _policy
+    if not os.path.exists(POLICY_LIB_PATH):
+        raise EngineError("policy operators' library missing: %s — build it with `python -m contracts_amd.build` (needs hipcc; there is "
+                          "no CPU fallback)" % POLICY_LIB_PATH)
+    import torch  # noqa: F401 — one HIP runtime for both, see load()
+    L = C.CDLL(POLICY_LIB_PATH)
+    for name, (res, args) in POLICY_EXPORTS.items():
+        fn = getattr(L, name)
+        fn.restype = res
+        fn.argtypes = args
+    if L.ce_policy_abi_version() != POLICY_ABI_VERSION:
+        raise EngineError("policy operators: ABI version mismatch")
+    _policy = L
+    return L
+
+
+def check_policy(rc, what):
+    if rc != 0:
+        raise EngineError("%s failed: %s (%d) %s" % (what, ERRORS.get(rc, "?"), rc, (load_policy().ce_policy_error() or b"").decode()))
 
 
 def check(rc, handle=None, what=""):

@@ -26,6 +26,15 @@ FLAGS = ["-O3", "--offload-arch=gfx950", "-std=c++17", "-fPIC", "-ffp-contract=o
          "-fno-gpu-rdc", "-Wall", "-Wno-unused-function", "-mllvm", "-amdgpu-kernarg-preload-count=16"]
 
 
+# The policy operators (include/contracts_policy.h) are a library of their own: the engine's stays the one its records describe.
+# No packed float arithmetic: some of its forms have given wrong results on this hardware.
+POLICY_LIB = os.path.join(CSRC, "libcontracts_policy.so")
+POLICY_SOURCES = ["cp_api.hip", "cp_scan.hip", "cp_scan_grad.hip", "cp_advantage.hip", "cp_logits.hip"]
+POLICY_HEADERS = ["cp_common.h", os.path.join("..", "..", "include", "contracts_policy.h"), os.path.join("..", "..", "include", "contracts_engine.h")]
+POLICY_FLAGS = ["-O3", "--offload-arch=gfx950", "-std=c++17", "-fPIC", "-fno-fast-math", "-fno-gpu-rdc", "-Wall",
+                "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops", "-mllvm", "-amdgpu-kernarg-preload-count=16"]
+
+
 def hipcc():
     exe = shutil.which("hipcc") or "/opt/rocm/bin/hipcc"
     if not os.path.exists(exe):
@@ -68,6 +77,11 @@ def fingerprint():
     return {"files": files, "flags": FLAGS}
 
 
+def policy_fingerprint():
+    """what the policy library is a function of"""
+    return {"files": {s: _sha16(os.path.join(CSRC, s)) for s in POLICY_SOURCES + POLICY_HEADERS}, "flags": POLICY_FLAGS}
+
+
 def kernels_sha16(fp=None):
     """one hash for "the kernel sources this library was built from": every source / header by content + the flags"""
     fp = fp or fingerprint()
@@ -101,7 +115,48 @@ def needs_build():
     rec = last_build()
     if not os.path.exists(LIB) or rec is None or not os.path.exists(pydict_path()):
         return True
+    if policy_needs_build():
+        return True
     return rec.get("fingerprint") != fingerprint() or rec.get("lib_sha16") != _sha16(LIB)
+
+
+POLICY_INFO = os.path.join(CSRC, "build_info_policy.json")  # (git-ignored, like the library)
+
+
+def policy_needs_build():
+    """needs_build for the policy library: its own record, by content"""
+    try:
+        with open(POLICY_INFO) as f:
+            rec = json.load(f)
+    except (OSError, ValueError):
+        return True
+    return not os.path.exists(POLICY_LIB) or rec.get("fingerprint") != policy_fingerprint() or rec.get("lib_sha16") != _sha16(POLICY_LIB)
+
+
+def build_policy(verbose=False):
+    _compile(POLICY_SOURCES, POLICY_FLAGS, POLICY_LIB, "", verbose)
+    with open(POLICY_INFO, "w") as f:
+        json.dump({"fingerprint": policy_fingerprint(), "lib_sha16": _sha16(POLICY_LIB), "offload_arch": "gfx950",
+                   "built_at": time.strftime("%Y-%m-%dT%H:%M:%SZ", time.gmtime())}, f, indent=1)
+    return POLICY_LIB
+
+
+def _compile(sources, flags, lib, suffix, verbose):
+    objs, procs = [], []
+    for src in sources:  # the translation units compile side by side
+        obj = os.path.join(CSRC, src.replace(".hip", suffix + ".o"))
+        cmd = [hipcc()] + flags + ["-c", os.path.join(CSRC, src), "-o", obj]
+        if verbose:
+            print(" ".join(cmd))
+        procs.append((cmd, subprocess.Popen(cmd)))
+        objs.append(obj)
+    failed = [cmd for cmd, proc in procs if proc.wait() != 0]
+    if failed:
+        raise subprocess.CalledProcessError(1, failed[0])
+    cmd = [hipcc(), "--offload-arch=gfx950", "-shared", "-fPIC", "-o", lib] + objs
+    if verbose:
+        print(" ".join(cmd))
+    subprocess.check_call(cmd)
 
 
 def build(force=False, verbose=False):
@@ -119,23 +174,10 @@ def build(force=False, verbose=False):
     if not force and not needs_build():
         return LIB
     t0 = time.time()
-    objs, procs = [], []
-    for src in SOURCES:  # the translation units compile side by side
-        obj = os.path.join(CSRC, src.replace(".hip", suffix + ".o"))
-        cmd = [hipcc()] + flags + ["-c", os.path.join(CSRC, src), "-o", obj]
-        if verbose:
-            print(" ".join(cmd))
-        procs.append((cmd, subprocess.Popen(cmd)))
-        objs.append(obj)
-    failed = [cmd for cmd, proc in procs if proc.wait() != 0]
-    if failed:
-        raise subprocess.CalledProcessError(1, failed[0])
-    cmd = [hipcc(), "--offload-arch=gfx950", "-shared", "-fPIC", "-o", lib] + objs
-    if verbose:
-        print(" ".join(cmd))
-    subprocess.check_call(cmd)
+    _compile(SOURCES, flags, lib, suffix, verbose)
     if lib == LIB:
         build_pydict(verbose)
+        build_policy(verbose)
         ver = subprocess.run([hipcc(), "--version"], capture_output=True, text=True).stdout.strip().splitlines()
         with open(INFO, "w") as f:
             head, dirty = git_state()

@@ -1,0 +1,333 @@
+// cp_api.hip — host side of the C-ABI in include/contracts_policy.h: checks every argument before anything is launched, names
+// the launch's shape, never throws, never allocates and never synchronises.
+#include <cmath>
+#include <cstdarg>
+#include <cstdio>
+
+#include "cp_common.h"
+
+namespace {
+
+thread_local char g_error[256] = "";
+
+int refuse(const char* what, ...) {
+  va_list ap;
+  va_start(ap, what);
+  vsnprintf(g_error, sizeof(g_error), what, ap);
+  va_end(ap);
+  return CE_EINVAL;
+}
+
+// The call's device while it is made; the caller's own is current again afterwards.
+struct OnDevice {
+  int before = -1;
+  hipError_t err;
+  explicit OnDevice(int device) {
+    err = hipGetDevice(&before);
+    if (err == hipSuccess && before != device) err = hipSetDevice(device);
+    else if (err == hipSuccess) before = -1;
+  }
+  ~OnDevice() {
+    if (before >= 0) (void)hipSetDevice(before);
+  }
+};
+
+int launched(hipError_t e, const char* what) {
+  if (e == hipSuccess) return CE_OK;
+  snprintf(g_error, sizeof(g_error), "%s: %s", what, hipGetErrorString(e));
+  return CE_ENODEV;
+}
+
+uint64_t size_of(uint32_t t) { return t == CE_U8 ? 1 : t == CE_BF16 || t == CE_F16 ? 2 : t == CE_F32 || t == CE_I32 ? 4 : 8; }
+bool half_or_float(uint32_t t) { return t == CE_F32 || t == CE_BF16 || t == CE_F16; }
+bool aligned(const void* p, uint64_t to) { return (uintptr_t)p % to == 0; }
+
+constexpr uint64_t kMost = 1ull << 28;   // columns of a scan: a launch has fewer than 2^32 threads
+constexpr uint64_t kMostRows = 1ull << 23;  // rows of scores, for the same reason
+constexpr uint64_t kFar = 1ull << 46;    // elements: products of sizes stay far inside 64 bits
+
+// ---- the scan ---------------------------------------------------------------------------------------------------------------------
+struct Plan {
+  cp::ScanParams p;
+  int mode, vec;
+};
+
+bool divides(int vec, std::initializer_list<int64_t> strides) {
+  for (int64_t s : strides)
+    if (s % vec) return false;
+  return true;
+}
+
+int check_scan(const ce_scan* s) {
+  if (!s) return refuse("null ce_scan");
+  if (s->abi_version != CE_POLICY_ABI_VERSION) return refuse("ce_scan.abi_version is %u, this library is %d", s->abi_version, CE_POLICY_ABI_VERSION);
+  if (!half_or_float(s->dtype) && s->dtype != CE_F64) return refuse("linear_scan: x must be float, bfloat16, half or double");
+  if (s->gate && s->gate_dtype != s->dtype && !(s->gate_dtype == CE_F32 && half_or_float(s->dtype)))
+    return refuse("linear_scan: the gate must be of x's type or float");
+  if (s->flags & ~CE_SCAN_REVERSE) return refuse("linear_scan: unknown flags %#x", s->flags);
+  if (s->channels && s->gate && (s->heads == 0 || s->heads > s->channels || s->channels % s->heads)) return refuse("linear_scan: heads must divide channels");
+  if (s->channels > kMost || s->rows > kMost || s->rows * s->channels > kMost) return refuse("linear_scan: more than 2^28 columns (rows x channels)");
+  if (s->steps > kFar || (s->steps && s->rows * s->channels > kFar / s->steps)) return refuse("linear_scan: too many elements");
+  if (s->rows * s->channels == 0) return CE_OK;
+  if (s->steps && (!s->x || !s->y)) return refuse("linear_scan: null x or y");
+  if (!s->gate && !std::isfinite(s->decay)) return refuse("linear_scan: decay must be finite");
+  const uint64_t b = size_of(s->dtype), a = s->dtype == CE_F64 ? 8 : 4;
+  if (!aligned(s->x, b) || !aligned(s->y, b) || !aligned(s->state, a) || !aligned(s->last, a) || !aligned(s->saved, 4) || (s->gate && !aligned(s->gate, size_of(s->gate_dtype))))
+    return refuse("linear_scan: a pointer is not aligned to its type");
+  return CE_OK;
+}
+
+// Chunks of the time axis: enough blocks of 4 waves for the chip where the columns alone are too few, and no chunk under 256 steps,
+// where folding the chunks before it would cost as much as the chunk.
+void split(cp::ScanParams& p, uint64_t blocks) {
+  p.chunks = 1;
+  uint64_t want = blocks >= 512 ? 1 : 512 / blocks;
+  const uint64_t most = p.T / 256;
+  if (want > most) want = most;
+  if (want > 64) want = 64;
+  if (want > 1) {
+    const uint64_t tile = 4 * CE_SCAN_SAVED_STEPS, each = ((p.T + want - 1) / want + tile - 1) / tile * tile;
+    p.chunk = each;
+    p.chunks = (uint32_t)((p.T + each - 1) / each);
+  }
+}
+
+void plan_scan(const ce_scan* s, const ce_scan_grad* g, Plan* o) {
+  cp::ScanParams& p = o->p;
+  p = cp::ScanParams();
+  const uint64_t T = s->steps, E = s->rows, C = s->channels, H = s->gate ? s->heads : C;
+  o->mode = !s->gate ? cp::kGateConst : H == C ? cp::kGateChannel : cp::kGateHead;
+  const uint64_t head = C / H, b = size_of(s->dtype), gb = size_of(s->gate_dtype);
+  // pairs of channels as one access: a lane of one 2-byte channel would move half a cache line a wave
+  int vec = b == 2 ? 2 : 1;
+  if (vec == 2) {
+    bool ok = C % 2 == 0 && divides(2, {s->x_step, s->x_row}) && aligned(s->x, 2 * b) && aligned(s->y, 2 * b);
+    if (o->mode == cp::kGateChannel) ok = ok && divides(2, {s->gate_step, s->gate_row}) && aligned(s->gate, 2 * gb);
+    if (o->mode == cp::kGateHead) ok = ok && head % 2 == 0;
+    if (g) ok = ok && aligned(g->dy, 2 * b) && aligned(g->dx, 2 * b) && (o->mode != cp::kGateChannel || aligned(g->dgate, 2 * gb));
+    if (!ok) vec = 1;
+  }
+  o->vec = vec;
+  const bool rev = s->flags & CE_SCAN_REVERSE;
+  const int64_t sign = rev ? -1 : 1, off = rev && T ? (int64_t)T - 1 : 0;
+  p.T = T;
+  p.cols = (uint32_t)(E * C / vec);
+  p.row_cols = (uint32_t)(C / vec);
+  p.head = (uint32_t)head;
+  p.heads = (uint32_t)H;
+  p.cut_off = rev ? 0 : -1;
+  p.x_step = sign * s->x_step;
+  p.x_row = s->x_row;
+  p.gate_step = sign * s->gate_step;
+  p.gate_row = s->gate_row;
+  p.done_step = sign * s->done_step;
+  p.done_row = s->done_row;
+  p.y_step = sign * (int64_t)(E * C);
+  p.dgate_step = sign * (int64_t)(E * H);
+  p.decay = s->decay;
+  auto from = [&](const void* q, int64_t step, uint64_t bytes) -> char* { return q ? (char*)q + off * step * (int64_t)bytes : nullptr; };
+  p.x = from(s->x, s->x_step, b);
+  p.gate = from(s->gate, s->gate_step, gb);
+  p.done = (const uint8_t*)from(s->done, s->done_step, 1);
+  p.state = s->state;
+  p.y = from(s->y, (int64_t)(E * C), b);
+  p.last = s->last;
+  p.saved = s->saved;
+  p.slabs = 1;
+  uint64_t blocks = ((uint64_t)p.cols + 63) / 64;
+  if (g) {
+    p.dy = from(g->dy, (int64_t)(E * C), b);
+    p.dlast = g->dlast;
+    p.dx = from(g->dx, (int64_t)(E * C), b);
+    p.dgate = from(g->dgate, (int64_t)(E * H), gb);
+    p.dstate = g->dstate;
+    if (o->mode == cp::kGateHead) {
+      const uint64_t lanes = head / vec;
+      uint64_t seg = 1;
+      while (seg < lanes && seg < 64) seg *= 2;
+      if (lanes > 64) seg = (lanes + 63) / 64 * 64;
+      p.seg = (uint32_t)seg;
+      p.slabs = seg > 64 ? (uint32_t)(seg / 64) : 1;
+      blocks = (E * H * seg + 63) / 64;
+    }
+  }
+  split(p, blocks ? blocks : 1);
+  // the chunks of a split time axis read the incoming state while the last of them writes the outgoing one
+  if (!g && s->last && s->last == s->state) p.chunks = 1;
+  if (p.chunks == 1) p.chunk = T;
+}
+
+uint64_t part_bytes(const Plan& o, uint32_t dtype) {
+  return o.p.chunks > 1 ? (uint64_t)(o.p.chunks - 1) * 2 * o.p.cols * o.vec * (dtype == CE_F64 ? 8 : 4) : 0;
+}
+uint64_t slab_bytes(const Plan& o, const ce_scan* s, const ce_scan_grad* g) {
+  return g->dgate && o.p.slabs > 1 ? (uint64_t)o.p.slabs * s->steps * s->rows * s->heads * 4 : 0;
+}
+
+}  // namespace
+
+extern "C" int ce_policy_abi_version(void) { return CE_POLICY_ABI_VERSION; }
+extern "C" const char* ce_policy_error(void) { return g_error; }
+
+extern "C" int ce_linear_scan_workspace(const ce_scan* s, uint64_t* bytes) {
+  if (!bytes) return refuse("null bytes");
+  if (int rc = check_scan(s)) return rc;
+  *bytes = 0;
+  if (s->rows * s->channels == 0) return CE_OK;
+  Plan o;
+  plan_scan(s, nullptr, &o);
+  *bytes = part_bytes(o, s->dtype);
+  return CE_OK;
+}
+
+extern "C" int ce_linear_scan(const ce_scan* s, void* stream) {
+  if (int rc = check_scan(s)) return rc;
+  if (s->saved && s->dtype == CE_F64) return refuse("linear_scan: double has no backward pass");
+  if (s->rows * s->channels == 0 || (s->steps == 0 && !s->last)) return CE_OK;
+  Plan o;
+  plan_scan(s, nullptr, &o);
+  const uint64_t need = part_bytes(o, s->dtype);
+  if (need && (!s->workspace || s->workspace_bytes < need || !aligned(s->workspace, 8)))
+    return refuse("linear_scan: workspace of %llu bytes needed, %llu given", (unsigned long long)need, (unsigned long long)(s->workspace ? s->workspace_bytes : 0));
+  o.p.part = s->workspace;
+  OnDevice dev(s->device);
+  if (dev.err != hipSuccess) return launched(dev.err, "linear_scan: device");
+  return launched(cp::launch_scan(o.p, s->dtype, s->gate ? s->gate_dtype : s->dtype, o.mode, o.vec, (hipStream_t)stream), "linear_scan");
+}
+
+static int check_scan_grad(const ce_scan* s, const ce_scan_grad* g) {
+  if (!g) return refuse("null ce_scan_grad");
+  if (!s) return refuse("null ce_scan");
+  ce_scan t = *s;
+  if (!t.y) t.y = g->dx ? g->dx : const_cast<void*>(t.x);  // the backward pass reads no y
+  if (int rc = check_scan(&t)) return rc;
+  if (s->dtype == CE_F64) return refuse("linear_scan: double has no backward pass");
+  if (s->rows * s->channels == 0) return CE_OK;
+  if (s->steps && !s->saved) return refuse("linear_scan_backward: the forward call's saved states are missing");
+  const uint64_t b = size_of(s->dtype);
+  if (!aligned(g->dy, b) || !aligned(g->dx, b) || !aligned(g->dlast, 4) || !aligned(g->dstate, 4) || (s->gate && !aligned(g->dgate, size_of(s->gate_dtype))))
+    return refuse("linear_scan_backward: a pointer is not aligned to its type");
+  if (g->dgate && !s->gate) return refuse("linear_scan_backward: a constant gate has no gradient");
+  return CE_OK;
+}
+
+extern "C" int ce_linear_scan_backward_workspace(const ce_scan* s, const ce_scan_grad* g, uint64_t* bytes) {
+  if (!bytes) return refuse("null bytes");
+  if (int rc = check_scan_grad(s, g)) return rc;
+  *bytes = 0;
+  if (s->rows * s->channels == 0) return CE_OK;
+  Plan o;
+  plan_scan(s, g, &o);
+  *bytes = part_bytes(o, s->dtype) + slab_bytes(o, s, g);
+  return CE_OK;
+}
+
+extern "C" int ce_linear_scan_backward(const ce_scan* s, const ce_scan_grad* g, void* stream) {
+  if (int rc = check_scan_grad(s, g)) return rc;
+  if (s->rows * s->channels == 0) return CE_OK;
+  Plan o;
+  plan_scan(s, g, &o);
+  const uint64_t part = part_bytes(o, s->dtype), need = part + slab_bytes(o, s, g);
+  if (need && (!s->workspace || s->workspace_bytes < need || !aligned(s->workspace, 8)))
+    return refuse("linear_scan_backward: workspace of %llu bytes needed, %llu given", (unsigned long long)need, (unsigned long long)(s->workspace ? s->workspace_bytes : 0));
+  o.p.part = s->workspace;
+  o.p.slab = s->workspace ? (float*)((char*)s->workspace + part) : nullptr;
+  OnDevice dev(s->device);
+  if (dev.err != hipSuccess) return launched(dev.err, "linear_scan_backward: device");
+  return launched(cp::launch_scan_grad(o.p, s->dtype, s->gate ? s->gate_dtype : s->dtype, o.mode, o.vec, (hipStream_t)stream), "linear_scan_backward");
+}
+
+// ---- advantages -------------------------------------------------------------------------------------------------------------------
+extern "C" int ce_advantages(const ce_advantage* a, void* stream) {
+  if (!a) return refuse("null ce_advantage");
+  if (a->abi_version != CE_POLICY_ABI_VERSION) return refuse("ce_advantage.abi_version is %u, this library is %d", a->abi_version, CE_POLICY_ABI_VERSION);
+  if (a->reward_dtype != CE_F64 && a->reward_dtype != CE_F32) return refuse("advantages: reward must be double or float");
+  if (!half_or_float(a->value_dtype)) return refuse("advantages: value must be float, bfloat16 or half");
+  if (a->flags & ~CE_ADV_DONE_PER_AGENT) return refuse("advantages: unknown flags %#x", a->flags);
+  if (!std::isfinite(a->gamma) || !std::isfinite(a->lam)) return refuse("advantages: gamma and lam must be finite");
+  if (a->rows > kMost || a->agents > kMost || a->rows * a->agents > kMost) return refuse("advantages: more than 2^28 columns (rows x agents)");
+  if (a->planes > kFar || (a->planes && a->rows * a->agents > kFar / a->planes)) return refuse("advantages: too many elements");
+  if (a->planes * a->rows * a->agents == 0) return CE_OK;
+  if (a->first_plane >= a->planes) return refuse("advantages: first_plane out of range");
+  if (!a->reward || !a->value || (!a->advantage && !a->ret)) return refuse("advantages: null reward, value or outputs");
+  if (!aligned(a->reward, size_of(a->reward_dtype)) || !aligned(a->value, size_of(a->value_dtype)) || !aligned(a->last_value, size_of(a->value_dtype)) ||
+      !aligned(a->advantage, 4) || !aligned(a->ret, 4))
+    return refuse("advantages: a pointer is not aligned to its type");
+  OnDevice dev(a->device);
+  if (dev.err != hipSuccess) return launched(dev.err, "advantages: device");
+  return launched(cp::launch_advantages(*a, (hipStream_t)stream), "advantages");
+}
+
+// ---- scores -----------------------------------------------------------------------------------------------------------------------
+static int check_logits(const ce_logits* s) {
+  if (!s) return refuse("null ce_logits");
+  if (s->abi_version != CE_POLICY_ABI_VERSION) return refuse("ce_logits.abi_version is %u, this library is %d", s->abi_version, CE_POLICY_ABI_VERSION);
+  if (!half_or_float(s->dtype)) return refuse("process_logits: logits must be float, bfloat16 or half");
+  if (s->out_dtype != s->dtype && s->out_dtype != CE_F32) return refuse("process_logits: the output must be of the logits' type or float");
+  if (s->rows > kMostRows) return refuse("process_logits: more than 2^23 rows");
+  if (s->vocab > (1ull << 28)) return refuse("process_logits: more than 2^28 tokens");
+  if (s->history > (1ull << 31) - 1) return refuse("process_logits: a history of more than 2^31 - 1 tokens");
+  if (s->rows * s->vocab == 0) return CE_OK;
+  if (!s->logits) return refuse("process_logits: null logits");
+  if (!aligned(s->logits, size_of(s->dtype)) || !aligned(s->out, size_of(s->out_dtype))) return refuse("process_logits: a pointer is not aligned to its type");
+  if (s->tokens) {
+    if (s->token_dtype != CE_U8 && s->token_dtype != CE_I32 && s->token_dtype != CE_I64) return refuse("process_logits: tokens must be uint8, int32 or int64");
+    if (!aligned(s->tokens, size_of(s->token_dtype))) return refuse("process_logits: tokens are not aligned to their type");
+    if (!s->repetition && !(s->repetition_all > 0 && std::isfinite(s->repetition_all))) return refuse("process_logits: repetition must be positive and finite");
+    if ((!s->presence && !std::isfinite(s->presence_all)) || (!s->frequency && !std::isfinite(s->frequency_all))) return refuse("process_logits: presence and frequency must be finite");
+  } else if (s->lengths || s->prompt_lengths) {
+    return refuse("process_logits: lengths without tokens");
+  }
+  if (s->bias) {
+    if (s->bias_dtype != CE_F32 && s->bias_dtype != s->dtype) return refuse("process_logits: bias must be float or of the logits' type");
+    if (!aligned(s->bias, size_of(s->bias_dtype))) return refuse("process_logits: bias is not aligned to its type");
+    if (s->bias_rows == 0 || s->rows % s->bias_rows) return refuse("process_logits: bias_rows must divide the rows");
+  }
+  if (s->mask) {
+    if (s->mask_dtype != CE_U8 && s->mask_dtype != CE_I32) return refuse("process_logits: a mask is uint8 tokens or int32 words");
+    if (!aligned(s->mask, size_of(s->mask_dtype))) return refuse("process_logits: the mask is not aligned to its type");
+    if (s->mask_rows == 0 || s->mask_rows > 0x7fffffffu || (!s->mask_index && s->rows % s->mask_rows)) return refuse("process_logits: mask_rows must divide the rows, or an index be given");
+  } else if (s->mask_index) {
+    return refuse("process_logits: mask_index without a mask");
+  }
+  return CE_OK;
+}
+
+extern "C" int ce_process_logits(const ce_logits* s, void* stream) {
+  if (int rc = check_logits(s)) return rc;
+  if (s->rows * s->vocab == 0) return CE_OK;
+  if (!s->out) return refuse("process_logits: null output");
+  if (s->out == s->logits && (s->out_dtype != s->dtype || s->out_row != s->logits_row)) return refuse("process_logits: in place needs one type and one stride");
+  OnDevice dev(s->device);
+  if (dev.err != hipSuccess) return launched(dev.err, "process_logits: device");
+  return launched(cp::launch_logits(*s, (hipStream_t)stream), "process_logits");
+}
+
+static int check_logits_grad(const ce_logits* s, const ce_logits_grad* g) {
+  if (!g) return refuse("null ce_logits_grad");
+  if (int rc = check_logits(s)) return rc;
+  if (s->rows * s->vocab == 0) return CE_OK;
+  if (!g->dout) return refuse("process_logits_backward: null dout");
+  if (g->dbias && !s->bias) return refuse("process_logits_backward: dbias without a bias");
+  if (!aligned(g->dout, size_of(s->out_dtype)) || !aligned(g->dlogits, size_of(s->dtype)) || (g->dbias && !aligned(g->dbias, size_of(s->bias_dtype))))
+    return refuse("process_logits_backward: a pointer is not aligned to its type");
+  return CE_OK;
+}
+
+extern "C" int ce_process_logits_backward_workspace(const ce_logits* s, const ce_logits_grad* g, uint64_t* bytes) {
+  if (!bytes) return refuse("null bytes");
+  if (int rc = check_logits_grad(s, g)) return rc;
+  *bytes = s->rows * s->vocab ? cp::logits_grad_workspace(*s, *g) : 0;
+  return CE_OK;
+}
+
+extern "C" int ce_process_logits_backward(const ce_logits* s, const ce_logits_grad* g, void* stream) {
+  if (int rc = check_logits_grad(s, g)) return rc;
+  if (s->rows * s->vocab == 0 || (!g->dlogits && !g->dbias)) return CE_OK;
+  const uint64_t need = cp::logits_grad_workspace(*s, *g);
+  if (need && (!s->workspace || s->workspace_bytes < need || !aligned(s->workspace, 4)))
+    return refuse("process_logits_backward: workspace of %llu bytes needed, %llu given", (unsigned long long)need, (unsigned long long)(s->workspace ? s->workspace_bytes : 0));
+  OnDevice dev(s->device);
+  if (dev.err != hipSuccess) return launched(dev.err, "process_logits_backward: device");
+  return launched(cp::launch_logits_grad(*s, *g, (hipStream_t)stream), "process_logits_backward");
+}

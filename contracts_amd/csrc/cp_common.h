@@ -1,0 +1,73 @@
+// cp_common.h — what the policy operators' kernels share: element types, the fold of a recurrence, launch parameters.
+#pragma once
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "../../include/contracts_policy.h"
+
+namespace cp {
+
+typedef __bf16 bf16;
+typedef _Float16 f16;
+constexpr int kWave = 64;
+
+// A lane's run of VEC neighbouring elements, moved as one access (the host picks VEC by the alignment of every array involved).
+template <class T, int N> struct alignas(sizeof(T) * N) Pack {
+  T v[N];
+};
+template <class T, int N> __device__ __forceinline__ Pack<T, N> load(const T* p) { return *reinterpret_cast<const Pack<T, N>*>(p); }
+template <class T, int N> __device__ __forceinline__ void store(T* p, const Pack<T, N>& v) { *reinterpret_cast<Pack<T, N>*>(p) = v; }
+
+template <class T> struct AccOf { typedef float type; };
+template <> struct AccOf<double> { typedef double type; };
+
+// One step of the recurrence.  A gate of 0 (done flags arrive as one) forgets the state, infinities and NaN included, where a plain
+// product would give NaN.
+template <class A> __device__ __forceinline__ A step(A a, A h, A x) { return a == A(0) ? x : __builtin_fma(a, h, x); }
+template <> __device__ __forceinline__ float step(float a, float h, float x) { return a == 0.f ? x : __builtin_fmaf(a, h, x); }
+
+// A run of steps as a map of the state before it: h -> P h + H, P the product of its gates.  A zero state takes no part, so
+// that a product past the type's range (gates over 1) does not turn it into NaN.
+template <class A> __device__ __forceinline__ A apply(A P, A H, A h) { return h == A(0) ? H : step(P, h, H); }
+
+struct ScanParams {
+  uint64_t T;
+  uint32_t cols;      // E * C / VEC: columns of VEC channels
+  uint32_t row_cols;  // C / VEC
+  uint64_t chunk;     // steps of one block (a multiple of every tile), T where the time axis is not split
+  uint32_t chunks;
+  uint32_t head;      // channels under one gate
+  int32_t cut_off;    // the flag that cuts the state ahead of processed step i is done[i + cut_off]
+  int64_t x_step, x_row, gate_step, gate_row, done_step, done_row, y_step;  // in processing order (steps may be negative)
+  double decay;
+  const void* x;
+  const void* gate;
+  const uint8_t* done;
+  const void* state;
+  void* y;
+  void* last;
+  float* saved;
+  void* part;         // [chunks][2][E * C]: product and state of each chunk
+  // backward pass
+  const void* dy;
+  const void* dlast;
+  void* dx;
+  void* dgate;
+  void* dstate;
+  int64_t dgate_step;
+  uint32_t heads;
+  uint32_t seg;       // lanes of one head's segment (padded); 0: a gate for each channel
+  uint32_t slabs;     // partial sums a head's gradient is made of
+  float* slab;        // [slabs][T][E][H] where slabs > 1
+};
+
+enum GateMode { kGateConst = 0, kGateChannel = 1, kGateHead = 2 };
+
+hipError_t launch_scan(const ScanParams& p, int dtype, int gate_dtype, int mode, int vec, hipStream_t stream);
+hipError_t launch_scan_grad(const ScanParams& p, int dtype, int gate_dtype, int mode, int vec, hipStream_t stream);
+hipError_t launch_advantages(const ce_advantage& a, hipStream_t stream);
+hipError_t launch_logits(const ce_logits& s, hipStream_t stream);
+hipError_t launch_logits_grad(const ce_logits& s, const ce_logits_grad& g, hipStream_t stream);
+uint64_t logits_grad_workspace(const ce_logits& s, const ce_logits_grad& g);
+
+}  // namespace cp

@@ -1,0 +1,178 @@
+// cp_scan.hip — the gated linear recurrence h_t = a_t h_{t-1} + x_t along the time axis of [T][E][C] planes (ce_linear_scan).
+//
+// A run of steps is a map h -> P h + H (P the product of its gates, H its state from zero), and runs compose, so the time
+// axis can be cut wherever that helps.  A block takes 64 lanes x VEC neighbouring channels (one coalesced access a step) and W
+// waves, each W-th run of kSteps steps to a wave: a wave takes its run into registers, reduces it to (P, H), the waves exchange
+// these through LDS, and each walks its run once more from the state it then knows — the data are read once, and the walk that
+// writes y is the plain recurrence in float, whatever the cut.  Where E * C gives too few blocks for the 256 CUs, the time
+// axis is cut into chunks too: a first launch reduces every chunk to (P, H), and a chunk of the second folds those before it.
+// Bound by HBM: reads x and a, writes y, 2 flops an element.
+#include "cp_common.h"
+
+namespace cp {
+
+constexpr int kSteps = CE_SCAN_SAVED_STEPS;
+
+template <class X, class G, int MODE, int VEC> struct Tile {
+  static constexpr int GV = MODE == kGateChannel ? VEC : 1;
+  Pack<X, VEC> x[kSteps];
+  Pack<G, GV> g[MODE == kGateConst ? 1 : kSteps];
+  uint8_t d[kSteps];
+};
+
+template <class X, class G, int MODE, int VEC, int W, bool REDUCE> __global__ __launch_bounds__(kWave * W) void k_scan(ScanParams p) {
+  typedef typename AccOf<X>::type A;
+  typedef Tile<X, G, MODE, VEC> TileT;
+  __shared__ A fold[W > 1 ? 2 : 1][W][2][VEC][kWave];
+  const int lane = threadIdx.x & 63, w = W > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : 0;
+  const uint32_t col = blockIdx.x * kWave + lane;
+  const bool live = col < p.cols;
+  const uint32_t colc = live ? col : p.cols - 1;  // lanes past the end read a column that exists and write nothing
+  const uint32_t e = colc / p.row_cols, c = (colc % p.row_cols) * VEC;
+  const X* x = (const X*)p.x + (int64_t)e * p.x_row + c;
+  const G* gate = (const G*)p.gate;
+  if (MODE != kGateConst) gate += (int64_t)e * p.gate_row + (MODE == kGateHead ? c / p.head : c);
+  const uint8_t* done = p.done ? p.done + (int64_t)e * p.done_row + (int64_t)p.cut_off * p.done_step : nullptr;
+  const uint64_t ch = (uint64_t)colc * VEC;  // index in the dense [E][C]
+  X* y = (X*)p.y + ch;
+  const uint64_t i0 = blockIdx.y * p.chunk, i1 = i0 + p.chunk < p.T ? i0 + p.chunk : p.T;
+
+  A h[VEC];
+#pragma unroll
+  for (int v = 0; v < VEC; ++v) h[v] = A(0);
+  if (!REDUCE) {
+    if (p.state)
+#pragma unroll
+      for (int v = 0; v < VEC; ++v) h[v] = ((const A*)p.state)[ch + v];
+    const uint64_t EC = (uint64_t)p.cols * VEC;
+    const A* part = (const A*)p.part + ch;
+    for (uint32_t k = 0; k < blockIdx.y; ++k)
+#pragma unroll
+      for (int v = 0; v < VEC; ++v) h[v] = apply(part[(uint64_t)k * 2 * EC + v], part[((uint64_t)k * 2 + 1) * EC + v], h[v]);
+  }
+  A P[VEC];  // REDUCE: the chunk's product so far
+#pragma unroll
+  for (int v = 0; v < VEC; ++v) P[v] = A(1);
+
+  auto take = [&](TileT& t, uint64_t i) {
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) {
+      const uint64_t at = i + s;
+      if (at < i1) {
+        t.x[s] = load<X, VEC>(x + (int64_t)at * p.x_step);
+        if (MODE != kGateConst) t.g[MODE == kGateConst ? 0 : s] = load<G, TileT::GV>(gate + (int64_t)at * p.gate_step);
+        const uint64_t flag = at + p.cut_off;  // wraps past T at the first step of a forward scan
+        t.d[s] = done && flag < p.T ? done[(int64_t)at * p.done_step] : 0;
+      }
+    }
+  };
+  auto gate_of = [&](const TileT& t, int s, int v) -> A {
+    const A a = MODE == kGateConst ? A(p.decay) : A((typename AccOf<G>::type)t.g[MODE == kGateConst ? 0 : s].v[MODE == kGateChannel ? v : 0]);
+    return t.d[s] ? A(0) : a;
+  };
+
+  int buf = 0;
+  for (uint64_t tile = i0; tile < i1; tile += (uint64_t)W * kSteps) {
+    const uint64_t i = tile + (uint64_t)w * kSteps;
+    TileT t;
+    take(t, i);
+    if (W > 1 || REDUCE) {
+      A rp[VEC], rh[VEC];
+#pragma unroll
+      for (int v = 0; v < VEC; ++v) rp[v] = A(1), rh[v] = A(0);
+#pragma unroll
+      for (int s = 0; s < kSteps; ++s)
+        if (i + s < i1)
+#pragma unroll
+          for (int v = 0; v < VEC; ++v) {
+            const A a = gate_of(t, s, v);
+            rp[v] *= a;
+            rh[v] = step(a, rh[v], A(t.x[s].v[v]));
+          }
+#pragma unroll
+      for (int v = 0; v < VEC; ++v) fold[buf][w][0][v][lane] = rp[v], fold[buf][w][1][v][lane] = rh[v];
+      if (W > 1) __syncthreads();
+    }
+    A mine[VEC];
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) mine[v] = h[v];
+    if (W > 1 || REDUCE) {
+#pragma unroll
+      for (int k = 0; k < W; ++k) {
+        if (k == w)
+#pragma unroll
+          for (int v = 0; v < VEC; ++v) mine[v] = h[v];
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) {
+          h[v] = apply(fold[buf][k][0][v][lane], fold[buf][k][1][v][lane], h[v]);
+          if (REDUCE) P[v] *= fold[buf][k][0][v][lane];
+        }
+      }
+      buf ^= W > 1;
+    }
+    if (!REDUCE) {
+      if (p.saved && i < i1 && live)
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) p.saved[(i / kSteps) * (uint64_t)p.cols * VEC + ch + v] = (float)mine[v];
+#pragma unroll
+      for (int s = 0; s < kSteps; ++s)
+        if (i + s < i1) {
+          Pack<X, VEC> o;
+#pragma unroll
+          for (int v = 0; v < VEC; ++v) {
+            mine[v] = step(gate_of(t, s, v), mine[v], A(t.x[s].v[v]));
+            o.v[v] = (X)mine[v];
+          }
+          if (live) store(y + (int64_t)(i + s) * p.y_step, o);
+        }
+      if (W == 1)
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) h[v] = mine[v];
+    }
+  }
+  if (!live || w != 0) return;
+  if (REDUCE) {
+    A* part = (A*)p.part + (uint64_t)blockIdx.y * 2 * p.cols * VEC + ch;
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) part[v] = P[v], part[(uint64_t)p.cols * VEC + v] = h[v];
+  } else if (p.last && blockIdx.y + 1 == gridDim.y) {
+    // forward in time the flag of the last step closes the border behind it
+    const bool cut = done && p.cut_off < 0 && p.T > 0 && done[(int64_t)p.T * p.done_step];
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) ((A*)p.last)[ch + v] = cut ? A(0) : h[v];
+  }
+}
+
+template <class X, class G, int MODE, int VEC> static hipError_t go(const ScanParams& p, hipStream_t stream) {
+  const dim3 grid((p.cols + kWave - 1) / kWave, p.chunks);
+  if (p.T <= kSteps) {
+    k_scan<X, G, MODE, VEC, 1, false><<<grid, kWave, 0, stream>>>(p);
+    return hipGetLastError();
+  }
+  if (p.chunks > 1) {
+    k_scan<X, G, MODE, VEC, 4, true><<<dim3(grid.x, p.chunks - 1), 4 * kWave, 0, stream>>>(p);
+    if (hipError_t e = hipGetLastError()) return e;
+  }
+  k_scan<X, G, MODE, VEC, 4, false><<<grid, 4 * kWave, 0, stream>>>(p);
+  return hipGetLastError();
+}
+
+template <class X, class G, int MODE> static hipError_t vecs(const ScanParams& p, int vec, hipStream_t s) {
+  if (vec == 2) return go<X, G, MODE, 2>(p, s);
+  return go<X, G, MODE, 1>(p, s);
+}
+template <class X, class G> static hipError_t modes(const ScanParams& p, int mode, int vec, hipStream_t s) {
+  if (mode == kGateConst) return vecs<X, X, kGateConst>(p, vec, s);
+  if (mode == kGateChannel) return vecs<X, G, kGateChannel>(p, vec, s);
+  return vecs<X, G, kGateHead>(p, vec, s);
+}
+
+hipError_t launch_scan(const ScanParams& p, int dtype, int gate_dtype, int mode, int vec, hipStream_t s) {
+  const bool wide = gate_dtype == CE_F32;
+  if (dtype == CE_F32) return modes<float, float>(p, mode, vec, s);
+  if (dtype == CE_F64) return modes<double, double>(p, mode, vec, s);
+  if (dtype == CE_BF16) return wide ? modes<bf16, float>(p, mode, vec, s) : modes<bf16, bf16>(p, mode, vec, s);
+  return wide ? modes<f16, float>(p, mode, vec, s) : modes<f16, f16>(p, mode, vec, s);
+}
+
+}  // namespace cp

@@ -110,6 +110,44 @@ class Trajectory:
             self.tensors[f] = t
             setattr(self.c, f, t.data_ptr())
 
+    def _planes(self, op):
+        """reward planes [P, E, n] and the done planes that end their sums: the env's [P, E], selfdrive's cars' [P, E, n]"""
+        done = "done_agents" if self.env.kind == "selfdrive" else "done"
+        missing = [f for f in ("reward", done) if f not in self.tensors]
+        if missing:
+            raise ValueError("%s needs the trajectory's %s planes (alloc_trajectory(fields=...))" % (op, " and ".join(missing)))
+        return self.tensors["reward"], self.tensors[done]
+
+    def returns(self, gamma, last_value=None, first_plane=None):
+        """discounted returns G_t = r_t + gamma G_{t+1} over the ring's planes, float64 [P, E, n] in the planes' order, on torch's
+        current stream; nothing crosses the border behind a step that ended the episode.  last_value: float64 [E, n], what follows the last step (None: 0).
+        The oldest plane is the one the next rollout would write (a full ring) unless first_plane names it."""
+        import torch
+        from . import policy_ops
+        reward, done = self._planes("returns")
+        first = self.c.first_plane if first_plane is None else int(first_plane)
+        if not 0 <= first < self.P:
+            raise ValueError("first_plane out of range")
+        if last_value is not None and tuple(last_value.shape) != (self.E, self.n):
+            raise ValueError("last_value must be [E, n] = %s" % ((self.E, self.n),))
+        per_agent = done.dim() == 3
+        if per_agent:  # every car is a row of its own
+            reward, done = reward.view(self.P, self.E * self.n, 1), done.view(self.P, self.E * self.n)
+        out = torch.empty_like(reward)
+        state = None if last_value is None else last_value.reshape(reward.shape[1:]).to(reward)
+        for lo, hi in ((0, first), (first, self.P)):  # the newer part of a wrapped ring lies in front
+            if hi > lo:
+                _, state = policy_ops.linear_scan(reward[lo:hi], gamma, state=state, done=done[lo:hi], reverse=True, out=out[lo:hi])
+        return out.view(self.P, self.E, self.n)
+
+    def advantages(self, value, last_value=None, gamma=0.99, lam=0.95, first_plane=None, out=None):
+        """(advantage, return), float32 [P, E, n], of the ring's rewards under a critic's values (policy_ops.advantages): value [P, E, n] in
+        the planes' order, last_value [E, n] of the observation behind the newest plane; the ring's order as in `returns`"""
+        from . import policy_ops
+        reward, done = self._planes("advantages")
+        first = self.c.first_plane if first_plane is None else int(first_plane)
+        return policy_ops.advantages(reward, value, last_value, done, gamma=gamma, lam=lam, first_plane=first, out=out)
+
     def host(self, field):
         """host copy [P, E, ...]; obs comes back dense [P, E, n, 15, 15, 3]"""
         a = self.tensors[field].cpu().numpy()
@@ -237,6 +275,24 @@ class BatchedEnv:
         check(self._L.ce_step_policy(self._h, policy_ptr, m, int(env_begin), int(cnt), stream), self._h, "ce_step_policy")
 
     _POLICY_MODES = {"bytes": _lib.POLICY_BYTES_MOD, "argmax": _lib.POLICY_ARGMAX_F32, "ahead_noise": _lib.POLICY_AHEAD_NOISE}
+
+    def shape_scores(self, scores, out=None, **shaping):
+        """scores [E, n, |A|] shaped ahead of step_policy_device(.., "argmax") by policy_ops.process_logits — masks of allowed actions, biases,
+        penalties for repeated actions (tokens=[E, n, L] past action ids) — as the float32 plane that mode reads: `out`
+        (float32 [E, n, |A|], may be `scores`) or a new one; on torch's current stream, which the step's stream has to follow"""
+        import torch
+        from . import policy_ops
+        if self.num_actions is None:
+            raise ValueError("shape_scores: %r has no discrete actions" % (self.kind,))
+        shape = (self.E, self.n, self.num_actions)
+        if tuple(scores.shape) != shape:
+            raise ValueError("shape_scores: scores must be [E, n, |A|] = %s, got %s" % (shape, tuple(scores.shape)))
+        if out is None:
+            out = torch.empty(shape, dtype=torch.float32, device=scores.device)
+        elif out.dtype != torch.float32 or not out.is_contiguous():
+            raise ValueError("shape_scores: out must be a dense float32 tensor")
+        with torch.no_grad():
+            return policy_ops.process_logits(scores, out=out, **shaping)
 
     def step_policy_sliced(self, policy_ptr, mode, streams=None, num_slices=None):
         """ce_step_policy_sliced: one policy step of ALL envs as env slices on `streams` (raw hipStream_t handles), the launch

@@ -1,0 +1,620 @@
+"""GPU: the policy operators against their definitions in 64 bits (policy_oracle.py), at the sizes, masks, strides and orders where they
+can go wrong; every bound is counted from the roundings there."""
+import numpy as np
+import pytest
+import torch
+
+import policy_oracle as oracle
+
+pytestmark = pytest.mark.gpu
+F32, BF16, F16, F64 = torch.float32, torch.bfloat16, torch.float16, torch.float64
+
+
+@pytest.fixture(scope="module")
+def ops():
+    from contracts_amd import policy_ops
+    return policy_ops
+
+
+def gen(seed):
+    g = torch.Generator(device="cuda")
+    g.manual_seed(seed)
+    return g
+
+
+def scan_inputs(T, E, C, H, dt, gt, seed, done=0.1):
+    g = gen(seed)
+    x = torch.randn((T, E, C), generator=g, device="cuda").to(dt)
+    gate = torch.sigmoid(torch.randn((T, E, H), generator=g, device="cuda") + 1).to(gt) if H else 0.9375
+    state = torch.randn((E, C), generator=g, device="cuda").to(F64 if dt == F64 else F32)
+    d = (torch.rand((T, E), generator=g, device="cuda") < done) if done else None
+    return x, gate, state, d
+
+
+def check_scan(ops, x, gate, state, done, reverse, tag, grad=True):
+    u = oracle.U64 if x.dtype == F64 else oracle.U32
+    want = oracle.scan(x, gate, state, done, reverse, u)
+    y, last = ops.linear_scan(x, gate, state=state, done=done, reverse=reverse)
+    assert y.dtype == x.dtype and y.shape == x.shape
+    oracle.close(y, want["y"], oracle.rounded(want["y"], want["ybound"], x.dtype), tag + " y")
+    oracle.close(last, want["last"], want["lastbound"] + np.abs(want["last"]) * u, tag + " last")
+    if not grad:
+        return
+    g = gen(99)
+    dy = torch.randn(x.shape, generator=g, device="cuda").to(x.dtype)
+    dl = torch.randn(last.shape, generator=g, device="cuda")
+    leaves = [t.clone().requires_grad_(True) if t is not None else None for t in (x, gate if isinstance(gate, torch.Tensor) else None, state)]
+    y2, last2 = ops.linear_scan(leaves[0], gate if leaves[1] is None else leaves[1], state=leaves[2], done=done, reverse=reverse)
+    assert y2.equal(y) and last2.equal(last), tag + ": the pass that keeps states gives other bits"
+    got = iter(torch.autograd.grad((y2, last2), [t for t in leaves if t is not None], (dy, dl)))
+    H = gate.shape[2] if isinstance(gate, torch.Tensor) else x.shape[2]
+    back = oracle.scan_grad(want, dy, dl, H, reverse, u)
+    oracle.close(next(got), back["dx"], oracle.rounded(back["dx"], back["dxbound"], x.dtype), tag + " dx")
+    if leaves[1] is not None:
+        oracle.close(next(got), back["dgate"], oracle.rounded(back["dgate"], back["dgatebound"], gate.dtype), tag + " dgate")
+    if leaves[2] is not None:
+        oracle.close(next(got), back["dstate"], back["dstatebound"] + np.abs(back["dstate"]) * u, tag + " dstate")
+
+
+# (T, E, C, H): one step, one run of 16 and its borders, tiles of 64, heads of every width (one lane, odd, a wave, several waves), a split time axis
+SIZES = [(1, 1, 1, 1), (1, 5, 7, 7), (2, 64, 256, 256), (15, 3, 2, 1), (16, 3, 2, 2), (17, 2, 64, 64), (63, 1, 65, 5), (64, 1, 130, 130), (65, 4, 130, 13), (100, 3, 40, 1),
+         (130, 2, 66, 33), (257, 1, 96, 3), (300, 3, 264, 1), (700, 1, 200, 1), (1000, 2, 6, 2), (1303, 1, 24, 3), (2051, 2, 10, 10), (5000, 1, 8, 8)]
+
+
+@pytest.mark.parametrize("T,E,C,H", SIZES)
+@pytest.mark.parametrize("dt,gt", [(F32, F32), (BF16, BF16), (BF16, F32), (F16, F16), (F16, F32)])
+def test_scan_and_its_gradients(ops, T, E, C, H, dt, gt):
+    for reverse in (False, True):
+        x, gate, state, done = scan_inputs(T, E, C, H, dt, gt, T + 7 * C)
+        check_scan(ops, x, gate, state, done, reverse, "%s reverse=%s" % ((T, E, C, H), reverse))
+
+
+@pytest.mark.parametrize("T,E,C", [(1, 3, 5), (40, 2, 9), (129, 7, 2), (1500, 2, 3)])
+@pytest.mark.parametrize("dt", [F32, BF16, F16, F64])
+def test_scan_under_a_constant_gate_without_state_or_done(ops, T, E, C, dt):
+    for reverse in (False, True):
+        x, gate, state, done = scan_inputs(T, E, C, 0, dt, dt, 5)
+        check_scan(ops, x, gate, None, None, reverse, "plain", grad=dt != F64)
+        check_scan(ops, x, gate, state, done, reverse, "state and done", grad=dt != F64)
+
+
+@pytest.mark.parametrize("T", [30, 700])
+def test_scan_in_double(ops, T):
+    x, gate, state, done = scan_inputs(T, 3, 6, 2, F64, F64, 8)
+    for reverse in (False, True):
+        check_scan(ops, x, gate, state, done, reverse, "double", grad=False)
+    with pytest.raises(ValueError, match="float64"):
+        ops.linear_scan(x.requires_grad_(True), gate)
+
+
+def test_scan_of_nothing(ops):
+    state = torch.randn((3, 4), device="cuda").requires_grad_(True)
+    y, last = ops.linear_scan(torch.zeros((0, 3, 4), device="cuda"), torch.zeros((0, 3, 2), device="cuda"), state=state)
+    assert y.shape == (0, 3, 4) and last.equal(state)
+    assert torch.autograd.grad(last.sum(), state)[0].equal(torch.ones_like(state))
+    y, last = ops.linear_scan(torch.zeros((5, 0, 4), device="cuda"), torch.zeros((5, 0, 4), device="cuda"), done=torch.zeros((5, 0), dtype=torch.bool, device="cuda"))
+    assert y.shape == (5, 0, 4) and last.shape == (0, 4)
+    x = torch.zeros((5, 2, 0), device="cuda").requires_grad_(True)
+    assert ops.linear_scan(x, 0.5)[0].shape == (5, 2, 0)
+
+
+@pytest.mark.parametrize("T", [40, 1400])
+def test_scan_forgets_what_done_or_a_zero_gate_closes_off(ops, T):
+    """infinities and NaN of a finished episode stay in it, in both directions; the same where the gate is exactly 0"""
+    for reverse in (False, True):
+        for by_gate in (False, True):
+            x, gate, state, done = scan_inputs(T, 2, 6, 6, F32, F32, 3, done=0)
+            done = torch.zeros((T, 2), dtype=torch.uint8, device="cuda")
+            t = T // 2
+            bad = t + 1 if reverse else t
+            x[bad, :, 0], x[bad, :, 1], x[bad, :, 2] = float("inf"), float("nan"), -float("inf")
+            if by_gate:
+                gate[t if reverse else t + 1] = 0
+            else:
+                done[t] = 1
+            x, gate = x.requires_grad_(True), gate.requires_grad_(True)
+            y, last = ops.linear_scan(x, gate, state=state, done=done, reverse=reverse)
+            want = oracle.scan(x, gate, state, done, reverse)
+            keep = slice(0, t + 1) if reverse else slice(t + 1, T)
+            assert bool(torch.isfinite(y[keep]).all()) and bool(torch.isfinite(last).all())
+            oracle.close(y[keep], want["y"][keep], oracle.rounded(want["y"], want["ybound"], F32)[keep])
+            # the gradient too: what lies behind the border gets none from what lies ahead of it
+            dx = torch.autograd.grad(y[keep].sum(), x)[0]
+            other = slice(t + 1, T) if reverse else slice(0, t + 1)
+            assert bool((dx[other] == 0).all()) and bool((dx[keep] >= 1).all())
+
+
+def test_scan_gates_past_one_over_a_zero_state(ops):
+    """products of gates leave float's range while the state is 0: the state stays 0, no NaN"""
+    x = torch.zeros((2000, 1, 3), device="cuda")
+    x[-1] = 1
+    gate = torch.full((2000, 1, 3), 3.0, device="cuda")
+    y, last = ops.linear_scan(x, gate)
+    assert y.equal(x) and last.equal(x[-1])
+
+
+def test_scan_takes_strides_orders_and_shared_gates(ops):
+    T, E, C = 70, 3, 12
+    x, gate, state, done = scan_inputs(T, E, C, 4, F32, F32, 6)
+    want = ops.linear_scan(x, gate, state=state, done=done)
+    batch = lambda t: t.transpose(0, 1).contiguous().transpose(0, 1)  # noqa: E731 — batch-major memory
+    chan = lambda t: t.permute(2, 0, 1).contiguous().permute(1, 2, 0)  # noqa: E731 — channels far apart (copied first)
+    wide = torch.zeros((T, E + 2, C + 6), device="cuda")
+    wide[:, 1:-1, 3:-3] = x
+    odd = torch.zeros((T, E, 13), device="cuda", dtype=BF16)[:, :, 1:]
+    odd.copy_(x)
+    for xx in (batch(x), chan(x), wide[:, 1:-1, 3:-3]):
+        for gg in (gate, batch(gate), chan(gate)):
+            got = ops.linear_scan(xx, gg, state=state.t().contiguous().t(), done=done.t().contiguous().t())
+            assert got[0].equal(want[0]) and got[1].equal(want[1])
+    assert ops.linear_scan(odd, gate, state=state, done=done)[0].equal(ops.linear_scan(odd.contiguous(), gate, state=state, done=done)[0])
+    for shape in ((1, 1, 12), (1, 3, 4), (70, 1, 4)):
+        small = torch.rand(shape, device="cuda").requires_grad_(True)
+        full = small.detach().expand(T, E, shape[2]).contiguous().requires_grad_(True)
+        a, b = ops.linear_scan(x, small.expand(T, E, shape[2]), done=done), ops.linear_scan(x, full, done=done)
+        assert a[0].equal(b[0])
+        ga, gb = torch.autograd.grad(a[0].sum(), small)[0], torch.autograd.grad(b[0].sum(), full)[0]
+        dims = [i for i in range(3) if shape[i] == 1 and i < 2]
+        assert torch.allclose(ga, gb.sum(dims, keepdim=True), rtol=1e-5, atol=1e-4)  # torch's own sum over the shared axes
+    dy = torch.ones((), device="cuda").expand(T, E, C)
+    xg = x.clone().requires_grad_(True)
+    y, _ = ops.linear_scan(xg, gate)
+    assert torch.autograd.grad(y, xg, dy, retain_graph=True)[0].equal(torch.autograd.grad(y, xg, dy.contiguous())[0])
+
+
+@pytest.mark.parametrize("reverse", [False, True])
+@pytest.mark.parametrize("dt", [F32, BF16])
+def test_scan_in_pieces_and_step_by_step(ops, reverse, dt):
+    """`last` of one call is `state` of the next, done flags on the borders included; single steps move a state on in place"""
+    T = 90
+    x, gate, state, done = scan_inputs(T, 4, 6, 6, dt, F32, 2, done=0.3)
+    want = oracle.scan(x, gate, state, done, reverse)
+    bound = oracle.rounded(want["y"], want["ybound"], dt)
+    for cuts in ([0, 1, 17, 64, 90], list(range(T + 1))):
+        pieces = list(zip(cuts, cuts[1:]))[::-1 if reverse else 1]
+        out, s = torch.empty_like(x), state.clone()
+        for lo, hi in pieces:
+            _, s2 = ops.linear_scan(x[lo:hi], gate[lo:hi], state=s, done=done[lo:hi], reverse=reverse, out=out[lo:hi], state_out=s)
+            assert s2 is s
+        oracle.close(out, want["y"], bound, "pieces")
+        oracle.close(s, want["last"], want["lastbound"] + np.abs(want["last"]) * oracle.U32, "last")
+    s = state.clone()
+    y, _ = ops.linear_scan(x, gate, state=s, done=done, reverse=reverse, state_out=s)
+    oracle.close(y, want["y"], bound, "in place over a long time axis")
+    oracle.close(s, want["last"], want["lastbound"] + np.abs(want["last"]) * oracle.U32, "last")
+
+
+def test_scan_gradient_against_differences(ops):
+    """the kernel's gradients against central differences of the definition in 64 bits (exact: every entry enters linearly)"""
+    x, gate, state, done = scan_inputs(6, 2, 4, 2, F32, F32, 4, done=0.2)
+    leaves = [t.clone().requires_grad_(True) for t in (x, gate, state)]
+    for reverse in (False, True):
+        y, last = ops.linear_scan(*leaves[:2], state=leaves[2], done=done, reverse=reverse)
+        grads = torch.autograd.grad(y.sum() + last.sum(), leaves)
+        at = [t.double().cpu() for t in (x, gate, state)]
+
+        def value():
+            f = oracle.scan(at[0], at[1], at[2], done.cpu(), reverse)
+            return f["y"].sum() + f["last"].sum()
+        for t, d in zip(at, grads):
+            flat, d = t.view(-1), d.double().cpu().reshape(-1)
+            for i in range(flat.numel()):
+                keep = flat[i].item()
+                flat[i] = keep + 0.5
+                up = value()
+                flat[i] = keep - 0.5
+                down = value()
+                flat[i] = keep
+                assert abs(up - down - d[i].item()) <= 1e-5 * (1 + abs(d[i].item())) * 8
+
+
+def test_scan_over_offsets_past_32_bits(ops):
+    """a rollout of 2^32 and some elements: the last columns and steps are where a 32-bit offset would wrap"""
+    T, E, C = 17, 131072, 1928  # 4.3e9 bfloat16 elements
+    x = torch.zeros((T, E, C), dtype=BF16, device="cuda")
+    x[0, -1], x[-1, -1], x[0, 0] = 1, 2, 3
+    y, last = ops.linear_scan(x, 0.5)
+    del x
+    assert y[0, 0, 0].item() == 3 and y[1, 0, 0].item() == 1.5 and y[0, -1, -1].item() == 1 and y[3, -1, 5].item() == 0.125
+    assert last[-1].eq(2 + 2.0 ** -16).all() and last[1:-1].count_nonzero().item() == 0 and last[0].eq(3 * 2.0 ** -16).all()
+    assert y[:, 1:-1].view(T, -1)[:, ::4099].count_nonzero().item() == 0
+
+
+def test_scan_refusals(ops):
+    x, gate, state, done = scan_inputs(4, 3, 6, 2, F32, F32, 1)
+    bad = [dict(x=x[0]), dict(x=x.int()), dict(x=x.cpu()), dict(gate=gate[:, :2]), dict(gate=torch.rand((4, 3, 4), device="cuda")), dict(gate=gate.bfloat16()), dict(gate=gate.double()),
+           dict(state=state[:2]), dict(state=state.half()), dict(done=done[:3]), dict(done=done.float()), dict(out=x), dict(out=torch.empty((4, 3, 6), dtype=F16, device="cuda")),
+           dict(state_out=torch.empty((3, 7), device="cuda")), dict(out=torch.empty((4, 6, 3), device="cuda").transpose(1, 2)), dict(state_out=x[0]),
+           dict(x=x.clone().requires_grad_(True), out=torch.empty_like(x))]
+    for kw in bad:
+        args = dict(dict(x=x, gate=gate, state=state, done=done), **kw)
+        with pytest.raises(ValueError):
+            ops.linear_scan(args.pop("x"), args.pop("gate"), **args)
+    from contracts_amd._lib import EngineError
+    with pytest.raises(EngineError, match="finite"):
+        ops.linear_scan(x, float("nan"))
+
+
+# ---- advantages -------------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("P,E,n", [(1, 1, 1), (2, 3, 2), (16, 5, 8), (17, 33, 2), (64, 9, 1), (100, 70, 3), (333, 4, 5)])
+@pytest.mark.parametrize("rt,vt", [(F64, F32), (F32, F32), (F64, BF16), (F32, F16)])
+def test_advantages(ops, P, E, n, rt, vt):
+    g = gen(P * n)
+    r = torch.randn((P, E, n), generator=g, device="cuda").to(rt)
+    v, lv = torch.randn((P, E, n), generator=g, device="cuda").to(vt), torch.randn((E, n), generator=g, device="cuda").to(vt)
+    dones = [None, torch.rand((P, E), generator=g, device="cuda") < 0.1, (torch.rand((P, E, n), generator=g, device="cuda") < 0.1).to(torch.uint8)]
+    for k, done in enumerate(dones):
+        first, last = (k * P) // 3, lv if k != 1 else None
+        got = ops.advantages(r, v, last, done, gamma=0.97, lam=0.9, first_plane=first)
+        want = oracle.advantages(r, v, last, done, 0.97, 0.9, first)
+        for a, b in zip(got, want):
+            assert a.dtype == F32
+            oracle.close(a, b, oracle.rounded(b, 1e-12 * (1 + np.abs(b)), F32), "P=%d first=%d" % (P, first))  # double sums: far below half a step of float
+
+
+def test_advantages_read_nothing_past_a_border(ops):
+    """a value or reward that is not finite stays on its side of the border"""
+    r, v = torch.ones((20, 3, 2), dtype=F64, device="cuda"), torch.zeros((20, 3, 2), device="cuda")
+    done = torch.zeros((20, 3), dtype=torch.uint8, device="cuda")
+    done[9] = 1
+    v[10], r[12] = float("nan"), float("inf")
+    adv, ret = ops.advantages(r, v, torch.full((3, 2), float("nan"), device="cuda"), done, gamma=0.5, lam=0.5)
+    assert torch.isfinite(adv[:10]).all() and adv[9].eq(1).all() and ret[8].eq(1.25).all()
+
+
+def test_advantages_write_into_given_planes_and_refuse_the_rest(ops):
+    r, v = torch.randn((6, 3, 2), dtype=F64, device="cuda"), torch.randn((6, 3, 2), device="cuda")
+    out = (torch.empty((6, 3, 2), device="cuda"), torch.empty((6, 3, 2), device="cuda"))
+    adv, ret = ops.advantages(r, v, out=out)
+    assert adv is out[0] and ret is out[1]
+    a2, r2 = ops.advantages(r.transpose(0, 1).contiguous().transpose(0, 1), v)
+    assert a2.equal(adv) and r2.equal(ret)
+    assert ops.advantages(r[:0], v[:0])[0].shape == (0, 3, 2)
+    for kw in (dict(value=v[:5]), dict(value=v.double()), dict(reward=r.half()), dict(last_value=v[0].half()), dict(done=torch.zeros((6, 2), dtype=torch.bool, device="cuda")), dict(first_plane=6),
+               dict(first_plane=-1), dict(out=(v, ret)), dict(out=(adv, adv)), dict(value=v.cpu())):
+        args = dict(dict(reward=r, value=v), **kw)
+        with pytest.raises(ValueError):
+            ops.advantages(**args)
+
+
+# ---- process_logits ---------------------------------------------------------------------------------------------------------------
+def logits_inputs(R, V, L, dt, seed, tokens=torch.int32):
+    g = gen(seed)
+    u = lambda *s: torch.rand(s, generator=g, device="cuda")  # noqa: E731
+    l = (torch.randn((R, V), generator=g, device="cuda") * 3).to(dt)
+    l[u(R, V) < 0.05] = 0
+    tok = (V * u(R, L) ** 3).long().clamp_(0, V - 1).to(tokens)
+    lengths = (u(R) * (L + 1)).to(torch.int32)
+    lengths[0] = L
+    prompt = (lengths * u(R)).to(torch.int32)
+    pen = dict(repetition=1 + u(R), presence=u(R) - 0.2, frequency=u(R) * 0.3)
+    return l, tok, lengths, prompt, pen, u
+
+
+def check_logits(ops, l, kw, allowed, tag, out_dtype=None, grad=True):
+    flat = {k: v for k, v in kw.items() if k not in ("mask", "mask_index")}
+    if flat.get("bias") is not None:
+        flat["bias"] = flat["bias"].reshape(-1, l.shape[-1])
+    dz = torch.randn(l.shape, generator=gen(5), device="cuda").to(l.dtype)
+    want = oracle.logits(l, allowed=None if allowed is None else allowed.cpu().numpy(), dz=dz, **flat)
+    z = ops.process_logits(l, **kw)
+    oracle.close(z, want["z"], oracle.rounded(np.where(np.isfinite(want["z"]), want["z"], 0), want["bound"], l.dtype), tag + " z")
+    if not grad:
+        return
+    leaves = [l.clone().requires_grad_(True)] + ([kw["bias"].clone().requires_grad_(True)] if kw.get("bias") is not None else [])
+    z2 = ops.process_logits(leaves[0], **(dict(kw, bias=leaves[1]) if len(leaves) > 1 else kw))
+    assert z2.equal(z)
+    got = torch.autograd.grad(z2, leaves, dz)
+    oracle.close(got[0], want["dlogits"], oracle.rounded(want["dlogits"], want["dlogitsbound"], l.dtype), tag + " dlogits")
+    if len(leaves) > 1:
+        oracle.close(got[1].reshape(want["dbias"].shape), want["dbias"], oracle.rounded(want["dbias"], want["dbiasbound"], kw["bias"].dtype), tag + " dbias")
+
+
+LOGITS = [(1, 1, 1), (1, 2, 5), (3, 7, 40), (130, 8, 16), (64, 9, 33), (257, 31, 4), (6, 32, 100), (10, 33, 9), (12, 64, 64), (5, 151, 333), (4, 1000, 17), (2, 1025, 300), (3, 4096, 70),
+          (2, 4097, 1000), (1, 50257, 777), (3, 9001, 6000)]
+
+
+@pytest.mark.parametrize("R,V,L", LOGITS)
+@pytest.mark.parametrize("dt", [F32, BF16, F16])
+def test_logits_and_their_gradients(ops, R, V, L, dt):
+    for k, (tt, maskkind, bt) in enumerate([(torch.int32, "rows", F32), (torch.int64, "bits", dt), (torch.uint8 if V <= 256 else torch.int32, None, None), (None, "bool", F32)]):
+        l, tok, lengths, prompt, pen, u = logits_inputs(R, V, L, dt, R + V + k, tt or torch.int32)
+        kw, allowed = dict(pen, tokens=tok, lengths=lengths, prompt_lengths=prompt) if tt is not None else {}, None
+        if bt is not None:
+            B = next(b for b in (3, 2, 1) if R % b == 0)
+            kw["bias"] = torch.randn((B, V), generator=gen(k), device="cuda").to(bt)
+        if maskkind == "rows":
+            allowed = u(R, V) < 0.6
+            allowed[R // 2] = False  # a row that the mask leaves nothing of
+            kw["mask"] = allowed.to(torch.uint8)
+        elif maskkind == "bool":
+            B = 2 if R % 2 == 0 else 1
+            m = u(B, V) < 0.5
+            kw["mask"], allowed = m, m.repeat(R // B, 1)
+        elif maskkind == "bits":
+            S = 5
+            m = u(S, V) < 0.5
+            index = (u(R) * (S + 2)).to(torch.int32) - 1  # -1: everything; S: past the end, nothing
+            kw["mask"], kw["mask_index"] = ops.pack_mask(m), index
+            allowed = torch.where((index < 0)[:, None], True, torch.where((index >= S)[:, None], False, m[index.clamp(0, S - 1).long()]))
+        check_logits(ops, l, kw, allowed, "%s %s case %d" % ((R, V, L), dt, k))
+
+
+@pytest.mark.parametrize("V", [8, 300, 5000])
+def test_logits_masked_places_hold_anything(ops, V):
+    l, tok, lengths, prompt, pen, u = logits_inputs(6, V, 20, F32, 3)
+    allowed = u(6, V) < 0.5
+    allowed[0], allowed[1] = False, True
+    bad = torch.tensor([float("nan"), float("inf"), -float("inf"), torch.finfo(F32).min], device="cuda")
+    l = torch.where(allowed, l, bad[(torch.arange(V, device="cuda") % 4)])
+    l[1, 0], l[1, V - 1] = float("nan"), -float("inf")
+    bias = torch.randn((6, V), generator=gen(1), device="cuda")
+    bias[:, 1] = torch.where(allowed[:, 1], bias[:, 1], torch.finfo(F32).min)
+    check_logits(ops, l, dict(pen, tokens=tok, lengths=lengths, bias=bias, mask=allowed), allowed, "V=%d" % V, grad=False)
+    leaf, bleaf = l.clone().requires_grad_(True), bias.clone().requires_grad_(True)
+    z = ops.process_logits(leaf, tokens=tok, lengths=lengths, bias=bleaf, mask=allowed, **pen)
+    assert torch.isneginf(z[0]).all()
+    dz = torch.where(allowed, 1.0, bad[0])  # a softmax over an empty row hands NaN back
+    dl, db = torch.autograd.grad(z, (leaf, bleaf), dz)
+    assert (dl[~allowed] == 0).all() and (db[~allowed] == 0).all() and (db[allowed] == 1).all()
+
+
+def test_logits_histories(ops):
+    """lengths past the ends, prompts longer than the history, ids outside the vocabulary, no history at all"""
+    R, V, L = 6, 40, 30
+    l, tok, lengths, prompt, pen, u = logits_inputs(R, V, L, F32, 9, torch.int64)
+    tok[1, ::2], tok[2, :], tok[3, 3] = -1, V, 2 ** 40
+    tok[4, 0] = 2 ** 32  # 0 in its low 32 bits
+    lengths = torch.tensor([L, L, L, L + 50, L, -3], dtype=torch.int32, device="cuda")
+    prompt = torch.tensor([0, -5, 10, L + 9, 1, 4], dtype=torch.int32, device="cuda")
+    check_logits(ops, l, dict(pen, tokens=tok, lengths=lengths, prompt_lengths=prompt), None, "odd lengths")
+    check_logits(ops, l, dict(pen, tokens=tok), None, "all of it")
+    check_logits(ops, l, dict(tokens=tok, repetition=1.5, presence=-0.5, frequency=0.25), None, "scalars")
+    check_logits(ops, l, dict(pen, tokens=tok[:, :0]), None, "empty")
+    check_logits(ops, l, dict(tokens=tok.to(torch.int32), repetition=2.0), None, "int32 wraps nothing")
+    z = ops.process_logits(l, repetition=2.0, presence=1.0)  # no history, no penalty
+    assert z.equal(l) and z.data_ptr() != l.data_ptr()
+
+
+@pytest.mark.parametrize("V", [5, 8, 200, 6000])
+def test_logits_strides_axes_and_outputs(ops, V):
+    E, n, T = 6, 4, 13
+    g = gen(V)
+    l = torch.randn((E, n, V), generator=g, device="cuda")
+    acts = (torch.rand((T, E, n), generator=g, device="cuda") * min(V, 256)).to(torch.uint8)
+    bias, mask = torch.randn((n, V), generator=g, device="cuda"), torch.rand((n, V), generator=g, device="cuda") < 0.7
+    kw = dict(tokens=acts.permute(1, 2, 0), lengths=torch.randint(0, T + 1, (E, n), generator=g, device="cuda"), repetition=1.25, frequency=0.125, bias=bias, mask=mask)
+    z = ops.process_logits(l, **kw)
+    flat = dict(kw, tokens=kw["tokens"].reshape(E * n, T), lengths=kw["lengths"].reshape(-1))
+    check_logits(ops, l.view(E * n, V), flat, mask.repeat(E, 1), "flat")
+    assert z.shape == l.shape and z.equal(ops.process_logits(l.view(E * n, V), **flat).view(E, n, V))
+    assert z.equal(ops.process_logits(l, **dict(kw, mask=ops.pack_mask(mask))))
+    assert z.equal(ops.process_logits(l, **dict(kw, tokens=kw["tokens"].contiguous().to(torch.int64), bias=bias.expand(E, n, V), mask=mask.expand(E, n, V))))
+    for off in (0, 1, 4):  # rows inside a wider table
+        wide = torch.full((E, n, V + 7), float("nan"), device="cuda")
+        wide[..., off:off + V] = l
+        to = torch.full((E * n, V + 9), 7.0, device="cuda")
+        assert ops.process_logits(wide[..., off:off + V], out=to.view(E, n, V + 9)[..., off:off + V], **kw).equal(z)
+        assert (to[:, :off] == 7).all() and (to[:, off + V:] == 7).all()
+    assert ops.process_logits(l.permute(2, 0, 1).contiguous().permute(1, 2, 0), **kw).equal(z)
+    assert ops.process_logits(l.transpose(0, 1).contiguous().transpose(0, 1), **kw).equal(z)
+    h = l.to(BF16)
+    assert ops.process_logits(h, out=torch.empty_like(l), **kw).to(BF16).equal(ops.process_logits(h, **kw))
+    same = l.clone()
+    assert ops.process_logits(same, out=same, **kw) is same and same.equal(z)
+    one = ops.process_logits(l[0, 0], tokens=acts[:, 0, 0], lengths=kw["lengths"][0, 0], repetition=1.25, frequency=0.125, bias=bias[0], mask=mask[0])
+    assert one.equal(z[0, 0])
+
+
+def test_logits_gradient_against_differences(ops):
+    l, tok, lengths, prompt, pen, u = logits_inputs(3, 6, 9, F32, 2)
+    l = torch.where(l.abs() < 0.5, torch.ones_like(l), l)  # differences do not cross 0
+    bias, allowed = torch.randn((1, 6), generator=gen(3), device="cuda"), u(3, 6) < 0.7
+    leaves = [l.clone().requires_grad_(True), bias.clone().requires_grad_(True)]
+    z = ops.process_logits(leaves[0], tokens=tok, lengths=lengths, prompt_lengths=prompt, bias=leaves[1], mask=allowed, **pen)
+    w = torch.randn((3, 6), generator=gen(4), device="cuda")
+    grads = torch.autograd.grad(z, leaves, w)
+    at = [l.double().cpu(), bias.double().cpu()]
+
+    def value():
+        f = oracle.logits(at[0], tok.cpu(), lengths.cpu(), prompt.cpu(), bias=at[1], **{k: v.cpu() for k, v in pen.items()})["z"]
+        return (np.where(allowed.cpu().numpy(), f, 0) * w.double().cpu().numpy()).sum()
+    for t, d in zip(at, grads):
+        flat, d = t.view(-1), d.double().cpu().reshape(-1)
+        for i in range(flat.numel()):
+            keep = flat[i].item()
+            flat[i] = keep + 0.25
+            up = value()
+            flat[i] = keep - 0.25
+            down = value()
+            flat[i] = keep
+            assert abs((up - down) / 0.5 - d[i].item()) <= 1e-5 * (1 + abs(d[i].item()))
+
+
+def test_logits_empty_and_refusals(ops):
+    l = torch.randn((6, 10), device="cuda")
+    tok = torch.zeros((6, 4), dtype=torch.int32, device="cuda")
+    assert ops.process_logits(l[:0], bias=l[0]).shape == (0, 10) and ops.process_logits(l[:, :0]).shape == (6, 0)
+    lg, bg = l[:0].clone().requires_grad_(True), l[0].clone().requires_grad_(True)
+    assert torch.autograd.grad(ops.process_logits(lg, bias=bg).sum(), bg)[0].equal(torch.zeros_like(bg))
+    ok = torch.ones((6, 10), dtype=torch.bool, device="cuda")
+    for kw in (dict(logits=l.double()), dict(logits=l.cpu()), dict(tokens=tok[:5]), dict(tokens=tok.float()), dict(lengths=tok[:, 0]), dict(tokens=tok, lengths=tok[:5, 0]),
+               dict(tokens=tok, lengths=tok[:, 0].float()), dict(tokens=tok, repetition=l[0, :5]), dict(bias=l[:, :9]), dict(bias=l.double()), dict(bias=l[:1].bfloat16()),
+               dict(mask=ok[:, :9]), dict(mask=ok.float()), dict(mask=torch.zeros((6, 2), dtype=torch.int32, device="cuda")), dict(mask_index=tok[:, 0]),
+               dict(mask=ok[:3], mask_index=tok[:5, 0]), dict(out=l.half()), dict(out=l[:5]), dict(out=l.t().contiguous().t()), dict(logits=l.clone().requires_grad_(True), out=torch.empty_like(l)),
+               dict(bias=l, logits=l.clone(), out=l)):
+        args = dict(dict(logits=l), **kw)
+        with pytest.raises(ValueError):
+            ops.process_logits(args.pop("logits"), **args)
+    from contracts_amd._lib import EngineError
+    for kw in (dict(bias=l[:4]), dict(mask=ok[:4]), dict(tokens=tok, repetition=0.0), dict(tokens=tok, repetition=-1.0)):
+        with pytest.raises(EngineError, match="CE_EINVAL"):
+            ops.process_logits(l, **kw)
+
+
+# ---- together, as they are used -----------------------------------------------------------------------------------------------------
+def test_a_learners_round_over_the_engine(ops):
+    """sampler: a recurrent policy's state moved on step by step, scores shaped (masks, biases, repeated actions), arg-max inside the step
+    kernel; learner: the same memory over the whole rollout, advantages and returns of the trajectory — all against 64 bits"""
+    from contracts_amd.engine import BatchedEnv
+    E, n, T, D = 9, 3, 24, 10
+    env = BatchedEnv("cleanup", E, n, contract="cleanup", horizon=7, auto_reset=True)
+    env.seed(seed0=3)
+    env.reset()
+    A, g = env.num_actions, gen(0)
+    feats, gates = torch.randn((T, E * n, D), generator=g, device="cuda"), torch.rand((T, E * n, D), generator=g, device="cuda")
+    head = torch.randn((D, A), generator=g, device="cuda")
+    allowed = torch.rand((n, A), generator=g, device="cuda") < 0.6
+    allowed[:, 0] = True
+    bias = torch.randn((n, A), generator=g, device="cuda")
+    acts = torch.zeros((T, E, n), dtype=torch.uint8, device="cuda")
+    reward, done = torch.zeros((T, E, n), dtype=F64, device="cuda"), torch.zeros((T, E), dtype=torch.uint8, device="cuda")
+    state, views = torch.zeros((E * n, D), device="cuda"), env.torch_tensors()
+    for t in range(T):
+        mem, _ = ops.linear_scan(feats[t:t + 1], gates[t:t + 1], state=state, state_out=state)
+        raw = (mem[0] @ head).view(E, n, A)
+        shaped = env.shape_scores(raw, tokens=acts[:t].permute(1, 2, 0), repetition=1.5, frequency=0.1, bias=bias, mask=allowed)
+        want = oracle.logits(raw.view(-1, A), acts[:t].permute(1, 2, 0).reshape(E * n, t), repetition=1.5, frequency=0.1, bias=bias, allowed=allowed.repeat(E, 1).cpu().numpy())
+        oracle.close(shaped.view(-1, A), want["z"], oracle.rounded(np.where(np.isfinite(want["z"]), want["z"], 0), want["bound"], F32), "step %d" % t)
+        env.step_policy_device(shaped.data_ptr(), "argmax")
+        env.synchronize()
+        acts[t] = torch.from_numpy(env.download("actions_taken")).cuda()
+        assert acts[t].long().equal(shaped.argmax(-1)) and bool(allowed.expand(E, n, A).gather(2, acts[t].long()[..., None]).all())
+        reward[t], done[t] = views["reward"], views["done"]
+        state = torch.where(done[t].repeat_interleave(n)[:, None] != 0, 0.0, state)  # the memory of an episode that ended
+    env.check_faults()
+    y, last = ops.linear_scan(feats, gates, done=done.repeat_interleave(n, 1))
+    want = oracle.scan(feats, gates, None, done.repeat_interleave(n, 1), False)
+    oracle.close(y, want["y"], oracle.rounded(want["y"], want["ybound"], F32), "learner's memory")
+    oracle.close(state, want["last"], want["lastbound"] + np.abs(want["last"]) * oracle.U32, "sampler's state")
+    # the same actions through the fused rollout: a ring of 10 planes keeps the last 10 steps, wrapped
+    env.seed(seed0=3)
+    env.reset()
+    traj = env.alloc_trajectory(10, fields=["reward", "done"])
+    env.rollout_fused(acts.data_ptr(), T, traj=traj)
+    env.synchronize()
+    first = traj.c.first_plane
+    assert first == T % 10 and traj.tensors["reward"].roll(-first, 0).equal(reward[-10:])
+    value, lv = torch.randn((10, E, n), generator=g, device="cuda"), torch.randn((E, n), generator=g, device="cuda")
+    adv, ret = traj.advantages(value, lv, gamma=0.9, lam=0.8)
+    for a, b in zip((adv, ret), oracle.advantages(traj.tensors["reward"], value, lv, traj.tensors["done"], 0.9, 0.8, first)):
+        oracle.close(a, b, oracle.rounded(b, 1e-12 * (1 + np.abs(b)), F32))
+    got = traj.returns(0.9, last_value=lv.double())
+    back = oracle.scan(reward[-10:], 0.9, lv.double(), done[-10:], True, oracle.U64)
+    oracle.close(got.roll(-first, 0), back["y"], oracle.rounded(back["y"], back["ybound"], F64), "returns")
+    env.close()
+
+
+def test_trajectory_methods_of_selfdrive_and_their_refusals(ops):
+    from contracts_amd.engine import BatchedEnv
+    env = BatchedEnv("selfdrive", 5, 4, contract="selfdrive_distprop", horizon=60, auto_reset=True)
+    env.seed(seed0=1)
+    env.reset()
+    T = 50
+    acts = torch.rand((T, 5, 4), device="cuda") * 0.2 - 0.1
+    traj = env.alloc_trajectory(T)
+    env.rollout_fused(acts.data_ptr(), T, traj=traj)
+    env.synchronize()
+    got = traj.returns(0.95)
+    d = traj.tensors["done_agents"]
+    want = oracle.scan(traj.tensors["reward"].view(T, 20, 1), 0.95, None, d.view(T, 20), True, oracle.U64)
+    oracle.close(got.view(T, 20, 1), want["y"], oracle.rounded(want["y"], want["ybound"], F64))
+    value = torch.randn((T, 5, 4), device="cuda")
+    for a, b in zip(traj.advantages(value), oracle.advantages(traj.tensors["reward"], value, None, d, 0.99, 0.95, 0)):
+        oracle.close(a, b, oracle.rounded(b, 1e-12 * (1 + np.abs(b)), F32))
+    with pytest.raises(ValueError, match="first_plane"):
+        traj.returns(0.9, first_plane=T)
+    with pytest.raises(ValueError, match="done_agents"):
+        env.alloc_trajectory(3, fields=["reward"]).returns(0.9)
+    with pytest.raises(ValueError, match="last_value"):
+        traj.returns(0.9, last_value=value[0, :3])
+    with pytest.raises(ValueError, match="no discrete actions"):
+        env.shape_scores(torch.zeros((5, 4, 1), device="cuda"))
+    env.close()
+    env = BatchedEnv("harvest", 2, 2)
+    with pytest.raises(ValueError, match="scores must be"):
+        env.shape_scores(torch.zeros((2, 2, 8), device="cuda"))
+    with pytest.raises(ValueError, match="float32"):
+        env.shape_scores(torch.zeros((2, 2, 7), device="cuda"), out=torch.zeros((2, 2, 7), device="cuda", dtype=F16))
+    env.close()
+
+
+# ---- streams, graphs, determinism -----------------------------------------------------------------------------------------------------
+def test_calls_follow_torchs_current_stream(ops):
+    """a producer that is still running on a side stream is waited for by stream order alone, workspaces and backward pass included"""
+    x, gate, state, done = scan_inputs(3000, 1, 16, 16, F32, F32, 12)
+    want = ops.linear_scan(x, gate, state=state, done=done)
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        big = torch.randn((4096, 4096), device="cuda")
+        for _ in range(20):
+            big = big @ big * 1e-2
+        late = x * (1 + 0 * torch.nan_to_num(big[0, 0], 0, 0, 0))
+        leaf = late.requires_grad_(True)
+        got = ops.linear_scan(leaf, gate, state=state, done=done)
+        dx = torch.autograd.grad(got[0].sum(), leaf)[0]
+        z = ops.process_logits(late[0].detach(), bias=late[1, 0].detach())
+    side.synchronize()
+    assert got[0].equal(want[0]) and got[1].equal(want[1]) and torch.isfinite(dx).all()
+    assert z.equal(x[0] + x[1, 0])
+
+
+@pytest.mark.parametrize("T", [1, 40, 3000])
+def test_calls_in_captured_graphs(ops, T):
+    """two graphs of the same calls, replayed in turn with eager work between: every replay gives the eager bits for its inputs"""
+    E, C, V, R = 2, 24, 300, 8
+    x, gate, state, done = scan_inputs(T, E, C, 6, BF16, F32, 21)
+    l, tok, lengths, prompt, pen, u = logits_inputs(R, V, 50, F32, 4)
+    bias = torch.randn((2, V), generator=gen(1), device="cuda")
+    r, v = torch.randn((T, E, 3), dtype=F64, device="cuda"), torch.randn((T, E, 3), device="cuda")
+    dy, dz = torch.randn(x.shape, device="cuda").to(BF16), torch.randn(l.shape, device="cuda")
+
+    def work():
+        leaves = [t.detach().requires_grad_(True) for t in (x, gate, state, l, bias)]
+        y, last = ops.linear_scan(leaves[0], leaves[1], state=leaves[2], done=done)
+        z = ops.process_logits(leaves[3], tokens=tok, lengths=lengths, prompt_lengths=prompt, bias=leaves[4], **pen)
+        grads = torch.autograd.grad((y, last, z), leaves, (dy, torch.ones_like(last), dz))
+        return [y.detach(), last.detach(), z.detach(), *grads, *ops.advantages(r, v, None, done)]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        work()
+    torch.cuda.current_stream().wait_stream(side)
+    graphs = []
+    for _ in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = work()
+        graphs.append((g, out))
+    for k in range(6):
+        x.copy_(torch.randn(x.shape, device="cuda"))
+        l.copy_(torch.randn(l.shape, device="cuda"))
+        r.copy_(torch.randn(r.shape, device="cuda"))
+        want = work()
+        torch.cuda.synchronize()
+        g, out = graphs[k % 2]
+        for o in out:
+            o.fill_(7)
+        g.replay()
+        eager = work()  # eager work between and beside the replays
+        torch.cuda.synchronize()
+        for i, (a, b, c) in enumerate(zip(out, want, eager)):
+            assert a.equal(b) and c.equal(b), "replay %d output %d" % (k, i)
+
+
+def test_the_same_call_gives_the_same_bits(ops):
+    x, gate, state, done = scan_inputs(2500, 3, 400, 2, BF16, F32, 30)
+    l, tok, lengths, prompt, pen, u = logits_inputs(300, 2000, 400, BF16, 31)
+    bias = torch.randn((3, 2000), generator=gen(1), device="cuda")
+    dy, dz = torch.randn(x.shape, device="cuda").to(BF16), torch.randn(l.shape, device="cuda").to(BF16)
+    first = None
+    for _ in range(5):
+        leaves = [t.detach().requires_grad_(True) for t in (x, gate, state, l, bias)]
+        y, last = ops.linear_scan(leaves[0], leaves[1], state=leaves[2], done=done)
+        z = ops.process_logits(leaves[3], tokens=tok, lengths=lengths, prompt_lengths=prompt, bias=leaves[4], **pen)
+        out = [y, last, z, *torch.autograd.grad((y, z), leaves, (dy, dz))]
+        if first is None:
+            first = out
+        assert all(a.equal(b) for a, b in zip(out, first))
