@@ -52,7 +52,7 @@ struct Plan {
   int mode, vec;
 };
 
-bool divides(int vec, std::initializer_list<int64_t> strides) {
+bool divides(int64_t vec, std::initializer_list<int64_t> strides) {
   for (int64_t s : strides)
     if (s % vec) return false;
   return true;
@@ -77,10 +77,13 @@ int check_scan(const ce_scan* s) {
   return CE_OK;
 }
 
-// Chunks of the time axis: enough blocks of 4 waves for the chip where the columns alone are too few, and no chunk under 256 steps,
-// where folding the chunks before it would cost as much as the chunk.
+// Waves of a block and chunks of the time axis.  A wave on its own walks a run once; sharing the time axis costs a second walk, and
+// chunks cost reading everything twice, so both come only where the columns alone leave the chip's 1024 SIMDs short of waves.
+// No chunk is under 256 steps, where folding the chunks before it would cost as much as the chunk.
 void split(cp::ScanParams& p, uint64_t blocks) {
   p.chunks = 1;
+  p.waves = p.T <= CE_SCAN_SAVED_STEPS || blocks >= 2048 ? 1 : 4;
+  if (p.waves == 1) return;
   uint64_t want = blocks >= 512 ? 1 : 512 / blocks;
   const uint64_t most = p.T / 256;
   if (want > most) want = most;
@@ -98,15 +101,16 @@ void plan_scan(const ce_scan* s, const ce_scan_grad* g, Plan* o) {
   const uint64_t T = s->steps, E = s->rows, C = s->channels, H = s->gate ? s->heads : C;
   o->mode = !s->gate ? cp::kGateConst : H == C ? cp::kGateChannel : cp::kGateHead;
   const uint64_t head = C / H, b = size_of(s->dtype), gb = size_of(s->gate_dtype);
-  // pairs of channels as one access: a lane of one 2-byte channel would move half a cache line a wave
-  int vec = b == 2 ? 2 : 1;
-  if (vec == 2) {
-    bool ok = C % 2 == 0 && divides(2, {s->x_step, s->x_row}) && aligned(s->x, 2 * b) && aligned(s->y, 2 * b);
-    if (o->mode == cp::kGateChannel) ok = ok && divides(2, {s->gate_step, s->gate_row}) && aligned(s->gate, 2 * gb);
-    if (o->mode == cp::kGateHead) ok = ok && head % 2 == 0;
-    if (g) ok = ok && aligned(g->dy, 2 * b) && aligned(g->dx, 2 * b) && (o->mode != cp::kGateChannel || aligned(g->dgate, 2 * gb));
-    if (!ok) vec = 1;
-  }
+  // 8 bytes of neighbouring channels to a lane, or less where the arrays' alignment or strides do not allow it
+  auto fits = [&](int64_t v) {
+    bool ok = (int64_t)C % v == 0 && divides(v, {s->x_step, s->x_row}) && aligned(s->x, v * b);
+    if (o->mode == cp::kGateChannel) ok = ok && divides(v, {s->gate_step, s->gate_row}) && aligned(s->gate, v * gb);
+    if (o->mode == cp::kGateHead) ok = ok && (int64_t)head % v == 0;
+    if (!g) return ok && aligned(s->y, v * b);
+    return ok && aligned(g->dy, v * b) && aligned(g->dx, v * b) && (o->mode != cp::kGateChannel || aligned(g->dgate, v * gb));
+  };
+  int vec = g ? (b == 2 ? 2 : 1) : b == 2 ? 4 : b == 4 ? 2 : 1;
+  while (vec > 1 && !fits(vec)) vec /= 2;
   o->vec = vec;
   const bool rev = s->flags & CE_SCAN_REVERSE;
   const int64_t sign = rev ? -1 : 1, off = rev && T ? (int64_t)T - 1 : 0;
@@ -115,6 +119,7 @@ void plan_scan(const ce_scan* s, const ce_scan_grad* g, Plan* o) {
   p.row_cols = (uint32_t)(C / vec);
   p.head = (uint32_t)head;
   p.heads = (uint32_t)H;
+  p.rows = (uint32_t)E;
   p.cut_off = rev ? 0 : -1;
   p.x_step = sign * s->x_step;
   p.x_row = s->x_row;
@@ -151,7 +156,9 @@ void plan_scan(const ce_scan* s, const ce_scan_grad* g, Plan* o) {
       blocks = (E * H * seg + 63) / 64;
     }
   }
-  split(p, blocks ? blocks : 1);
+  const uint64_t row_lanes = g && o->mode == cp::kGateHead ? H * p.seg : p.row_cols;
+  p.flags = !s->done ? cp::kFlagsNone : row_lanes >= cp::kBallotRow ? cp::kFlagsBallot : cp::kFlagsLane;
+  split(p, blocks);
   // the chunks of a split time axis read the incoming state while the last of them writes the outgoing one
   if (!g && s->last && s->last == s->state) p.chunks = 1;
   if (p.chunks == 1) p.chunk = T;

@@ -30,13 +30,22 @@ template <> __device__ __forceinline__ float step(float a, float h, float x) { r
 // that a product past the type's range (gates over 1) does not turn it into NaN.
 template <class A> __device__ __forceinline__ A apply(A P, A H, A h) { return h == A(0) ? H : step(P, h, H); }
 
+// Done flags of a wave's run of 16 steps as 16 bits a lane.  A wave spans at most 4 rows where a row has 21 lanes or more: then each
+// quarter of the lanes reads one row's 16 flags with a single access and a ballot spreads them (kFlagsBallot); shorter rows
+// take an access a step (kFlagsLane).
+enum FlagMode { kFlagsNone = 0, kFlagsBallot = 1, kFlagsLane = 2 };
+constexpr uint32_t kBallotRow = 21;
+
 struct ScanParams {
   uint64_t T;
   uint32_t cols;      // E * C / VEC: columns of VEC channels
   uint32_t row_cols;  // C / VEC
   uint64_t chunk;     // steps of one block (a multiple of every tile), T where the time axis is not split
   uint32_t chunks;
+  uint32_t waves;     // waves of a block
   uint32_t head;      // channels under one gate
+  uint32_t rows;      // E
+  int32_t flags;      // FlagMode
   int32_t cut_off;    // the flag that cuts the state ahead of processed step i is done[i + cut_off]
   int64_t x_step, x_row, gate_step, gate_row, done_step, done_row, y_step;  // in processing order (steps may be negative)
   double decay;
@@ -60,6 +69,44 @@ struct ScanParams {
   uint32_t slabs;     // partial sums a head's gradient is made of
   float* slab;        // [slabs][T][E][H] where slabs > 1
 };
+
+// The done flags of steps i .. i + n of a wave's run: read ahead with its other loads (constructor), spread to a lane's bits later.
+struct Flags {
+  uint8_t d[16];
+  bool any = false;
+  __device__ __forceinline__ Flags(const ScanParams& p, uint32_t e, uint32_t e0, int lane, uint64_t i, int n) {
+    d[0] = 0;
+    if (p.flags == kFlagsBallot) {
+      const uint32_t row = e0 + (lane >> 4);
+      const uint64_t flag = i + (lane & 15) + (int64_t)p.cut_off;  // wraps past T ahead of the first step of a forward scan
+      if ((lane & 15) < n && flag < p.T && row < p.rows) d[0] = p.done[(int64_t)row * p.done_row + (int64_t)flag * p.done_step];
+    } else if (p.flags == kFlagsLane) {
+#pragma unroll
+      for (int s = 0; s < 16; ++s) {
+        const uint64_t flag = i + s + (int64_t)p.cut_off;
+        d[s] = 0;
+        if (s < n && flag < p.T) d[s] = p.done[(int64_t)e * p.done_row + (int64_t)flag * p.done_step];
+      }
+    }
+  }
+  __device__ __forceinline__ uint32_t bits(const ScanParams& p, uint32_t e, uint32_t e0, int n) {
+    uint32_t cut = 0;
+    if (p.flags == kFlagsBallot) {
+      const uint64_t m = __ballot(d[0] != 0);
+      any = m != 0;
+      cut = (uint32_t)(m >> ((e - e0) * 16)) & 0xffffu;
+    } else if (p.flags == kFlagsLane) {
+#pragma unroll
+      for (int s = 0; s < 16; ++s) cut |= (d[s] != 0 ? 1u : 0u) << s;
+      any = __any(cut != 0);
+    }
+    return cut;
+  }
+};
+
+__device__ __forceinline__ float fma_(float a, float b, float c) { return __builtin_fmaf(a, b, c); }
+__device__ __forceinline__ double fma_(double a, double b, double c) { return __builtin_fma(a, b, c); }
+template <class A> __device__ __forceinline__ bool finite(A a) { return __builtin_isfinite(a); }
 
 enum GateMode { kGateConst = 0, kGateChannel = 1, kGateHead = 2 };
 

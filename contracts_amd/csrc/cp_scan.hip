@@ -13,26 +13,18 @@ namespace cp {
 
 constexpr int kSteps = CE_SCAN_SAVED_STEPS;
 
-template <class X, class G, int MODE, int VEC> struct Tile {
-  static constexpr int GV = MODE == kGateChannel ? VEC : 1;
-  Pack<X, VEC> x[kSteps];
-  Pack<G, GV> g[MODE == kGateConst ? 1 : kSteps];
-  uint8_t d[kSteps];
-};
-
 template <class X, class G, int MODE, int VEC, int W, bool REDUCE> __global__ __launch_bounds__(kWave * W) void k_scan(ScanParams p) {
   typedef typename AccOf<X>::type A;
-  typedef Tile<X, G, MODE, VEC> TileT;
+  constexpr int GV = MODE == kGateChannel ? VEC : 1;
   __shared__ A fold[W > 1 ? 2 : 1][W][2][VEC][kWave];
   const int lane = threadIdx.x & 63, w = W > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : 0;
   const uint32_t col = blockIdx.x * kWave + lane;
   const bool live = col < p.cols;
   const uint32_t colc = live ? col : p.cols - 1;  // lanes past the end read a column that exists and write nothing
-  const uint32_t e = colc / p.row_cols, c = (colc % p.row_cols) * VEC;
+  const uint32_t e = colc / p.row_cols, c = (colc % p.row_cols) * VEC, e0 = __builtin_amdgcn_readfirstlane(e);
   const X* x = (const X*)p.x + (int64_t)e * p.x_row + c;
   const G* gate = (const G*)p.gate;
   if (MODE != kGateConst) gate += (int64_t)e * p.gate_row + (MODE == kGateHead ? c / p.head : c);
-  const uint8_t* done = p.done ? p.done + (int64_t)e * p.done_row + (int64_t)p.cut_off * p.done_step : nullptr;
   const uint64_t ch = (uint64_t)colc * VEC;  // index in the dense [E][C]
   X* y = (X*)p.y + ch;
   const uint64_t i0 = blockIdx.y * p.chunk, i1 = i0 + p.chunk < p.T ? i0 + p.chunk : p.T;
@@ -54,49 +46,67 @@ template <class X, class G, int MODE, int VEC, int W, bool REDUCE> __global__ __
 #pragma unroll
   for (int v = 0; v < VEC; ++v) P[v] = A(1);
 
-  auto take = [&](TileT& t, uint64_t i) {
-#pragma unroll
-    for (int s = 0; s < kSteps; ++s) {
-      const uint64_t at = i + s;
-      if (at < i1) {
-        t.x[s] = load<X, VEC>(x + (int64_t)at * p.x_step);
-        if (MODE != kGateConst) t.g[MODE == kGateConst ? 0 : s] = load<G, TileT::GV>(gate + (int64_t)at * p.gate_step);
-        const uint64_t flag = at + p.cut_off;  // wraps past T at the first step of a forward scan
-        t.d[s] = done && flag < p.T ? done[(int64_t)at * p.done_step] : 0;
-      }
-    }
-  };
-  auto gate_of = [&](const TileT& t, int s, int v) -> A {
-    const A a = MODE == kGateConst ? A(p.decay) : A((typename AccOf<G>::type)t.g[MODE == kGateConst ? 0 : s].v[MODE == kGateChannel ? v : 0]);
-    return t.d[s] ? A(0) : a;
-  };
-
   int buf = 0;
   for (uint64_t tile = i0; tile < i1; tile += (uint64_t)W * kSteps) {
     const uint64_t i = tile + (uint64_t)w * kSteps;
-    TileT t;
-    take(t, i);
-    if (W > 1 || REDUCE) {
-      A rp[VEC], rh[VEC];
+    const int n = i >= i1 ? 0 : i1 - i < kSteps ? (int)(i1 - i) : kSteps;  // steps of this wave's run
+    Pack<X, VEC> tx[kSteps];
+    Pack<G, GV> tg[kSteps];
+    Flags flags(p, e, e0, lane, i, n);
 #pragma unroll
-      for (int v = 0; v < VEC; ++v) rp[v] = A(1), rh[v] = A(0);
-#pragma unroll
-      for (int s = 0; s < kSteps; ++s)
-        if (i + s < i1)
-#pragma unroll
-          for (int v = 0; v < VEC; ++v) {
-            const A a = gate_of(t, s, v);
-            rp[v] *= a;
-            rh[v] = step(a, rh[v], A(t.x[s].v[v]));
-          }
-#pragma unroll
-      for (int v = 0; v < VEC; ++v) fold[buf][w][0][v][lane] = rp[v], fold[buf][w][1][v][lane] = rh[v];
-      if (W > 1) __syncthreads();
+    for (int s = 0; s < kSteps; ++s) {  // steps past the end read the last one that exists: every load is issued, none is waited for
+      const int64_t at = (int64_t)(i + s < i1 ? i + s : i1 - 1);
+      tx[s] = load<X, VEC>(x + at * p.x_step);
+      if (MODE != kGateConst) tg[s] = load<G, GV>(gate + at * p.gate_step);
     }
+    const uint32_t cut = flags.bits(p, e, e0, n);
+    const bool plain = n == kSteps && !flags.any;  // uniform: a whole run that no border cuts
+    auto gate_of = [&](int s, int v) -> A { return MODE == kGateConst ? A(p.decay) : A((typename AccOf<G>::type)tg[s].v[GV > 1 ? v : 0]); };
+    // The state along a run.  The quick walk is the bare multiply-add: a state that is not finite stays so to the run's end under it, and
+    // then, as where done cuts the run, the careful walk takes its place, which forgets at a gate of 0.
+    auto careful = [&](int s, int v, A from) -> A {
+      const A a = (cut >> s) & 1 ? A(0) : gate_of(s, v);
+      return step(a, from, A(tx[s].v[v]));
+    };
     A mine[VEC];
 #pragma unroll
     for (int v = 0; v < VEC; ++v) mine[v] = h[v];
     if (W > 1 || REDUCE) {
+      A rp[VEC], rh[VEC];
+#pragma unroll
+      for (int v = 0; v < VEC; ++v) rp[v] = A(1), rh[v] = A(0);
+      bool odd = !plain;
+      if (plain) {
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s)
+#pragma unroll
+          for (int v = 0; v < VEC; ++v) {
+            if (MODE != kGateHead || v == 0) rp[v] *= gate_of(s, v);
+            rh[v] = fma_(gate_of(s, v), rh[v], A(tx[s].v[v]));
+          }
+        bool bad = false;
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) {
+          if (MODE == kGateHead && v > 0) rp[v] = rp[0];
+          bad |= !finite(rh[v]);
+        }
+        odd = __any(bad);
+      }
+      if (odd) {
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) rp[v] = A(1), rh[v] = A(0);
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s)
+          if (s < n)
+#pragma unroll
+            for (int v = 0; v < VEC; ++v) {
+              rp[v] *= (cut >> s) & 1 ? A(0) : gate_of(s, v);
+              rh[v] = careful(s, v, rh[v]);
+            }
+      }
+#pragma unroll
+      for (int v = 0; v < VEC; ++v) fold[buf][w][0][v][lane] = rp[v], fold[buf][w][1][v][lane] = rh[v];
+      if (W > 1) __syncthreads();
 #pragma unroll
       for (int k = 0; k < W; ++k) {
         if (k == w)
@@ -110,25 +120,48 @@ template <class X, class G, int MODE, int VEC, int W, bool REDUCE> __global__ __
       }
       buf ^= W > 1;
     }
-    if (!REDUCE) {
-      if (p.saved && i < i1 && live)
+    if (REDUCE) continue;
+    if (p.saved && n > 0 && live)
 #pragma unroll
-        for (int v = 0; v < VEC; ++v) p.saved[(i / kSteps) * (uint64_t)p.cols * VEC + ch + v] = (float)mine[v];
+      for (int v = 0; v < VEC; ++v) p.saved[(i / kSteps) * (uint64_t)p.cols * VEC + ch + v] = (float)mine[v];
+    A at[VEC];
+    bool odd = !plain;
+    if (plain) {
+#pragma unroll
+      for (int v = 0; v < VEC; ++v) at[v] = mine[v];
+#pragma unroll
+      for (int s = 0; s < kSteps; ++s) {
+        Pack<X, VEC> o;
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) {
+          at[v] = fma_(gate_of(s, v), at[v], A(tx[s].v[v]));
+          o.v[v] = (X)at[v];
+        }
+        if (live) store(y + (int64_t)(i + s) * p.y_step, o);
+      }
+      bool bad = false;
+#pragma unroll
+      for (int v = 0; v < VEC; ++v) bad |= !finite(at[v]);
+      odd = __any(bad);
+    }
+    if (odd) {
+#pragma unroll
+      for (int v = 0; v < VEC; ++v) at[v] = mine[v];
 #pragma unroll
       for (int s = 0; s < kSteps; ++s)
-        if (i + s < i1) {
+        if (s < n) {
           Pack<X, VEC> o;
 #pragma unroll
           for (int v = 0; v < VEC; ++v) {
-            mine[v] = step(gate_of(t, s, v), mine[v], A(t.x[s].v[v]));
-            o.v[v] = (X)mine[v];
+            at[v] = careful(s, v, at[v]);
+            o.v[v] = (X)at[v];
           }
           if (live) store(y + (int64_t)(i + s) * p.y_step, o);
         }
-      if (W == 1)
-#pragma unroll
-        for (int v = 0; v < VEC; ++v) h[v] = mine[v];
     }
+    if (W == 1)
+#pragma unroll
+      for (int v = 0; v < VEC; ++v) h[v] = at[v];
   }
   if (!live || w != 0) return;
   if (REDUCE) {
@@ -137,7 +170,7 @@ template <class X, class G, int MODE, int VEC, int W, bool REDUCE> __global__ __
     for (int v = 0; v < VEC; ++v) part[v] = P[v], part[(uint64_t)p.cols * VEC + v] = h[v];
   } else if (p.last && blockIdx.y + 1 == gridDim.y) {
     // forward in time the flag of the last step closes the border behind it
-    const bool cut = done && p.cut_off < 0 && p.T > 0 && done[(int64_t)p.T * p.done_step];
+    const bool cut = p.flags && p.cut_off < 0 && p.T > 0 && p.done[(int64_t)e * p.done_row + (int64_t)(p.T - 1) * p.done_step];
 #pragma unroll
     for (int v = 0; v < VEC; ++v) ((A*)p.last)[ch + v] = cut ? A(0) : h[v];
   }
@@ -145,7 +178,7 @@ template <class X, class G, int MODE, int VEC, int W, bool REDUCE> __global__ __
 
 template <class X, class G, int MODE, int VEC> static hipError_t go(const ScanParams& p, hipStream_t stream) {
   const dim3 grid((p.cols + kWave - 1) / kWave, p.chunks);
-  if (p.T <= kSteps) {
+  if (p.waves == 1) {
     k_scan<X, G, MODE, VEC, 1, false><<<grid, kWave, 0, stream>>>(p);
     return hipGetLastError();
   }
@@ -158,7 +191,8 @@ template <class X, class G, int MODE, int VEC> static hipError_t go(const ScanPa
 }
 
 template <class X, class G, int MODE> static hipError_t vecs(const ScanParams& p, int vec, hipStream_t s) {
-  if (vec == 2) return go<X, G, MODE, 2>(p, s);
+  if (sizeof(X) == 2 && vec == 4) return go<X, G, MODE, sizeof(X) == 2 ? 4 : 1>(p, s);
+  if (sizeof(X) <= 4 && vec == 2) return go<X, G, MODE, sizeof(X) <= 4 ? 2 : 1>(p, s);
   return go<X, G, MODE, 1>(p, s);
 }
 template <class X, class G> static hipError_t modes(const ScanParams& p, int mode, int vec, hipStream_t s) {

@@ -14,15 +14,8 @@ namespace cp {
 
 constexpr int kSteps = CE_SCAN_SAVED_STEPS;
 
-template <class X, class G, int MODE, int VEC> struct GradTile {
-  static constexpr int GV = MODE == kGateChannel ? VEC : 1;
-  Pack<X, VEC> x[kSteps], dy[kSteps];
-  Pack<G, GV> g[MODE == kGateConst ? 1 : kSteps];
-  uint8_t d[kSteps];
-};
-
 template <class X, class G, int MODE, int VEC, int W, bool REDUCE> __global__ __launch_bounds__(kWave * W) void k_scan_grad(ScanParams p) {
-  typedef GradTile<X, G, MODE, VEC> TileT;
+  constexpr int GV = MODE == kGateChannel ? VEC : 1;
   __shared__ float fold[W > 1 ? 2 : 1][W][2][VEC][kWave];
   const int lane = threadIdx.x & 63, w = W > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : 0;
   const uint32_t slot = blockIdx.x * kWave + lane;
@@ -30,20 +23,20 @@ template <class X, class G, int MODE, int VEC, int W, bool REDUCE> __global__ __
   bool live;
   if (MODE == kGateHead) {  // `seg` lanes to a head of head / VEC columns
     const uint32_t group = slot / p.seg, in = (slot % p.seg) * VEC;
-    live = in < p.head && group < p.cols / (p.head / VEC);
-    e = group / p.heads;
-    head = group % p.heads;
-    c = head * p.head + in;
+    live = in < p.head && group < p.rows * p.heads;
+    const uint32_t g = group < p.rows * p.heads ? group : 0;  // lanes past the end read a column that exists, write nothing and add 0
+    e = g / p.heads;
+    head = g % p.heads;
+    c = head * p.head + (in < p.head ? in : 0);
   } else {
     live = slot < p.cols;
-    e = slot / p.row_cols;
-    c = (slot % p.row_cols) * VEC;
+    e = live ? slot / p.row_cols : 0;
+    c = live ? (slot % p.row_cols) * VEC : 0;
   }
-  if (!live) e = 0, c = 0, head = 0;  // lanes past the end read a column that exists, write nothing and add 0
+  const uint32_t e0 = __builtin_amdgcn_readfirstlane(e);
   const X* x = (const X*)p.x + (int64_t)e * p.x_row + c;
   const G* gate = (const G*)p.gate;
   if (MODE != kGateConst) gate += (int64_t)e * p.gate_row + (MODE == kGateHead ? head : c);
-  const uint8_t* done = p.done ? p.done + (int64_t)e * p.done_row + (int64_t)p.cut_off * p.done_step : nullptr;
   const uint64_t EC = (uint64_t)p.cols * VEC, ch = (uint64_t)e * p.row_cols * VEC + c;
   const X* dy = (const X*)p.dy + ch;
   X* dx = (X*)p.dx + ch;
@@ -54,7 +47,7 @@ template <class X, class G, int MODE, int VEC, int W, bool REDUCE> __global__ __
 #pragma unroll
   for (int v = 0; v < VEC; ++v) R[v] = 0.f, P[v] = 1.f;
   if (!REDUCE) {
-    const bool cut = done && p.cut_off < 0 && p.T > 0 && done[(int64_t)p.T * p.done_step];
+    const bool cut = p.flags && p.cut_off < 0 && p.T > 0 && p.done[(int64_t)e * p.done_row + (int64_t)(p.T - 1) * p.done_step];
     if (p.dlast && !cut)
 #pragma unroll
       for (int v = 0; v < VEC; ++v) R[v] = ((const float*)p.dlast)[ch + v];
@@ -64,51 +57,75 @@ template <class X, class G, int MODE, int VEC, int W, bool REDUCE> __global__ __
       for (int v = 0; v < VEC; ++v) R[v] = apply(part[(uint64_t)(k - 1) * 2 * EC + v], part[((uint64_t)(k - 1) * 2 + 1) * EC + v], R[v]);
   }
 
-  auto take = [&](TileT& t, uint64_t i) {
-#pragma unroll
-    for (int s = 0; s < kSteps; ++s) {
-      const uint64_t at = i + s;
-      if (at < i1) {
-        if (!REDUCE) t.x[s] = load<X, VEC>(x + (int64_t)at * p.x_step);
-        if (p.dy) t.dy[s] = load<X, VEC>(dy + (int64_t)at * p.y_step);
-        if (MODE != kGateConst) t.g[MODE == kGateConst ? 0 : s] = load<G, TileT::GV>(gate + (int64_t)at * p.gate_step);
-        const uint64_t flag = at + p.cut_off;
-        t.d[s] = done && flag < p.T ? done[(int64_t)at * p.done_step] : 0;
-      }
-    }
-  };
-  auto gate_of = [&](const TileT& t, int s, int v) -> float {
-    const float a = MODE == kGateConst ? (float)p.decay : (float)t.g[MODE == kGateConst ? 0 : s].v[MODE == kGateChannel ? v : 0];
-    return t.d[s] ? 0.f : a;
-  };
-
   int buf = 0;
   const uint64_t span = (uint64_t)W * kSteps, tiles = i1 > i0 ? (i1 - i0 + span - 1) / span : 0;
-  for (uint64_t n = tiles; n-- > 0;) {
-    const uint64_t i = i0 + n * span + (uint64_t)w * kSteps;
-    TileT t;
-    take(t, i);
+  for (uint64_t m = tiles; m-- > 0;) {
+    const uint64_t i = i0 + m * span + (uint64_t)w * kSteps;
+    const int n = i >= i1 ? 0 : i1 - i < kSteps ? (int)(i1 - i) : kSteps;  // steps of this wave's run
+    Pack<X, VEC> tx[kSteps], ty[kSteps];
+    Pack<G, GV> tg[kSteps];
+    float from[VEC];
+    Flags flags(p, e, e0, lane, i, n);
+    if (!REDUCE)
+#pragma unroll
+      for (int v = 0; v < VEC; ++v) from[v] = p.saved[((n ? i : i1 - 1) / kSteps) * EC + ch + v];
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) {  // steps past the end read the last one that exists
+      const int64_t at = (int64_t)(i + s < i1 ? i + s : i1 - 1);
+      if (!REDUCE) tx[s] = load<X, VEC>(x + at * p.x_step);
+      if (p.dy) ty[s] = load<X, VEC>(dy + at * p.y_step);
+      if (MODE != kGateConst) tg[s] = load<G, GV>(gate + at * p.gate_step);
+    }
+    if (!p.dy)
+#pragma unroll
+      for (int s = 0; s < kSteps; ++s)
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) ty[s].v[v] = (X)0.f;
+    const uint32_t cut = flags.bits(p, e, e0, n);
+    const bool plain = n == kSteps && !flags.any;
+    auto gate_of = [&](int s, int v) -> float { return MODE == kGateConst ? (float)p.decay : (float)tg[s].v[GV > 1 ? v : 0]; };
+    auto cut_gate = [&](int s, int v) -> float { return (cut >> s) & 1 ? 0.f : gate_of(s, v); };
+    float mine[VEC];
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) mine[v] = R[v];
+    // As in the forward pass: a quick walk that the careful one replaces where done cuts the run or a value is not finite.
     if (W > 1 || REDUCE) {
       float rp[VEC], rq[VEC];
 #pragma unroll
       for (int v = 0; v < VEC; ++v) rp[v] = 1.f, rq[v] = 0.f;
+      bool odd = !plain;
+      if (plain) {
 #pragma unroll
-      for (int s = kSteps - 1; s >= 0; --s)
-        if (i + s < i1)
+        for (int s = kSteps - 1; s >= 0; --s)
 #pragma unroll
           for (int v = 0; v < VEC; ++v) {
-            const float a = gate_of(t, s, v), gt = (p.dy ? (float)t.dy[s].v[v] : 0.f) + rq[v];
-            rp[v] *= a;
-            rq[v] = a == 0.f ? 0.f : a * gt;
+            if (MODE != kGateHead || v == 0) rp[v] *= gate_of(s, v);
+            rq[v] = gate_of(s, v) * ((float)ty[s].v[v] + rq[v]);
           }
+        bool bad = false;
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) {
+          if (MODE == kGateHead && v > 0) rp[v] = rp[0];
+          bad |= !finite(rq[v]);
+        }
+        odd = __any(bad);
+      }
+      if (odd) {
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) rp[v] = 1.f, rq[v] = 0.f;
+#pragma unroll
+        for (int s = kSteps - 1; s >= 0; --s)
+          if (s < n)
+#pragma unroll
+            for (int v = 0; v < VEC; ++v) {
+              const float a = cut_gate(s, v);
+              rp[v] *= a;
+              rq[v] = a == 0.f ? 0.f : a * ((float)ty[s].v[v] + rq[v]);
+            }
+      }
 #pragma unroll
       for (int v = 0; v < VEC; ++v) fold[buf][w][0][v][lane] = rp[v], fold[buf][w][1][v][lane] = rq[v];
       if (W > 1) __syncthreads();
-    }
-    float mine[VEC];
-#pragma unroll
-    for (int v = 0; v < VEC; ++v) mine[v] = R[v];
-    if (W > 1 || REDUCE) {
 #pragma unroll
       for (int k = W - 1; k >= 0; --k) {
         if (k == w)
@@ -123,59 +140,94 @@ template <class X, class G, int MODE, int VEC, int W, bool REDUCE> __global__ __
       buf ^= W > 1;
     }
     if (REDUCE) continue;
-    float k[kSteps][VEC];  // the state that each step multiplies
-    if (i < i1) {
-      float h[VEC];
+    auto emit = [&](int s, const float (&gt)[VEC], const float (&k)[VEC]) {
+      Pack<X, VEC> o;
 #pragma unroll
-      for (int v = 0; v < VEC; ++v) h[v] = p.saved[(i / kSteps) * EC + ch + v];
+      for (int v = 0; v < VEC; ++v) o.v[v] = (X)gt[v];
+      if (live && p.dx) store(dx + (int64_t)(i + s) * p.y_step, o);
+      if (!p.dgate) return;
+      if (MODE == kGateChannel) {
+        Pack<G, VEC> q;
 #pragma unroll
-      for (int s = 0; s < kSteps; ++s)
-        if (i + s < i1)
+        for (int v = 0; v < VEC; ++v) q.v[v] = (G)(gt[v] * k[v]);
+        if (live) store((G*)p.dgate + ch + (int64_t)(i + s) * p.dgate_step, q);
+      } else if (MODE == kGateHead) {
+        float sum = 0.f;
 #pragma unroll
-          for (int v = 0; v < VEC; ++v) {
-            k[s][v] = t.d[s] ? 0.f : h[v];
-            h[v] = step(gate_of(t, s, v), h[v], (float)t.x[s].v[v]);
-          }
-    }
-#pragma unroll
-    for (int s = kSteps - 1; s >= 0; --s)
-      if (i + s < i1) {
-        Pack<X, VEC> o;
-        float da[VEC];
-#pragma unroll
-        for (int v = 0; v < VEC; ++v) {
-          const float a = gate_of(t, s, v), gt = (p.dy ? (float)t.dy[s].v[v] : 0.f) + mine[v];
-          mine[v] = a == 0.f ? 0.f : a * gt;
-          o.v[v] = (X)gt;
-          da[v] = live ? gt * k[s][v] : 0.f;
-        }
-        if (live && p.dx) store(dx + (int64_t)(i + s) * p.y_step, o);
-        if (!p.dgate) continue;
-        if (MODE == kGateChannel) {
-          Pack<G, VEC> q;
-#pragma unroll
-          for (int v = 0; v < VEC; ++v) q.v[v] = (G)da[v];
-          if (live) store((G*)p.dgate + ch + (int64_t)(i + s) * p.dgate_step, q);
-        } else if (MODE == kGateHead) {
-          float sum = da[0];
-#pragma unroll
-          for (int v = 1; v < VEC; ++v) sum += da[v];
-          const uint32_t width = p.seg < kWave ? p.seg : kWave;
-          for (uint32_t m = width / 2; m > 0; m >>= 1) sum += __shfl_xor(sum, (int)m);
-          if (live && (lane & (width - 1)) == 0) {
-            const uint64_t at = (uint64_t)e * p.heads + head;
-            if (p.slabs == 1) {
-              ((G*)p.dgate)[at + (int64_t)(i + s) * p.dgate_step] = (G)sum;
-            } else {
-              const uint64_t TEH = p.T * (uint64_t)(p.cols / p.row_cols) * p.heads;
-              p.slab[((slot % p.seg) / kWave) * TEH + (i + s) * (uint64_t)(p.cols / p.row_cols) * p.heads + at] = sum;
-            }
+        for (int v = 0; v < VEC; ++v) sum = fma_(gt[v], k[v], sum);
+        if (!live) sum = 0.f;
+        const uint32_t width = p.seg < kWave ? p.seg : kWave;
+        for (uint32_t j = width / 2; j > 0; j >>= 1) sum += __shfl_xor(sum, (int)j);
+        if (live && (lane & (width - 1)) == 0) {
+          const uint64_t at = (uint64_t)e * p.heads + head;
+          if (p.slabs == 1) {
+            ((G*)p.dgate)[at + (int64_t)(i + s) * p.dgate_step] = (G)sum;
+          } else {
+            const uint64_t EH = (uint64_t)p.rows * p.heads;
+            p.slab[((slot % p.seg) / kWave) * p.T * EH + (i + s) * EH + at] = sum;
           }
         }
       }
-    if (W == 1)
+    };
+    float k[kSteps][VEC];  // the state that each step multiplies
+    bool odd = !plain;
+    if (plain) {
+      float h[VEC], r[VEC];
 #pragma unroll
-      for (int v = 0; v < VEC; ++v) R[v] = mine[v];
+      for (int v = 0; v < VEC; ++v) h[v] = from[v], r[v] = mine[v];
+#pragma unroll
+      for (int s = 0; s < kSteps; ++s)
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) {
+          k[s][v] = h[v];
+          h[v] = fma_(gate_of(s, v), h[v], (float)tx[s].v[v]);
+        }
+#pragma unroll
+      for (int s = kSteps - 1; s >= 0; --s) {
+        float gt[VEC];
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) {
+          gt[v] = (float)ty[s].v[v] + r[v];
+          r[v] = gate_of(s, v) * gt[v];
+        }
+        emit(s, gt, k[s]);
+      }
+      bool bad = false;
+#pragma unroll
+      for (int v = 0; v < VEC; ++v) bad |= !finite(h[v]) || !finite(r[v]);
+      odd = __any(bad);
+      if (W == 1 && !odd)
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) R[v] = r[v];
+    }
+    if (odd) {
+      float h[VEC], r[VEC];
+#pragma unroll
+      for (int v = 0; v < VEC; ++v) h[v] = from[v], r[v] = mine[v];
+#pragma unroll
+      for (int s = 0; s < kSteps; ++s)
+        if (s < n)
+#pragma unroll
+          for (int v = 0; v < VEC; ++v) {
+            k[s][v] = (cut >> s) & 1 ? 0.f : h[v];
+            h[v] = step(cut_gate(s, v), h[v], (float)tx[s].v[v]);
+          }
+#pragma unroll
+      for (int s = kSteps - 1; s >= 0; --s)
+        if (s < n) {
+          float gt[VEC];
+#pragma unroll
+          for (int v = 0; v < VEC; ++v) {
+            const float a = cut_gate(s, v);
+            gt[v] = (float)ty[s].v[v] + r[v];
+            r[v] = a == 0.f ? 0.f : a * gt[v];
+          }
+          emit(s, gt, k[s]);
+        }
+      if (W == 1)
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) R[v] = r[v];
+    }
   }
   if (!live || w != 0) return;
   if (REDUCE) {
@@ -190,7 +242,7 @@ template <class X, class G, int MODE, int VEC, int W, bool REDUCE> __global__ __
 
 // [slabs][T][E][H] partial sums -> dgate, in slab order; `i` counts processed steps
 template <class G> __global__ __launch_bounds__(256) void k_scan_grad_slabs(ScanParams p) {
-  const uint64_t EH = (uint64_t)(p.cols / p.row_cols) * p.heads, n = p.T * EH;
+  const uint64_t EH = (uint64_t)p.rows * p.heads, n = p.T * EH;
   for (uint64_t j = (uint64_t)blockIdx.x * 256 + threadIdx.x; j < n; j += (uint64_t)gridDim.x * 256) {
     float sum = p.slab[j];
     for (uint32_t s = 1; s < p.slabs; ++s) sum += p.slab[(uint64_t)s * n + j];
@@ -199,9 +251,9 @@ template <class G> __global__ __launch_bounds__(256) void k_scan_grad_slabs(Scan
 }
 
 template <class X, class G, int MODE, int VEC> static hipError_t go(const ScanParams& p, hipStream_t stream) {
-  const uint64_t slots = MODE == kGateHead ? (uint64_t)(p.cols / (p.head / VEC)) * p.seg : p.cols;
+  const uint64_t slots = MODE == kGateHead ? (uint64_t)p.rows * p.heads * p.seg : p.cols;
   const dim3 grid((uint32_t)((slots + kWave - 1) / kWave), p.chunks);
-  if (p.T <= kSteps) {
+  if (p.waves == 1) {
     k_scan_grad<X, G, MODE, VEC, 1, false><<<grid, kWave, 0, stream>>>(p);
   } else {
     if (p.chunks > 1) {
@@ -212,14 +264,14 @@ template <class X, class G, int MODE, int VEC> static hipError_t go(const ScanPa
   }
   if (hipError_t e = hipGetLastError()) return e;
   if (MODE == kGateHead && p.dgate && p.slabs > 1 && p.T > 0) {
-    const uint64_t n = p.T * (uint64_t)(p.cols / p.row_cols) * p.heads, blocks = (n + 255) / 256;
+    const uint64_t n = p.T * (uint64_t)p.rows * p.heads, blocks = (n + 255) / 256;
     k_scan_grad_slabs<G><<<(uint32_t)(blocks < 4096 ? blocks : 4096), 256, 0, stream>>>(p);
   }
   return hipGetLastError();
 }
 
 template <class X, class G, int MODE> static hipError_t vecs(const ScanParams& p, int vec, hipStream_t s) {
-  if (vec == 2) return go<X, G, MODE, 2>(p, s);
+  if (sizeof(X) == 2 && vec == 2) return go<X, G, MODE, sizeof(X) == 2 ? 2 : 1>(p, s);
   return go<X, G, MODE, 1>(p, s);
 }
 template <class X, class G> static hipError_t modes(const ScanParams& p, int mode, int vec, hipStream_t s) {
