@@ -1,5 +1,6 @@
 // cp_api.hip — host side of the C-ABI in include/contracts_policy.h: checks every argument before anything is launched, names
 // the launch's shape, never throws, never allocates and never synchronises.
+#include <algorithm>
 #include <cmath>
 #include <cstdarg>
 #include <cstdio>
@@ -74,6 +75,10 @@ int check_scan(const ce_scan* s) {
   const uint64_t b = size_of(s->dtype), a = s->dtype == CE_F64 ? 8 : 4;
   if (!aligned(s->x, b) || !aligned(s->y, b) || !aligned(s->state, a) || !aligned(s->last, a) || !aligned(s->saved, 4) || (s->gate && !aligned(s->gate, size_of(s->gate_dtype))))
     return refuse("linear_scan: a pointer is not aligned to its type");
+  // a wave's lanes reach each other by 32-bit offsets: rows that far apart exist only where short rows are very long in time
+  const int64_t span = std::min<int64_t>((int64_t)s->rows - 1, 255 / (int64_t)s->channels + 1), most = (int64_t)((1ull << 32) / 8);
+  for (int64_t row : {s->x_row, s->gate ? s->gate_row : 0})
+    if (row < 0 || (span && row > (most - (int64_t)kMost) / span)) return refuse("linear_scan: rows lie too far apart for a wave; lay x and gate out time-major");
   return CE_OK;
 }
 
@@ -168,7 +173,7 @@ uint64_t part_bytes(const Plan& o, uint32_t dtype) {
   return o.p.chunks > 1 ? (uint64_t)(o.p.chunks - 1) * 2 * o.p.cols * o.vec * (dtype == CE_F64 ? 8 : 4) : 0;
 }
 uint64_t slab_bytes(const Plan& o, const ce_scan* s, const ce_scan_grad* g) {
-  return g->dgate && o.p.slabs > 1 ? (uint64_t)o.p.slabs * s->steps * s->rows * s->heads * 4 : 0;
+  return s->gate && o.p.slabs > 1 ? (uint64_t)o.p.slabs * s->steps * s->rows * s->heads * 4 : 0;
 }
 
 }  // namespace
@@ -206,11 +211,12 @@ static int check_scan_grad(const ce_scan* s, const ce_scan_grad* g) {
   if (!g) return refuse("null ce_scan_grad");
   if (!s) return refuse("null ce_scan");
   ce_scan t = *s;
-  if (!t.y) t.y = g->dx ? g->dx : const_cast<void*>(t.x);  // the backward pass reads no y
+  t.y = const_cast<void*>(t.x);  // the backward pass reads no y
   if (int rc = check_scan(&t)) return rc;
   if (s->dtype == CE_F64) return refuse("linear_scan: double has no backward pass");
   if (s->rows * s->channels == 0) return CE_OK;
   if (s->steps && !s->saved) return refuse("linear_scan_backward: the forward call's saved states are missing");
+  if (s->steps && (!g->dy || !g->dx || (s->gate && !g->dgate))) return refuse("linear_scan_backward: null dy, dx or dgate");
   const uint64_t b = size_of(s->dtype);
   if (!aligned(g->dy, b) || !aligned(g->dx, b) || !aligned(g->dlast, 4) || !aligned(g->dstate, 4) || (s->gate && !aligned(g->dgate, size_of(s->gate_dtype))))
     return refuse("linear_scan_backward: a pointer is not aligned to its type");

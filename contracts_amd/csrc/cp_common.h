@@ -11,12 +11,29 @@ typedef __bf16 bf16;
 typedef _Float16 f16;
 constexpr int kWave = 64;
 
-// A lane's run of VEC neighbouring elements, moved as one access (the host picks VEC by the alignment of every array involved).
+// A lane's run of N neighbouring elements, moved as one access (the host picks N by the alignment of every array involved).  Addresses are a
+// base that the whole wave shares (scalar registers) and a lane's own 32-bit offset in bytes, so walking the time axis costs no
+// vector arithmetic; `hold` keeps a running base a running base, where the compiler would rather keep one for every step.
 template <class T, int N> struct alignas(sizeof(T) * N) Pack {
   T v[N];
 };
-template <class T, int N> __device__ __forceinline__ Pack<T, N> load(const T* p) { return *reinterpret_cast<const Pack<T, N>*>(p); }
-template <class T, int N> __device__ __forceinline__ void store(T* p, const Pack<T, N>& v) { *reinterpret_cast<Pack<T, N>*>(p) = v; }
+template <int BYTES> struct Raw;
+template <> struct Raw<1> { typedef uint8_t type; };
+template <> struct Raw<2> { typedef uint16_t type; };
+template <> struct Raw<4> { typedef uint32_t type; };
+template <> struct Raw<8> { typedef uint32_t type __attribute__((ext_vector_type(2))); };
+template <> struct Raw<16> { typedef uint32_t type __attribute__((ext_vector_type(4))); };
+#define CP_GLOBAL __attribute__((address_space(1)))
+
+template <class T, int N> __device__ __forceinline__ Pack<T, N> load(uint64_t base, uint32_t off) {
+  typedef typename Raw<sizeof(T) * N>::type R;
+  return __builtin_bit_cast(Pack<T, N>, *(const CP_GLOBAL R*)(base + off));
+}
+template <class T, int N> __device__ __forceinline__ void store(uint64_t base, uint32_t off, const Pack<T, N>& v) {
+  typedef typename Raw<sizeof(T) * N>::type R;
+  *(CP_GLOBAL R*)(base + off) = __builtin_bit_cast(R, v);
+}
+__device__ __forceinline__ void hold(uint64_t& base) { asm volatile("" : "+s"(base)); }
 
 template <class T> struct AccOf { typedef float type; };
 template <> struct AccOf<double> { typedef double type; };
@@ -70,34 +87,30 @@ struct ScanParams {
   float* slab;        // [slabs][T][E][H] where slabs > 1
 };
 
-// The done flags of steps i .. i + n of a wave's run: read ahead with its other loads (constructor), spread to a lane's bits later.
+// The done flags that cut the state ahead of the n steps i, i + 1, .. of a wave's run; a flag ahead of the first step (index -1, forward
+// in time) or past the run cuts nothing.  kFlagsBallot reads with the run's other loads, long before bits() asks.
 struct Flags {
-  uint8_t d[16];
+  uint8_t d = 0;
   bool any = false;
-  __device__ __forceinline__ Flags(const ScanParams& p, uint32_t e, uint32_t e0, int lane, uint64_t i, int n) {
-    d[0] = 0;
-    if (p.flags == kFlagsBallot) {
-      const uint32_t row = e0 + (lane >> 4);
-      const uint64_t flag = i + (lane & 15) + (int64_t)p.cut_off;  // wraps past T ahead of the first step of a forward scan
-      if ((lane & 15) < n && flag < p.T && row < p.rows) d[0] = p.done[(int64_t)row * p.done_row + (int64_t)flag * p.done_step];
-    } else if (p.flags == kFlagsLane) {
-#pragma unroll
-      for (int s = 0; s < 16; ++s) {
-        const uint64_t flag = i + s + (int64_t)p.cut_off;
-        d[s] = 0;
-        if (s < n && flag < p.T) d[s] = p.done[(int64_t)e * p.done_row + (int64_t)flag * p.done_step];
-      }
-    }
+  __device__ __forceinline__ Flags(const ScanParams& p, uint32_t e0, int lane, uint64_t i, int n) {
+    if (p.flags != kFlagsBallot) return;
+    const uint32_t row = e0 + (lane >> 4);
+    const uint64_t flag = i + (lane & 15) + (int64_t)p.cut_off;
+    if ((lane & 15) < n && flag < p.T && row < p.rows) d = p.done[(int64_t)row * p.done_row + (int64_t)flag * p.done_step];
   }
-  __device__ __forceinline__ uint32_t bits(const ScanParams& p, uint32_t e, uint32_t e0, int n) {
+  __device__ __forceinline__ uint32_t bits(const ScanParams& p, uint32_t e, uint32_t e0, uint64_t i, int n) {
     uint32_t cut = 0;
     if (p.flags == kFlagsBallot) {
-      const uint64_t m = __ballot(d[0] != 0);
+      const uint64_t m = __ballot(d != 0);
       any = m != 0;
       cut = (uint32_t)(m >> ((e - e0) * 16)) & 0xffffu;
-    } else if (p.flags == kFlagsLane) {
+    } else if (p.flags == kFlagsLane && n > 0) {
+      const uint8_t* row = p.done + (int64_t)e * p.done_row;
 #pragma unroll
-      for (int s = 0; s < 16; ++s) cut |= (d[s] != 0 ? 1u : 0u) << s;
+      for (int s = 0; s < 16; ++s) {
+        const uint64_t flag = i + (s < n ? s : 0) + (int64_t)p.cut_off, at = flag < p.T ? flag : 0;
+        cut |= (row[(int64_t)at * p.done_step] != 0 && flag < p.T && s < n ? 1u : 0u) << s;
+      }
       any = __any(cut != 0);
     }
     return cut;

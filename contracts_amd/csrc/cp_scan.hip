@@ -19,14 +19,15 @@ template <class X, class G, int MODE, int VEC, int W, bool REDUCE> __global__ __
   __shared__ A fold[W > 1 ? 2 : 1][W][2][VEC][kWave];
   const int lane = threadIdx.x & 63, w = W > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : 0;
   const uint32_t col = blockIdx.x * kWave + lane;
-  const bool live = col < p.cols;
-  const uint32_t colc = live ? col : p.cols - 1;  // lanes past the end read a column that exists and write nothing
+  const uint32_t colc = col < p.cols ? col : p.cols - 1;  // lanes past the end do what the last one does, and write the same
   const uint32_t e = colc / p.row_cols, c = (colc % p.row_cols) * VEC, e0 = __builtin_amdgcn_readfirstlane(e);
-  const X* x = (const X*)p.x + (int64_t)e * p.x_row + c;
-  const G* gate = (const G*)p.gate;
-  if (MODE != kGateConst) gate += (int64_t)e * p.gate_row + (MODE == kGateHead ? c / p.head : c);
   const uint64_t ch = (uint64_t)colc * VEC;  // index in the dense [E][C]
-  X* y = (X*)p.y + ch;
+  // a lane's offsets from row e0 of the strided inputs, from the wave's first channel of the dense arrays
+  const uint32_t x_off = (uint32_t)((int64_t)(e - e0) * p.x_row + c) * (uint32_t)sizeof(X), y_off = (colc - blockIdx.x * kWave) * (uint32_t)(VEC * sizeof(X));
+  const uint32_t g_off = MODE == kGateConst ? 0 : (uint32_t)((int64_t)(e - e0) * p.gate_row + (MODE == kGateHead ? c / p.head : c)) * (uint32_t)sizeof(G);
+  const uint64_t x0 = (uint64_t)((const X*)p.x + (int64_t)e0 * p.x_row), g0 = (uint64_t)((const G*)p.gate + (int64_t)e0 * p.gate_row);
+  const uint64_t y0 = (uint64_t)((X*)p.y + (uint64_t)blockIdx.x * kWave * VEC);
+  const uint64_t x_step = (uint64_t)(p.x_step * (int64_t)sizeof(X)), g_step = (uint64_t)(p.gate_step * (int64_t)sizeof(G)), y_step = (uint64_t)(p.y_step * (int64_t)sizeof(X));
   const uint64_t i0 = blockIdx.y * p.chunk, i1 = i0 + p.chunk < p.T ? i0 + p.chunk : p.T;
 
   A h[VEC];
@@ -52,14 +53,22 @@ template <class X, class G, int MODE, int VEC, int W, bool REDUCE> __global__ __
     const int n = i >= i1 ? 0 : i1 - i < kSteps ? (int)(i1 - i) : kSteps;  // steps of this wave's run
     Pack<X, VEC> tx[kSteps];
     Pack<G, GV> tg[kSteps];
-    Flags flags(p, e, e0, lane, i, n);
+    Flags flags(p, e0, lane, i, n);
+    {
+      const uint64_t first = n ? i : i1 - 1;
+      uint64_t xs = x0 + first * x_step, gs = g0 + first * g_step;
 #pragma unroll
-    for (int s = 0; s < kSteps; ++s) {  // steps past the end read the last one that exists: every load is issued, none is waited for
-      const int64_t at = (int64_t)(i + s < i1 ? i + s : i1 - 1);
-      tx[s] = load<X, VEC>(x + at * p.x_step);
-      if (MODE != kGateConst) tg[s] = load<G, GV>(gate + at * p.gate_step);
+      for (int s = 0; s < kSteps; ++s) {  // steps past the end read the last one that exists: every load is issued, none is waited for
+        tx[s] = load<X, VEC>(xs, x_off);
+        if (MODE != kGateConst) tg[s] = load<G, GV>(gs, g_off);
+        xs += s + 1 < n ? x_step : 0;
+        gs += s + 1 < n ? g_step : 0;
+        hold(xs);
+        hold(gs);
+      }
     }
-    const uint32_t cut = flags.bits(p, e, e0, n);
+    uint64_t ys = y0 + i * y_step;
+    const uint32_t cut = flags.bits(p, e, e0, i, n);
     const bool plain = n == kSteps && !flags.any;  // uniform: a whole run that no border cuts
     auto gate_of = [&](int s, int v) -> A { return MODE == kGateConst ? A(p.decay) : A((typename AccOf<G>::type)tg[s].v[GV > 1 ? v : 0]); };
     // The state along a run.  The quick walk is the bare multiply-add: a state that is not finite stays so to the run's end under it, and
@@ -121,7 +130,7 @@ template <class X, class G, int MODE, int VEC, int W, bool REDUCE> __global__ __
       buf ^= W > 1;
     }
     if (REDUCE) continue;
-    if (p.saved && n > 0 && live)
+    if (p.saved && n > 0)
 #pragma unroll
       for (int v = 0; v < VEC; ++v) p.saved[(i / kSteps) * (uint64_t)p.cols * VEC + ch + v] = (float)mine[v];
     A at[VEC];
@@ -137,7 +146,9 @@ template <class X, class G, int MODE, int VEC, int W, bool REDUCE> __global__ __
           at[v] = fma_(gate_of(s, v), at[v], A(tx[s].v[v]));
           o.v[v] = (X)at[v];
         }
-        if (live) store(y + (int64_t)(i + s) * p.y_step, o);
+        store(ys, y_off, o);
+        ys += y_step;
+        hold(ys);
       }
       bool bad = false;
 #pragma unroll
@@ -145,6 +156,7 @@ template <class X, class G, int MODE, int VEC, int W, bool REDUCE> __global__ __
       odd = __any(bad);
     }
     if (odd) {
+      ys = y0 + i * y_step;
 #pragma unroll
       for (int v = 0; v < VEC; ++v) at[v] = mine[v];
 #pragma unroll
@@ -156,14 +168,16 @@ template <class X, class G, int MODE, int VEC, int W, bool REDUCE> __global__ __
             at[v] = careful(s, v, at[v]);
             o.v[v] = (X)at[v];
           }
-          if (live) store(y + (int64_t)(i + s) * p.y_step, o);
+          store(ys, y_off, o);
+          ys += y_step;
+          hold(ys);
         }
     }
     if (W == 1)
 #pragma unroll
       for (int v = 0; v < VEC; ++v) h[v] = at[v];
   }
-  if (!live || w != 0) return;
+  if (w != 0) return;
   if (REDUCE) {
     A* part = (A*)p.part + (uint64_t)blockIdx.y * 2 * p.cols * VEC + ch;
 #pragma unroll

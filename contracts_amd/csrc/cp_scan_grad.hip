@@ -24,22 +24,28 @@ template <class X, class G, int MODE, int VEC, int W, bool REDUCE> __global__ __
   if (MODE == kGateHead) {  // `seg` lanes to a head of head / VEC columns
     const uint32_t group = slot / p.seg, in = (slot % p.seg) * VEC;
     live = in < p.head && group < p.rows * p.heads;
-    const uint32_t g = group < p.rows * p.heads ? group : 0;  // lanes past the end read a column that exists, write nothing and add 0
+    const uint32_t g = group < p.rows * p.heads ? group : p.rows * p.heads - 1;
     e = g / p.heads;
     head = g % p.heads;
-    c = head * p.head + (in < p.head ? in : 0);
+    c = head * p.head + (live ? in : 0);
   } else {
     live = slot < p.cols;
-    e = live ? slot / p.row_cols : 0;
-    c = live ? (slot % p.row_cols) * VEC : 0;
+    const uint32_t col = live ? slot : p.cols - 1;
+    e = col / p.row_cols;
+    c = (col % p.row_cols) * VEC;
   }
+  // lanes that are not live do what another one does and write the same; none lies ahead of the wave's first row e0, from which all count
   const uint32_t e0 = __builtin_amdgcn_readfirstlane(e);
-  const X* x = (const X*)p.x + (int64_t)e * p.x_row + c;
-  const G* gate = (const G*)p.gate;
-  if (MODE != kGateConst) gate += (int64_t)e * p.gate_row + (MODE == kGateHead ? head : c);
   const uint64_t EC = (uint64_t)p.cols * VEC, ch = (uint64_t)e * p.row_cols * VEC + c;
-  const X* dy = (const X*)p.dy + ch;
-  X* dx = (X*)p.dx + ch;
+  // a lane's offsets from row e0
+  const uint32_t x_off = (uint32_t)((int64_t)(e - e0) * p.x_row + c) * (uint32_t)sizeof(X), y_off = ((e - e0) * p.row_cols * VEC + c) * (uint32_t)sizeof(X);
+  const uint32_t g_off = MODE == kGateConst ? 0 : (uint32_t)((int64_t)(e - e0) * p.gate_row + (MODE == kGateHead ? head : c)) * (uint32_t)sizeof(G);
+  const uint32_t dg_off = ((e - e0) * p.row_cols * VEC + c) * (uint32_t)sizeof(G);
+  const uint64_t x0 = (uint64_t)((const X*)p.x + (int64_t)e0 * p.x_row), g0 = (uint64_t)((const G*)p.gate + (int64_t)e0 * p.gate_row);
+  const uint64_t row0 = (uint64_t)e0 * p.row_cols * VEC;
+  const uint64_t dy0 = (uint64_t)((const X*)p.dy + row0), dx0 = (uint64_t)((X*)p.dx + row0), dg0 = (uint64_t)((G*)p.dgate + row0);
+  const uint64_t x_step = (uint64_t)(p.x_step * (int64_t)sizeof(X)), g_step = (uint64_t)(p.gate_step * (int64_t)sizeof(G));
+  const uint64_t y_step = (uint64_t)(p.y_step * (int64_t)sizeof(X)), dg_step = (uint64_t)(p.dgate_step * (int64_t)sizeof(G));
   const uint32_t chunk = blockIdx.y + (REDUCE ? 1 : 0);  // nobody folds chunk 0
   const uint64_t i0 = chunk * p.chunk, i1 = i0 + p.chunk < p.T ? i0 + p.chunk : p.T;
 
@@ -65,23 +71,27 @@ template <class X, class G, int MODE, int VEC, int W, bool REDUCE> __global__ __
     Pack<X, VEC> tx[kSteps], ty[kSteps];
     Pack<G, GV> tg[kSteps];
     float from[VEC];
-    Flags flags(p, e, e0, lane, i, n);
+    Flags flags(p, e0, lane, i, n);
     if (!REDUCE)
 #pragma unroll
       for (int v = 0; v < VEC; ++v) from[v] = p.saved[((n ? i : i1 - 1) / kSteps) * EC + ch + v];
+    {
+      const uint64_t first = n ? i : i1 - 1;
+      uint64_t xs = x0 + first * x_step, gs = g0 + first * g_step, ds = dy0 + first * y_step;
 #pragma unroll
-    for (int s = 0; s < kSteps; ++s) {  // steps past the end read the last one that exists
-      const int64_t at = (int64_t)(i + s < i1 ? i + s : i1 - 1);
-      if (!REDUCE) tx[s] = load<X, VEC>(x + at * p.x_step);
-      if (p.dy) ty[s] = load<X, VEC>(dy + at * p.y_step);
-      if (MODE != kGateConst) tg[s] = load<G, GV>(gate + at * p.gate_step);
+      for (int s = 0; s < kSteps; ++s) {  // steps past the end read the last one that exists
+        if (!REDUCE) tx[s] = load<X, VEC>(xs, x_off);
+        ty[s] = load<X, VEC>(ds, y_off);
+        if (MODE != kGateConst) tg[s] = load<G, GV>(gs, g_off);
+        xs += s + 1 < n ? x_step : 0;
+        gs += s + 1 < n ? g_step : 0;
+        ds += s + 1 < n ? y_step : 0;
+        hold(xs);
+        hold(gs);
+        hold(ds);
+      }
     }
-    if (!p.dy)
-#pragma unroll
-      for (int s = 0; s < kSteps; ++s)
-#pragma unroll
-        for (int v = 0; v < VEC; ++v) ty[s].v[v] = (X)0.f;
-    const uint32_t cut = flags.bits(p, e, e0, n);
+    const uint32_t cut = flags.bits(p, e, e0, i, n);
     const bool plain = n == kSteps && !flags.any;
     auto gate_of = [&](int s, int v) -> float { return MODE == kGateConst ? (float)p.decay : (float)tg[s].v[GV > 1 ? v : 0]; };
     auto cut_gate = [&](int s, int v) -> float { return (cut >> s) & 1 ? 0.f : gate_of(s, v); };
@@ -140,17 +150,21 @@ template <class X, class G, int MODE, int VEC, int W, bool REDUCE> __global__ __
       buf ^= W > 1;
     }
     if (REDUCE) continue;
+    uint64_t os = 0, qs = 0;  // where dx and dgate of the step at hand go; the walk runs backwards
     auto emit = [&](int s, const float (&gt)[VEC], const float (&k)[VEC]) {
       Pack<X, VEC> o;
 #pragma unroll
       for (int v = 0; v < VEC; ++v) o.v[v] = (X)gt[v];
-      if (live && p.dx) store(dx + (int64_t)(i + s) * p.y_step, o);
-      if (!p.dgate) return;
+      store(os, y_off, o);
+      os -= y_step;
+      hold(os);
       if (MODE == kGateChannel) {
         Pack<G, VEC> q;
 #pragma unroll
         for (int v = 0; v < VEC; ++v) q.v[v] = (G)(gt[v] * k[v]);
-        if (live) store((G*)p.dgate + ch + (int64_t)(i + s) * p.dgate_step, q);
+        store(qs, dg_off, q);
+        qs -= dg_step;
+        hold(qs);
       } else if (MODE == kGateHead) {
         float sum = 0.f;
 #pragma unroll
@@ -182,6 +196,8 @@ template <class X, class G, int MODE, int VEC, int W, bool REDUCE> __global__ __
           k[s][v] = h[v];
           h[v] = fma_(gate_of(s, v), h[v], (float)tx[s].v[v]);
         }
+      os = dx0 + (i + kSteps - 1) * y_step;
+      qs = dg0 + (i + kSteps - 1) * dg_step;
 #pragma unroll
       for (int s = kSteps - 1; s >= 0; --s) {
         float gt[VEC];
@@ -212,6 +228,8 @@ template <class X, class G, int MODE, int VEC, int W, bool REDUCE> __global__ __
             k[s][v] = (cut >> s) & 1 ? 0.f : h[v];
             h[v] = step(cut_gate(s, v), h[v], (float)tx[s].v[v]);
           }
+      os = dx0 + (i + (n ? n - 1 : 0)) * y_step;
+      qs = dg0 + (i + (n ? n - 1 : 0)) * dg_step;
 #pragma unroll
       for (int s = kSteps - 1; s >= 0; --s)
         if (s < n) {
@@ -263,7 +281,7 @@ template <class X, class G, int MODE, int VEC> static hipError_t go(const ScanPa
     k_scan_grad<X, G, MODE, VEC, 4, false><<<grid, 4 * kWave, 0, stream>>>(p);
   }
   if (hipError_t e = hipGetLastError()) return e;
-  if (MODE == kGateHead && p.dgate && p.slabs > 1 && p.T > 0) {
+  if (MODE == kGateHead && p.slabs > 1 && p.T > 0) {
     const uint64_t n = p.T * (uint64_t)p.rows * p.heads, blocks = (n + 255) / 256;
     k_scan_grad_slabs<G><<<(uint32_t)(blocks < 4096 ? blocks : 4096), 256, 0, stream>>>(p);
   }

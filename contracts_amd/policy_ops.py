@@ -100,15 +100,15 @@ def _scan_forward(x, gate, state, done, reverse, y, last, want_saved):
     return y, last, saved
 
 
-def _scan_backward(x, gate, done, reverse, saved, dy, dlast, need_x, need_gate, need_state):
+def _scan_backward(x, gate, done, reverse, saved, dy, dlast, need_state):
     L = _lib.load_policy()
     T, E, Ch = x.shape
-    dx = torch.empty((T, E, Ch), dtype=x.dtype, device=x.device) if need_x else None
-    dgate = (torch.empty if x.numel() else torch.zeros)(gate.shape, dtype=gate.dtype, device=x.device) if need_gate else None
+    dx = torch.empty((T, E, Ch), dtype=x.dtype, device=x.device)
+    dgate = (torch.empty if x.numel() else torch.zeros)(gate.shape, dtype=gate.dtype, device=x.device) if isinstance(gate, torch.Tensor) else None
     dstate = torch.empty((E, Ch), dtype=torch.float32, device=x.device) if need_state else None
     s = _scan_struct(x, gate, done, reverse)
     s.saved = _ptr(saved)
-    dy = None if dy is None else dy.contiguous()
+    dy = torch.zeros((T, E, Ch), dtype=x.dtype, device=x.device) if dy is None else dy.contiguous()
     dlast = None if dlast is None else dlast.contiguous()
     g = _lib.CeScanGrad(dy=_ptr(dy), dlast=_ptr(dlast), dx=_ptr(dx), dgate=_ptr(dgate), dstate=_ptr(dstate))
     ws = _workspace(L.ce_linear_scan_backward_workspace, x.device, s, g)
@@ -131,8 +131,8 @@ class _Scan(torch.autograd.Function):
     def backward(ctx, dy, dlast):
         x, gate, done, saved = ctx.saved_tensors
         need = ctx.needs_input_grad
-        dx, dgate, dstate = _scan_backward(x, gate if ctx.const is None else ctx.const, done, ctx.reverse, saved, dy, dlast, need[0], need[1], need[2])
-        return dx, dgate, dstate, None, None
+        dx, dgate, dstate = _scan_backward(x, gate if ctx.const is None else ctx.const, done, ctx.reverse, saved, dy, dlast, need[2])
+        return dx if need[0] else None, dgate if need[1] else None, dstate, None, None
 
 
 def linear_scan(x, gate, state=None, done=None, reverse=False, out=None, state_out=None):
@@ -171,9 +171,10 @@ def linear_scan(x, gate, state=None, done=None, reverse=False, out=None, state_o
         if t is not None:
             _need(not grad, "linear_scan: %s cannot be given where gradients are wanted", name)
             _need(tuple(t.shape) == shape and t.dtype == dtype and t.is_contiguous(), "linear_scan: %s must be a dense %s %s", name, dtype, shape)
-    if x.stride(2) != 1 and Ch > 1:
+    far = (1 << 28) // (255 // max(Ch, 1) + 1)  # rows that far apart are more than a wave's 32-bit offsets
+    if (x.stride(2) != 1 and Ch > 1) or x.stride(1) > far:
         x = x.contiguous()
-    if tensor_gate and gate.stride(2) != 1 and gate.shape[2] > 1:
+    if tensor_gate and ((gate.stride(2) != 1 and gate.shape[2] > 1) or gate.stride(1) > far):
         gate = gate.contiguous()
     in_place = state_out is not None and state is not None and state_out.data_ptr() == state.data_ptr()
     _need(not in_place or state.is_contiguous(), "linear_scan: state_out overlaps an input")

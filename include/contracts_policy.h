@@ -41,7 +41,8 @@ const char* ce_policy_error(void);
  * y is rounded once to its own type and the rounded value is not used again.  T = 0 hands the state on.
  * Types: x and y dtype; gate dtype or CE_F32; state and last float (CE_F64: double throughout, and no backward pass).
  * gate == NULL: the constant `decay`.  state / done / last / saved may be NULL (zeros / none ended / not wanted).
- * `last` may be `state` itself (a state moved on in place); no other overlap of outputs with inputs. */
+ * `last` may be `state` itself (a state moved on in place); no other overlap of outputs with inputs.  x_row and gate_row are not
+ * negative, and rows of under 256 channels lie less than 2^28 elements apart per row that a wave of 256 channels spans. */
 #define CE_SCAN_REVERSE 1u
 #define CE_SCAN_SAVED_STEPS 16 /* saved: float [ceil(T / 16)][E][C], what ce_linear_scan_backward starts its tiles from */
 
@@ -68,11 +69,11 @@ typedef struct ce_scan {
 int ce_linear_scan_workspace(const ce_scan* s, uint64_t* bytes);
 int ce_linear_scan(const ce_scan* s, void* stream);
 
-/* The gradients of y and last (dy [T][E][C] dense, or NULL; dlast [E][C] dense, or NULL) taken back to x, gate and state.  `fwd` describes the
+/* The gradients of y and last (dy [T][E][C] dense; dlast [E][C] dense, or NULL) taken back to x, gate and state.  `fwd` describes the
  * forward call: x, gate, done, strides, `saved` as it was filled (y, last and state are not read).
  *   g_t = dy_t + (the successor's a g, nothing over a border that done closes);  dx = g;  dgate = sum over a head's channels
  *   of g_t k_t;  dstate = a g of the first step
- * dx in dtype, dgate in gate_dtype ([T][E][H] dense, NULL with a constant gate), dstate float; each NULL if not wanted.
+ * dx in dtype, dgate in gate_dtype ([T][E][H] dense, NULL with a constant gate), dstate float (or NULL).
  * Sums run in float, in one fixed order: the same call gives the same bits. */
 typedef struct ce_scan_grad {
   const void* dy;
