@@ -1,203 +1,455 @@
 // cp_logits.hip — scores shaped ahead of a selection (ce_process_logits): penalties for repeated tokens, biases, masks; and the
 // gradients of logits and bias.
 //
-// A block takes a row's run of kChunk tokens: a table in LDS counts the history's tokens that fall into the run (the prompt's
-// only as "seen", the top bit), then the run streams through once: read, penalise, bias, mask, write.
-// Bound by HBM: each score is read once and written once.
+// A block takes a tile of kTile scores: a run of one row's vocabulary, or a whole number of short rows.  A table in LDS counts what the
+// tile's histories hold (the prompt's tokens only as "seen", the top bit), then the tile streams through once, 8 neighbouring
+// scores to a lane: read, penalise, bias, mask, write.  Bound by HBM: each score is read once and written once; a history is
+// read once for every run of its row's vocabulary, from L2.
 #include "cp_common.h"
 
 namespace cp {
 
-constexpr int kBlock = 256, kChunk = 4096;
+constexpr int kBlock = 256, kTile = 4096, kLane = 8;
 constexpr uint32_t kSeen = 0x80000000u;
+constexpr uint32_t kRowsMost = 512;  // short rows of a tile (their parameters lie in LDS too)
 
 struct Row {  // what a row is penalised with
   float repetition, presence, frequency;
-  uint64_t used, prompt;  // how much of its history counts, and how much of that is its prompt
 };
 __device__ __forceinline__ Row row_of(const ce_logits& s, uint64_t r) {
   Row o;
   o.repetition = s.repetition ? s.repetition[r] : (float)s.repetition_all;
   o.presence = s.presence ? s.presence[r] : (float)s.presence_all;
   o.frequency = s.frequency ? s.frequency[r] : (float)s.frequency_all;
-  o.used = s.tokens ? s.history : 0;
-  if (s.lengths) {
-    const int32_t l = s.lengths[r];
-    if (l < 0) o.used = 0;
-    else if ((uint64_t)l < o.used) o.used = l;
-  }
-  o.prompt = 0;
-  if (s.prompt_lengths) {
-    const int32_t l = s.prompt_lengths[r];
-    o.prompt = l > 0 ? l : 0;
-  }
   return o;
 }
-// The token at place i of row r's history, or a number past every vocabulary.
-__device__ __forceinline__ uint64_t token(const ce_logits& s, uint64_t r, uint64_t i) {
-  const int64_t at = (int64_t)r * s.token_row + (int64_t)i * s.token_step;
-  if (s.token_dtype == CE_U8) return ((const uint8_t*)s.tokens)[at];
-  if (s.token_dtype == CE_I32) return (uint64_t)(int64_t)((const int32_t*)s.tokens)[at];
-  return (uint64_t)((const int64_t*)s.tokens)[at];
+// How much of row r's history counts, and how much of that is its prompt.
+__device__ __forceinline__ uint32_t used_of(const ce_logits& s, uint64_t r) {
+  if (!s.tokens) return 0;
+  if (!s.lengths) return (uint32_t)s.history;
+  const int32_t l = s.lengths[r];
+  return l < 0 ? 0u : (uint32_t)l < (uint32_t)s.history ? (uint32_t)l : (uint32_t)s.history;
+}
+__device__ __forceinline__ uint32_t prompt_of(const ce_logits& s, uint64_t r) {
+  if (!s.prompt_lengths) return 0;
+  const int32_t l = s.prompt_lengths[r];
+  return l > 0 ? (uint32_t)l : 0u;
+}
+// The token at place i of row r's history; a number past every vocabulary where it is no token.
+template <class K> __device__ __forceinline__ uint64_t token(const ce_logits& s, uint64_t r, uint32_t i) {
+  return (uint64_t)(int64_t)((const K*)s.tokens)[(int64_t)r * s.token_row + (int64_t)i * s.token_step];
 }
 // The mask's row of row r: -1 = everything is allowed, -2 = nothing is.
 __device__ __forceinline__ int64_t mask_row(const ce_logits& s, uint64_t r) {
   if (!s.mask) return -1;
-  if (!s.mask_index) return (int64_t)(r % s.mask_rows);
+  if (!s.mask_index) return s.mask_rows == s.rows ? (int64_t)r : (int64_t)((uint32_t)r % (uint32_t)s.mask_rows);
   const int32_t m = s.mask_index[r];
   return m < 0 ? -1 : (uint64_t)m < s.mask_rows ? m : -2;
 }
-__device__ __forceinline__ bool allowed(const ce_logits& s, int64_t m, uint64_t v) {
+__device__ __forceinline__ bool allowed(const ce_logits& s, int64_t m, uint32_t v) {
   if (m < 0) return m == -1;
   if (s.mask_dtype == CE_U8) return ((const uint8_t*)s.mask)[(uint64_t)m * s.vocab + v] != 0;
   return (((const uint32_t*)s.mask)[(uint64_t)m * ((s.vocab + 31) / 32) + v / 32] >> (v % 32)) & 1u;
+}
+// 8 neighbouring tokens' permissions as bits; all 8 lie inside the row.
+__device__ __forceinline__ uint32_t allowed8(const ce_logits& s, int64_t m, uint32_t v) {
+  if (m < 0) return m == -1 ? 0xffu : 0u;
+  if (s.mask_dtype == CE_U8) {
+    uint64_t b;
+    __builtin_memcpy(&b, (const uint8_t*)s.mask + (uint64_t)m * s.vocab + v, 8);
+    uint32_t bits = 0;
+#pragma unroll
+    for (int q = 0; q < 8; ++q) bits |= ((b >> (8 * q)) & 0xff ? 1u : 0u) << q;
+    return bits;
+  }
+  const uint32_t* words = (const uint32_t*)s.mask + (uint64_t)m * ((s.vocab + 31) / 32);
+  uint32_t bits = words[v / 32] >> (v % 32);
+  if (v % 32 > 24) bits |= words[v / 32 + 1] << (32 - v % 32);  // the 8 tokens reach into the next word, which the row has
+  return bits & 0xffu;
+}
+// 8 neighbouring elements of any alignment as float.
+template <class T> __device__ __forceinline__ void load8(const T* p, float (&o)[8]) {
+  T t[8];
+  __builtin_memcpy(t, __builtin_assume_aligned(p, alignof(T)), sizeof(t));
+#pragma unroll
+  for (int q = 0; q < 8; ++q) o[q] = (float)t[q];
+}
+template <class T> __device__ __forceinline__ void store8(T* p, const float (&v)[8]) {
+  T t[8];
+#pragma unroll
+  for (int q = 0; q < 8; ++q) t[q] = (T)v[q];
+  __builtin_memcpy(__builtin_assume_aligned(p, alignof(T)), t, sizeof(t));
 }
 __device__ __forceinline__ float bias_at(const ce_logits& s, uint64_t at) {
   if (s.bias_dtype == CE_F32) return ((const float*)s.bias)[at];
   if (s.bias_dtype == CE_BF16) return (float)((const bf16*)s.bias)[at];
   return (float)((const f16*)s.bias)[at];
 }
+__device__ __forceinline__ void bias8(const ce_logits& s, uint64_t at, float (&o)[8]) {
+  if (s.bias_dtype == CE_F32) load8((const float*)s.bias + at, o);
+  else if (s.bias_dtype == CE_BF16) load8((const bf16*)s.bias + at, o);
+  else load8((const f16*)s.bias + at, o);
+}
+__device__ __forceinline__ float penalise(float l, uint32_t entry, const Row& row) {
+  if (!entry) return l;
+  const uint32_t count = entry & ~kSeen;
+  const float z = l > 0.f ? l / row.repetition : l * row.repetition;
+  return count ? z - row.presence - row.frequency * (float)count : z;
+}
 
-template <class X, class O> __global__ __launch_bounds__(kBlock) void k_logits(ce_logits s) {
-  __shared__ uint32_t table[kChunk];
-  const uint64_t r = blockIdx.x, v0 = (uint64_t)blockIdx.y * kChunk;
-  const uint32_t n = (uint32_t)(s.vocab - v0 < kChunk ? s.vocab - v0 : kChunk);
-  const Row row = row_of(s, r);
-  const bool history = row.used > 0;
-  if (history) {
-    for (uint32_t k = threadIdx.x; k < n; k += kBlock) table[k] = 0;
+// ---- a run of one row -----------------------------------------------------------------------------------------------------------
+template <class X, class O, class K> __global__ __launch_bounds__(kBlock) void k_logits_run(ce_logits s, uint64_t row0, uint32_t runs) {
+  __shared__ __attribute__((aligned(16))) uint32_t table[kTile];
+  const uint64_t r = row0 + blockIdx.x / runs;
+  const uint32_t v0 = blockIdx.x % runs * kTile, V = (uint32_t)s.vocab, n = V - v0 < kTile ? V - v0 : kTile;
+  const X* x = (const X*)s.logits + (int64_t)r * s.logits_row + v0;
+  O* o = (O*)s.out + (int64_t)r * s.out_row + v0;
+  float l[kTile / kBlock / kLane][kLane];
+#pragma unroll
+  for (int g = 0; g < kTile / kBlock / kLane; ++g) {  // in flight while the history is counted
+    const uint32_t k = (g * kBlock + threadIdx.x) * kLane;
+    if (k + kLane <= n) load8(x + k, l[g]);
+  }
+  const uint32_t used = used_of(s, r);
+  if (used) {
+    const uint32_t prompt = prompt_of(s, r);
+    for (uint32_t k = threadIdx.x; k < kTile / 4; k += kBlock) ((uint4*)table)[k] = uint4{0, 0, 0, 0};
     __syncthreads();
-    for (uint64_t i = threadIdx.x; i < row.used; i += kBlock) {
-      const uint64_t t = token(s, r, i) - v0;
+    for (uint32_t i = threadIdx.x; i < used; i += kBlock) {
+      const uint64_t t = token<K>(s, r, i) - v0;
       if (t < n) {
-        if (i < row.prompt) atomicOr(&table[t], kSeen);
+        if (i < prompt) atomicOr(&table[t], kSeen);
         else atomicAdd(&table[t], 1u);
       }
     }
     __syncthreads();
   }
+  const Row row = row_of(s, r);
   const int64_t m = mask_row(s, r);
-  const X* x = (const X*)s.logits + (int64_t)r * s.logits_row;
-  O* o = (O*)s.out + (int64_t)r * s.out_row;
-  const uint64_t b = s.bias ? (r % s.bias_rows) * s.vocab : 0;
-  for (uint32_t k = threadIdx.x; k < n; k += kBlock) {
-    const uint64_t v = v0 + k;
-    const float l = (float)x[v];
-    float z = l;
-    if (history && table[k]) {
-      const uint32_t count = table[k] & ~kSeen;
-      z = l > 0.f ? l / row.repetition : l * row.repetition;
-      if (count) z = z - row.presence - row.frequency * (float)count;
+  const uint64_t b = s.bias ? (s.bias_rows == 1 ? 0 : r % s.bias_rows) * s.vocab + v0 : 0;
+#pragma unroll
+  for (int g = 0; g < kTile / kBlock / kLane; ++g) {
+    const uint32_t k = (g * kBlock + threadIdx.x) * kLane;
+    if (k + kLane <= n) {
+      if (used) {
+        const uint4 lo = ((const uint4*)table)[k / 4], hi = ((const uint4*)table)[k / 4 + 1];
+        const uint32_t e[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+        if (lo.x | lo.y | lo.z | lo.w | hi.x | hi.y | hi.z | hi.w)
+#pragma unroll
+          for (int q = 0; q < 8; ++q) l[g][q] = penalise(l[g][q], e[q], row);
+      }
+      if (s.bias) {
+        float add[8];
+        bias8(s, b + k, add);
+#pragma unroll
+        for (int q = 0; q < 8; ++q) l[g][q] += add[q];
+      }
+      const uint32_t ok = allowed8(s, m, v0 + k);
+#pragma unroll
+      for (int q = 0; q < 8; ++q) l[g][q] = (ok >> q) & 1 ? l[g][q] : -__builtin_inff();
+      store8(o + k, l[g]);
+    } else {
+      for (uint32_t j = k; j < n; ++j) {  // the row's last scores
+        float z = (float)x[j];
+        if (used) z = penalise(z, table[j], row);
+        if (s.bias) z += bias_at(s, b + j);
+        o[j] = (O)(allowed(s, m, v0 + j) ? z : -__builtin_inff());
+      }
     }
-    if (s.bias) z += bias_at(s, b + v);
-    if (!allowed(s, m, v)) z = -__builtin_inff();
-    o[v] = (O)z;
   }
 }
 
-template <class X> static void outs(const ce_logits& s, dim3 grid, hipStream_t st) {
-  if (s.out_dtype == s.dtype) k_logits<X, X><<<grid, kBlock, 0, st>>>(s);
-  else k_logits<X, float><<<grid, kBlock, 0, st>>>(s);
+// ---- short rows -----------------------------------------------------------------------------------------------------------------
+// G rows (a power of two) of V <= kTile / G scores each; dense rows are one run of memory, 8 scores a lane whatever row they are of.
+template <class X, class O, class K> __global__ __launch_bounds__(kBlock) void k_logits_rows(ce_logits s, uint32_t G, uint32_t shift, int dense) {
+  __shared__ __attribute__((aligned(16))) uint32_t table[kTile];
+  __shared__ Row rows[kRowsMost];
+  __shared__ uint32_t used[kRowsMost], prompt[kRowsMost];
+  __shared__ int64_t masks[kRowsMost];
+  const uint64_t r0 = (uint64_t)blockIdx.x * G;
+  const uint32_t V = (uint32_t)s.vocab, have = s.rows - r0 < G ? (uint32_t)(s.rows - r0) : G, n = have * V;
+  for (uint32_t j = threadIdx.x; j < have; j += kBlock) {
+    rows[j] = row_of(s, r0 + j);
+    used[j] = used_of(s, r0 + j);
+    prompt[j] = prompt_of(s, r0 + j);
+    masks[j] = mask_row(s, r0 + j);
+  }
+  if (s.tokens) {
+    for (uint32_t k = threadIdx.x; k < (n + 3) / 4; k += kBlock) ((uint4*)table)[k] = uint4{0, 0, 0, 0};
+    __syncthreads();
+    auto count = [&](uint32_t j, uint32_t i) {
+      const uint64_t t = token<K>(s, r0 + j, i);
+      if (t < V) {
+        if (i < prompt[j]) atomicOr(&table[j * V + t], kSeen);
+        else atomicAdd(&table[j * V + t], 1u);
+      }
+    };
+    if (s.token_row < s.token_step) {  // planes of actions: the same step of neighbouring rows lies together
+      const uint32_t j = threadIdx.x & (G - 1);
+      if (G >= kBlock) {
+        for (uint32_t k = threadIdx.x; k < have; k += kBlock)
+          for (uint32_t i = 0; i < used[k]; ++i) count(k, i);
+      } else if (j < have) {
+        for (uint32_t i = threadIdx.x >> shift; i < used[j]; i += kBlock >> shift) count(j, i);
+      }
+    } else {  // histories row by row: 16 lanes to a row
+      for (uint32_t j = threadIdx.x / 16; j < have; j += kBlock / 16)
+        for (uint32_t i = threadIdx.x % 16; i < used[j]; i += 16) count(j, i);
+    }
+  }
+  __syncthreads();
+  const X* x = (const X*)s.logits + (int64_t)r0 * s.logits_row;
+  O* o = (O*)s.out + (int64_t)r0 * s.out_row;
+  const uint32_t B = (uint32_t)s.bias_rows;
+  for (uint32_t k = threadIdx.x * kLane; k < n; k += kBlock * kLane) {
+    uint32_t j = k / V, v = k - j * V;
+    const bool whole = k + kLane <= n;
+    float l[8];
+    if (dense && whole) load8(x + k, l);
+    uint32_t jj = j, vv = v;
+#pragma unroll
+    for (int q = 0; q < 8; ++q) {
+      if (k + q < n) {
+        if (!(dense && whole)) l[q] = (float)x[(int64_t)jj * s.logits_row + vv];
+        if (s.tokens) l[q] = penalise(l[q], table[k + q], rows[jj]);
+        if (s.bias) l[q] += bias_at(s, (B == 1 ? 0 : (uint64_t)((uint32_t)(r0 + jj) % B) * V) + vv);
+        if (!allowed(s, masks[jj], vv)) l[q] = -__builtin_inff();
+        if (!(dense && whole)) o[(int64_t)jj * s.out_row + vv] = (O)l[q];
+        if (++vv == V) ++jj, vv = 0;
+      }
+    }
+    if (dense && whole) store8(o + k, l);
+  }
+}
+
+template <class X, class O, class K> static void shapes(const ce_logits& s, hipStream_t st) {
+  // Half a tile and longer a row is worth blocks of its own; below, a block takes as many rows as fit.
+  if (s.vocab > kTile / 2) {
+    const uint32_t runs = (uint32_t)((s.vocab + kTile - 1) / kTile);
+    const uint64_t most = (1u << 23) / runs;  // rows of a launch: fewer than 2^32 threads
+    for (uint64_t r = 0; r < s.rows; r += most)
+      k_logits_run<X, O, K><<<(uint32_t)(s.rows - r < most ? s.rows - r : most) * runs, kBlock, 0, st>>>(s, r, runs);
+    return;
+  }
+  uint32_t shift = 0;
+  while ((2ull << shift) * s.vocab <= kTile && (2u << shift) <= kRowsMost && (s.rows >> shift) > 512) ++shift;
+  const uint32_t G = 1u << shift;
+  const int dense = s.logits_row == (int64_t)s.vocab && s.out_row == (int64_t)s.vocab;
+  k_logits_rows<X, O, K><<<(uint32_t)((s.rows + G - 1) / G), kBlock, 0, st>>>(s, G, shift, dense);
+}
+
+template <class X, class O> static void tokens_of(const ce_logits& s, hipStream_t st) {
+  if (s.tokens && s.token_dtype == CE_I32) shapes<X, O, int32_t>(s, st);
+  else if (s.tokens && s.token_dtype == CE_I64) shapes<X, O, int64_t>(s, st);
+  else shapes<X, O, uint8_t>(s, st);
+}
+template <class X> static void outs(const ce_logits& s, hipStream_t st) {
+  if (s.out_dtype == s.dtype) tokens_of<X, X>(s, st);
+  else tokens_of<X, float>(s, st);
 }
 
 hipError_t launch_logits(const ce_logits& s, hipStream_t st) {
-  const dim3 grid((uint32_t)s.rows, (uint32_t)((s.vocab + kChunk - 1) / kChunk));
-  if (s.dtype == CE_F32) outs<float>(s, grid, st);
-  else if (s.dtype == CE_BF16) outs<bf16>(s, grid, st);
-  else outs<f16>(s, grid, st);
+  if (s.dtype == CE_F32) outs<float>(s, st);
+  else if (s.dtype == CE_BF16) outs<bf16>(s, st);
+  else outs<f16>(s, st);
   return hipGetLastError();
 }
 
 // ---- gradients ------------------------------------------------------------------------------------------------------------------
-constexpr int kGradChunk = kBlock * 4;
+// Where a bias wants a gradient, the B rows that its table covers in turn are one long row of B V columns, so that a lane keeps its 8
+// columns while it walks down the R / B long rows and sums them in float; otherwise a long row is a row.  A block takes a run of
+// 2048 columns, or as many whole long rows at a time as fill its lanes; it marks the tokens seen by kPasses of its steps in LDS
+// (one bit a score) ahead of walking them.  The long rows are cut into parts; a second launch adds their sums in a fixed order.
+constexpr int kPasses = 16, kCols = kBlock * kLane;
 
-// Rows that share a bias row are cut into `parts` runs; a block sums its run in float, row after row, and a second launch adds the
-// parts in their order.
-static uint32_t grad_parts(const ce_logits& s, const ce_logits_grad& g) {
-  const uint64_t b = g.dbias ? s.bias_rows : 1, each = (s.rows + b - 1) / b, chunks = (s.vocab + kGradChunk - 1) / kGradChunk;
-  uint64_t parts = 2048 / (b * chunks) + 1;
-  if (parts > each) parts = each;
-  return (uint32_t)parts;
+struct GradShape {
+  uint64_t B, width, long_rows;  // rows of a long row, its columns, how many there are
+  uint64_t chunks;               // runs of kCols columns
+  uint32_t lanes, at_once;       // lanes of a long row (in a run), long rows a block walks side by side
+  uint64_t parts;
+};
+static GradShape grad_shape(const ce_logits& s, const ce_logits_grad& g) {
+  GradShape o;
+  o.B = g.dbias ? s.bias_rows : 1;
+  o.width = o.B * s.vocab;
+  o.long_rows = s.rows / o.B;
+  o.chunks = (o.width + kCols - 1) / kCols;
+  o.lanes = o.width >= kCols ? kBlock : (uint32_t)((o.width + kLane - 1) / kLane);
+  o.at_once = kBlock / o.lanes;
+  const uint64_t passes = (o.long_rows + o.at_once - 1) / o.at_once;
+  uint64_t parts = o.chunks >= 1024 ? 1 : 1024 / o.chunks;  // 4 blocks a CU, and sums of no more parts than that takes
+  o.parts = parts < passes ? parts : passes;
+  return o;
 }
 
-template <class X, class D> __global__ __launch_bounds__(kBlock) void k_logits_grad(ce_logits s, ce_logits_grad g, uint32_t B, uint32_t parts) {
-  __shared__ uint32_t bits[kGradChunk / 32];
-  const uint32_t chunks = (uint32_t)((s.vocab + kGradChunk - 1) / kGradChunk), rest = blockIdx.x / chunks;
-  const uint64_t v0 = (uint64_t)(blockIdx.x % chunks) * kGradChunk;
-  const uint32_t b = rest % B, part = rest / B;
-  const uint64_t each = (s.rows - b + B - 1) / B;  // rows b, b + B, ...
-  const uint64_t k0 = each * part / parts, k1 = each * (part + 1) / parts;
-  float sum[4] = {0, 0, 0, 0};
-  for (uint64_t k = k0; k < k1; ++k) {
-    const uint64_t r = b + k * B;
-    const Row row = row_of(s, r);
-    const bool history = g.dlogits && row.used > 0 && row.repetition != 1.f;
+template <class X, class D, class K> __global__ __launch_bounds__(kBlock) void k_logits_grad(ce_logits s, ce_logits_grad g, GradShape w, uint64_t block0) {
+  __shared__ uint32_t marks[kPasses * kBlock / 4];  // a byte for a lane's 8 columns of a pass
+  __shared__ float sums[kBlock][kLane + 1];
+  const uint64_t block = block0 + blockIdx.x, chunk = block % w.chunks, part = block / w.chunks;
+  const uint32_t V = (uint32_t)s.vocab, sub = threadIdx.x / w.lanes, t = threadIdx.x - sub * w.lanes;
+  const uint64_t c0 = chunk * kCols, c = c0 + (uint64_t)t * kLane;
+  const bool active = sub < w.at_once && c < w.width;
+  const uint32_t cols = active ? (uint32_t)(w.width - c < kLane ? w.width - c : kLane) : 0;
+  const uint64_t b0 = c / V;
+  const uint32_t v0 = (uint32_t)(c - b0 * V);
+  const bool one_row = cols == kLane && v0 + kLane <= V, run = one_row || (cols == kLane && g.dout_row == (int64_t)V);
+  const uint64_t passes = (w.long_rows + w.at_once - 1) / w.at_once;
+  const uint64_t p0 = passes * part / w.parts, p1 = passes * (part + 1) / w.parts;
+  // the rows of a long row that this run of columns touches
+  const uint64_t last = (c0 + kCols < w.width ? c0 + kCols : w.width) - 1, b_lo = c0 / V;
+  const uint32_t touched = (uint32_t)(last / V - b_lo) + 1;
+  const bool history = s.tokens && g.dlogits && (s.repetition || s.repetition_all != 1.0);
+  float sum[kLane] = {0, 0, 0, 0, 0, 0, 0, 0};
+  for (uint64_t p = p0; p < p1; p += kPasses) {
+    const uint32_t np = p1 - p < kPasses ? (uint32_t)(p1 - p) : kPasses;
     if (history) {
       __syncthreads();
-      if (threadIdx.x < kGradChunk / 32) bits[threadIdx.x] = 0;
+      for (uint32_t k = threadIdx.x; k < np * kBlock / 4; k += kBlock) marks[k] = 0;
       __syncthreads();
-      for (uint64_t i = threadIdx.x; i < row.used; i += kBlock) {
-        const uint64_t t = token(s, r, i), at = t - v0;
-        if (at < kGradChunk && t < s.vocab) atomicOr(&bits[at / 32], 1u << (at % 32));
+      const uint64_t first = p * w.at_once, end = first + (uint64_t)np * w.at_once < w.long_rows ? first + (uint64_t)np * w.at_once : w.long_rows;
+      const uint32_t n = (uint32_t)(end - first) * touched;  // rows whose histories matter
+      auto mark = [&](uint32_t k, uint32_t from, uint32_t stride) {
+        const uint32_t lr = k / touched, b = k - lr * touched;
+        const uint64_t r = (first + lr) * w.B + b_lo + b;
+        const uint32_t used = used_of(s, r), byte0 = (lr / w.at_once) * kBlock + (lr % w.at_once) * w.lanes;
+        for (uint32_t i = from; i < used; i += stride) {
+          const uint64_t tok = token<K>(s, r, i);
+          if (tok >= V) continue;
+          const uint64_t at = (b_lo + b) * V + tok - c0;  // wraps where it lies ahead of the run
+          if (at >= kCols || at >= w.width - c0) continue;
+          const uint32_t byte = byte0 + (uint32_t)at / kLane;
+          atomicOr(&marks[byte / 4], 1u << (byte % 4 * 8 + (uint32_t)at % kLane));
+        }
+      };
+      if (s.token_row < s.token_step) {  // neighbouring rows' tokens of a step lie together: neighbouring lanes take them
+        if (n >= kBlock) {
+          for (uint32_t k = threadIdx.x; k < n; k += kBlock) mark(k, 0, 1);
+        } else if (threadIdx.x / n < kBlock / n) {
+          mark(threadIdx.x % n, threadIdx.x / n, kBlock / n);
+        }
+      } else {  // 16 lanes to a row
+        for (uint32_t k = threadIdx.x / 16; k < n; k += kBlock / 16) mark(k, threadIdx.x % 16, 16);
       }
       __syncthreads();
     }
-    const int64_t m = mask_row(s, r);
+    if (!active) continue;
+#pragma unroll 4
+    for (uint32_t q = 0; q < np; ++q) {
+      const uint64_t lr = (p + q) * w.at_once + sub;
+      if (lr >= w.long_rows) break;
+      const uint32_t seen = history ? ((const uint8_t*)marks)[q * kBlock + threadIdx.x] : 0u;
+      if (run && one_row) {
+        const uint64_t r = lr * w.B + b0;
+        float d[kLane];
+        load8((const D*)g.dout + (int64_t)r * g.dout_row + v0, d);
+        const uint32_t ok = allowed8(s, mask_row(s, r), v0);
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const uint32_t at = q * kBlock + threadIdx.x;
-      const uint64_t v = v0 + at;
-      if (v >= s.vocab) continue;
-      float d = (float)((const D*)g.dout)[(int64_t)r * g.dout_row + v];
-      if (!allowed(s, m, v)) d = 0.f;
-      sum[q] += d;
-      if (!g.dlogits) continue;
-      if (history && ((bits[at / 32] >> (at % 32)) & 1u)) {
-        const float l = (float)((const X*)s.logits)[(int64_t)r * s.logits_row + v];
-        d = l > 0.f ? d / row.repetition : d * row.repetition;
+        for (int j = 0; j < kLane; ++j) {
+          d[j] = (ok >> j) & 1 ? d[j] : 0.f;
+          sum[j] += d[j];
+        }
+        if (!g.dlogits) continue;
+        if (seen) {
+          const float rep = s.repetition ? s.repetition[r] : (float)s.repetition_all;
+          float l[kLane];
+          load8((const X*)s.logits + (int64_t)r * s.logits_row + v0, l);
+#pragma unroll
+          for (int j = 0; j < kLane; ++j)
+            if ((seen >> j) & 1) d[j] = l[j] > 0.f ? d[j] / rep : d[j] * rep;
+        }
+        store8((X*)g.dlogits + lr * w.width + c, d);
+      } else {
+        uint64_t r = lr * w.B + b0;
+        uint32_t v = v0;
+        int64_t m = mask_row(s, r);
+        float d[kLane];
+        if (run) load8((const D*)g.dout + lr * w.width + c, d);
+#pragma unroll
+        for (int j = 0; j < kLane; ++j) {
+          if (j >= (int)cols) continue;
+          if (!run) d[j] = (float)((const D*)g.dout)[(int64_t)r * g.dout_row + v];
+          if (!allowed(s, m, v)) d[j] = 0.f;
+          sum[j] += d[j];
+          if ((seen >> j) & 1) {
+            const float rep = s.repetition ? s.repetition[r] : (float)s.repetition_all;
+            d[j] = (float)((const X*)s.logits)[(int64_t)r * s.logits_row + v] > 0.f ? d[j] / rep : d[j] * rep;
+          }
+          if (!run && g.dlogits) ((X*)g.dlogits)[lr * w.width + c + j] = (X)d[j];
+          if (++v == V && j + 1 < (int)cols) {
+            v = 0;
+            m = mask_row(s, ++r);
+          }
+        }
+        if (run && g.dlogits) store8((X*)g.dlogits + lr * w.width + c, d);
       }
-      ((X*)g.dlogits)[r * s.vocab + v] = (X)d;
     }
   }
   if (!g.dbias) return;
+  if (w.at_once > 1) {  // the long rows walked side by side, in their order
 #pragma unroll
-  for (int q = 0; q < 4; ++q) {
-    const uint64_t v = v0 + q * kBlock + threadIdx.x;
-    if (v < s.vocab) ((float*)s.workspace)[((uint64_t)part * B + b) * s.vocab + v] = sum[q];
+    for (int j = 0; j < kLane; ++j) sums[threadIdx.x][j] = sum[j];
+    __syncthreads();
+    if (sub == 0)
+      for (uint32_t k = 1; k < w.at_once; ++k)
+#pragma unroll
+        for (int j = 0; j < kLane; ++j) sum[j] += sums[k * w.lanes + t][j];
+    if (sub != 0) return;
   }
+  for (uint32_t j = 0; j < kLane; ++j)
+    if (j < cols) ((float*)s.workspace)[part * w.width + c + j] = sum[j];
 }
 
-template <class T> __global__ __launch_bounds__(kBlock) void k_logits_bias(const float* part, T* dbias, uint64_t n, uint32_t parts) {
-  const uint64_t i = (uint64_t)blockIdx.x * kBlock + threadIdx.x;
-  if (i >= n) return;
-  float sum = part[i];
-  for (uint32_t k = 1; k < parts; ++k) sum += part[(uint64_t)k * n + i];
-  dbias[i] = (T)sum;
+// 64 columns to a block, each 4th part to a wave, the waves' sums in their order
+template <class T> __global__ __launch_bounds__(kBlock) void k_logits_bias(const float* part, T* dbias, uint64_t n, uint32_t parts, uint64_t block0) {
+  __shared__ float sums[4][kWave];
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  const uint64_t i = (block0 + blockIdx.x) * kWave + lane;
+  float sum = 0.f;
+  if (i < n)
+#pragma unroll 8
+    for (uint32_t k = w; k < parts; k += 4) sum += part[(uint64_t)k * n + i];
+  sums[w][lane] = sum;
+  __syncthreads();
+  if (w == 0 && i < n) dbias[i] = (T)(((sums[0][lane] + sums[1][lane]) + sums[2][lane]) + sums[3][lane]);
 }
 
 uint64_t logits_grad_workspace(const ce_logits& s, const ce_logits_grad& g) {
-  return g.dbias ? (uint64_t)grad_parts(s, g) * s.bias_rows * s.vocab * sizeof(float) : 0;
+  const GradShape w = grad_shape(s, g);
+  return g.dbias ? w.parts * w.width * sizeof(float) : 0;
 }
 
-template <class X> static void douts(const ce_logits& s, const ce_logits_grad& g, dim3 grid, uint32_t B, uint32_t parts, hipStream_t st) {
-  if (s.out_dtype == s.dtype) k_logits_grad<X, X><<<grid, kBlock, 0, st>>>(s, g, B, parts);
-  else k_logits_grad<X, float><<<grid, kBlock, 0, st>>>(s, g, B, parts);
+constexpr uint64_t kBlocksMost = 1u << 23;  // of a launch: fewer than 2^32 threads
+
+template <class X, class D, class K> static void grad_go(const ce_logits& s, const ce_logits_grad& g, const GradShape& w, hipStream_t st) {
+  const uint64_t blocks = w.chunks * w.parts;
+  for (uint64_t b = 0; b < blocks; b += kBlocksMost)
+    k_logits_grad<X, D, K><<<(uint32_t)(blocks - b < kBlocksMost ? blocks - b : kBlocksMost), kBlock, 0, st>>>(s, g, w, b);
+}
+template <class X, class D> static void grad_tokens(const ce_logits& s, const ce_logits_grad& g, const GradShape& w, hipStream_t st) {
+  if (s.tokens && s.token_dtype == CE_I32) grad_go<X, D, int32_t>(s, g, w, st);
+  else if (s.tokens && s.token_dtype == CE_I64) grad_go<X, D, int64_t>(s, g, w, st);
+  else grad_go<X, D, uint8_t>(s, g, w, st);
+}
+template <class X> static void grad_outs(const ce_logits& s, const ce_logits_grad& g, const GradShape& w, hipStream_t st) {
+  if (s.out_dtype == s.dtype) grad_tokens<X, X>(s, g, w, st);
+  else grad_tokens<X, float>(s, g, w, st);
+}
+template <class T> static void bias_go(const ce_logits& s, const ce_logits_grad& g, const GradShape& w, hipStream_t st) {
+  const uint64_t blocks = (w.width + kWave - 1) / kWave;
+  for (uint64_t b = 0; b < blocks; b += kBlocksMost)
+    k_logits_bias<T><<<(uint32_t)(blocks - b < kBlocksMost ? blocks - b : kBlocksMost), kBlock, 0, st>>>((const float*)s.workspace, (T*)g.dbias, w.width, (uint32_t)w.parts, b);
 }
 
 hipError_t launch_logits_grad(const ce_logits& s, const ce_logits_grad& g, hipStream_t st) {
-  const uint32_t B = g.dbias ? (uint32_t)s.bias_rows : 1, parts = grad_parts(s, g);
-  const dim3 grid((uint32_t)((s.vocab + kGradChunk - 1) / kGradChunk) * B * parts);
-  if (s.dtype == CE_F32) douts<float>(s, g, grid, B, parts, st);
-  else if (s.dtype == CE_BF16) douts<bf16>(s, g, grid, B, parts, st);
-  else douts<f16>(s, g, grid, B, parts, st);
+  const GradShape w = grad_shape(s, g);
+  if (s.dtype == CE_F32) grad_outs<float>(s, g, w, st);
+  else if (s.dtype == CE_BF16) grad_outs<bf16>(s, g, w, st);
+  else grad_outs<f16>(s, g, w, st);
   if (hipError_t e = hipGetLastError()) return e;
   if (g.dbias) {
-    const uint64_t n = (uint64_t)B * s.vocab;
-    const uint32_t blocks = (uint32_t)((n + kBlock - 1) / kBlock);
-    const float* part = (const float*)s.workspace;
-    if (s.bias_dtype == CE_F32) k_logits_bias<float><<<blocks, kBlock, 0, st>>>(part, (float*)g.dbias, n, parts);
-    else if (s.bias_dtype == CE_BF16) k_logits_bias<bf16><<<blocks, kBlock, 0, st>>>(part, (bf16*)g.dbias, n, parts);
-    else k_logits_bias<f16><<<blocks, kBlock, 0, st>>>(part, (f16*)g.dbias, n, parts);
+    if (s.bias_dtype == CE_F32) bias_go<float>(s, g, w, st);
+    else if (s.bias_dtype == CE_BF16) bias_go<bf16>(s, g, w, st);
+    else bias_go<f16>(s, g, w, st);
   }
   return hipGetLastError();
 }
