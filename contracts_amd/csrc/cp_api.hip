@@ -82,22 +82,38 @@ int check_scan(const ce_scan* s) {
   return CE_OK;
 }
 
-// Waves of a block and chunks of the time axis.  A wave on its own walks a run once; sharing the time axis costs a second walk, and
-// chunks cost reading everything twice, so both come only where the columns alone leave the chip's 1024 SIMDs short of waves.
-// No chunk is under 256 steps, where folding the chunks before it would cost as much as the chunk.
-void split(cp::ScanParams& p, uint64_t blocks) {
+// Lanes, waves and chunks.  The chip wants about 2048 waves in flight (2 on each of its 1024 SIMDs).  Columns give them
+// cheapest: with enough, a wave takes its columns' whole time axis on its own, 8 bytes to a lane.  Then the 4 or 8 waves of a block
+// share the time axis, which costs a second walk in registers; then lanes take fewer channels; and last the time axis is cut into chunks, which costs
+// reading x and the gate twice.  No chunk is under CE_SCAN_SPLIT_STEPS / 2 steps.
+constexpr uint64_t kWavesWanted = 2048;
+
+void share(cp::ScanParams& p, int* vec, int least, uint64_t columns, uint64_t (*blocks)(const cp::ScanParams&, uint64_t columns, int vec)) {
   p.chunks = 1;
-  p.waves = p.T <= CE_SCAN_SAVED_STEPS || blocks >= 2048 ? 1 : 4;
-  if (p.waves == 1) return;
-  uint64_t want = blocks >= 512 ? 1 : 512 / blocks;
-  const uint64_t most = p.T / 256;
-  if (want > most) want = most;
-  if (want > 64) want = 64;
+  p.waves = 1;
+  if (p.T <= CE_SCAN_SAVED_STEPS) return;
+  if (blocks(p, columns, *vec) >= kWavesWanted) return;
+  p.waves = 4;
+  while (*vec > least && blocks(p, columns, *vec) * 4 < kWavesWanted) *vec /= 2;
+  uint64_t have = blocks(p, columns, *vec);
+  if (have * 4 >= kWavesWanted || p.T < 16 * CE_SCAN_SAVED_STEPS) return;
+  p.waves = 8;
+  have *= 8;
+  uint64_t want = have ? kWavesWanted / have : 1;
+  const uint64_t most = p.T / (CE_SCAN_SPLIT_STEPS / 2);
+  want = std::min<uint64_t>({want, most, 64});
   if (want > 1) {
-    const uint64_t tile = 4 * CE_SCAN_SAVED_STEPS, each = ((p.T + want - 1) / want + tile - 1) / tile * tile;
+    const uint64_t tile = 8 * CE_SCAN_SAVED_STEPS, each = ((p.T + want - 1) / want + tile - 1) / tile * tile;
     p.chunk = each;
     p.chunks = (uint32_t)((p.T + each - 1) / each);
   }
+}
+
+// Waves side by side that a scan's columns make (with a head's gradient to add up, heads keep to a wave, or take several).
+uint64_t flat_waves(const cp::ScanParams&, uint64_t columns, int vec) { return (columns / vec + 63) / 64; }
+uint64_t head_waves(const cp::ScanParams& p, uint64_t columns, int vec) {
+  const uint64_t lanes = p.head / vec, groups = columns / p.head;
+  return lanes > 64 ? groups * ((lanes + 63) / 64) : (groups + 64 / lanes - 1) / (64 / lanes);
 }
 
 void plan_scan(const ce_scan* s, const ce_scan_grad* g, Plan* o) {
@@ -114,15 +130,18 @@ void plan_scan(const ce_scan* s, const ce_scan_grad* g, Plan* o) {
     if (!g) return ok && aligned(s->y, v * b);
     return ok && aligned(g->dy, v * b) && aligned(g->dx, v * b) && (o->mode != cp::kGateChannel || aligned(g->dgate, v * gb));
   };
-  int vec = g ? (b == 2 ? 2 : 1) : b == 2 ? 4 : b == 4 ? 2 : 1;
+  int vec = b == 8 ? 1 : (int)(8 / b);
+  if (g) vec = b == 2 ? 2 : 1;
   while (vec > 1 && !fits(vec)) vec /= 2;
+  p.T = T;
+  p.head = (uint32_t)head;
+  const bool sums = g && o->mode == cp::kGateHead;
+  share(p, &vec, 1, E * C, sums ? head_waves : flat_waves);
   o->vec = vec;
   const bool rev = s->flags & CE_SCAN_REVERSE;
   const int64_t sign = rev ? -1 : 1, off = rev && T ? (int64_t)T - 1 : 0;
-  p.T = T;
   p.cols = (uint32_t)(E * C / vec);
   p.row_cols = (uint32_t)(C / vec);
-  p.head = (uint32_t)head;
   p.heads = (uint32_t)H;
   p.rows = (uint32_t)E;
   p.cut_off = rev ? 0 : -1;
@@ -144,26 +163,19 @@ void plan_scan(const ce_scan* s, const ce_scan_grad* g, Plan* o) {
   p.last = s->last;
   p.saved = s->saved;
   p.slabs = 1;
-  uint64_t blocks = ((uint64_t)p.cols + 63) / 64;
   if (g) {
     p.dy = from(g->dy, (int64_t)(E * C), b);
     p.dlast = g->dlast;
     p.dx = from(g->dx, (int64_t)(E * C), b);
     p.dgate = from(g->dgate, (int64_t)(E * H), gb);
     p.dstate = g->dstate;
-    if (o->mode == cp::kGateHead) {
-      const uint64_t lanes = head / vec;
-      uint64_t seg = 1;
-      while (seg < lanes && seg < 64) seg *= 2;
-      if (lanes > 64) seg = (lanes + 63) / 64 * 64;
-      p.seg = (uint32_t)seg;
-      p.slabs = seg > 64 ? (uint32_t)(seg / 64) : 1;
-      blocks = (E * H * seg + 63) / 64;
+    if (sums) {
+      p.lanes = (uint32_t)(head / vec);
+      p.in_wave = p.lanes <= 64 ? 64 / p.lanes : 0;
+      p.slabs = p.in_wave ? 1 : (p.lanes + 63) / 64;
     }
   }
-  const uint64_t row_lanes = g && o->mode == cp::kGateHead ? H * p.seg : p.row_cols;
-  p.flags = !s->done ? cp::kFlagsNone : row_lanes >= cp::kBallotRow ? cp::kFlagsBallot : cp::kFlagsLane;
-  split(p, blocks);
+  p.flags = !s->done ? cp::kFlagsNone : p.row_cols >= cp::kBallotRow ? cp::kFlagsBallot : cp::kFlagsLane;
   // the chunks of a split time axis read the incoming state while the last of them writes the outgoing one
   if (!g && s->last && s->last == s->state) p.chunks = 1;
   if (p.chunks == 1) p.chunk = T;

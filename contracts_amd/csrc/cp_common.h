@@ -82,7 +82,8 @@ struct ScanParams {
   void* dstate;
   int64_t dgate_step;
   uint32_t heads;
-  uint32_t seg;       // lanes of one head's segment (padded); 0: a gate for each channel
+  uint32_t lanes;     // backward pass, gates shared by a head: lanes of a head (head / VEC)
+  uint32_t in_wave;   // whole heads side by side in a wave (0: a head takes `slabs` waves)
   uint32_t slabs;     // partial sums a head's gradient is made of
   float* slab;        // [slabs][T][E][H] where slabs > 1
 };

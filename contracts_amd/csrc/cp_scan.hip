@@ -190,17 +190,19 @@ template <class X, class G, int MODE, int VEC, int W, bool REDUCE> __global__ __
   }
 }
 
-template <class X, class G, int MODE, int VEC> static hipError_t go(const ScanParams& p, hipStream_t stream) {
-  const dim3 grid((p.cols + kWave - 1) / kWave, p.chunks);
-  if (p.waves == 1) {
-    k_scan<X, G, MODE, VEC, 1, false><<<grid, kWave, 0, stream>>>(p);
-    return hipGetLastError();
-  }
+template <class X, class G, int MODE, int VEC, int W> static hipError_t waves(const ScanParams& p, uint32_t x, hipStream_t stream) {
   if (p.chunks > 1) {
-    k_scan<X, G, MODE, VEC, 4, true><<<dim3(grid.x, p.chunks - 1), 4 * kWave, 0, stream>>>(p);
+    k_scan<X, G, MODE, VEC, W, true><<<dim3(x, p.chunks - 1), W * kWave, 0, stream>>>(p);
     if (hipError_t e = hipGetLastError()) return e;
   }
-  k_scan<X, G, MODE, VEC, 4, false><<<grid, 4 * kWave, 0, stream>>>(p);
+  k_scan<X, G, MODE, VEC, W, false><<<dim3(x, p.chunks), W * kWave, 0, stream>>>(p);
+  return hipGetLastError();
+}
+
+template <class X, class G, int MODE, int VEC> static hipError_t go(const ScanParams& p, hipStream_t stream) {
+  const uint32_t x = (p.cols + kWave - 1) / kWave;
+  if (p.waves == 1) k_scan<X, G, MODE, VEC, 1, false><<<x, kWave, 0, stream>>>(p);
+  else if (hipError_t e = p.waves == 4 ? waves<X, G, MODE, VEC, 4>(p, x, stream) : waves<X, G, MODE, VEC, 8>(p, x, stream)) return e;
   return hipGetLastError();
 }
 

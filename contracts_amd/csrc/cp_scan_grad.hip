@@ -6,8 +6,9 @@
 // kSteps steps is the map R -> P R + Q, the waves exchange (P, Q) through LDS, and a time axis cut into chunks is reduced by a launch of
 // its own first.  The states are not kept in y's rounded type: the forward pass left the float state ahead of every run (1 / 16
 // of a float plane), and a wave walks its run forward again in registers.  Reads x, a, dy, writes dx and da, once each.
-// A head's gate sums over its channels: lanes of a segment by butterflies, a head wider than a wave through partial sums that a
-// second launch adds up in a fixed order (no atomics: the same call gives the same bits).
+// A head's gate sums over its channels: the run's terms go through LDS, where a lane adds up a step of a head (a butterfly in
+// registers would take 6 exchanges a step: 178 us against X at scan of 37 x 9 heads of 40 channels, 1000 steps); a head wider than a wave leaves partial sums
+// that a second launch adds up in a fixed order (no atomics: the same call gives the same bits).
 #include "cp_common.h"
 
 namespace cp {
@@ -17,22 +18,26 @@ constexpr int kSteps = CE_SCAN_SAVED_STEPS;
 template <class X, class G, int MODE, int VEC, int W, bool REDUCE> __global__ __launch_bounds__(kWave * W) void k_scan_grad(ScanParams p) {
   constexpr int GV = MODE == kGateChannel ? VEC : 1;
   __shared__ float fold[W > 1 ? 2 : 1][W][2][VEC][kWave];
+  // a run's terms of dgate, a row of lanes to a step; rows are 65 apart, so that lanes which add up different steps read different banks
+  __shared__ float terms[MODE == kGateHead && !REDUCE ? W : 1][MODE == kGateHead && !REDUCE ? kSteps : 1][kWave + 1];
   const int lane = threadIdx.x & 63, w = W > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : 0;
-  const uint32_t slot = blockIdx.x * kWave + lane;
-  uint32_t e, c, head = 0;
+  uint32_t e, c, head = 0, group0 = 0;
   bool live;
-  if (MODE == kGateHead) {  // `seg` lanes to a head of head / VEC columns
-    const uint32_t group = slot / p.seg, in = (slot % p.seg) * VEC;
-    live = in < p.head && group < p.rows * p.heads;
-    const uint32_t g = group < p.rows * p.heads ? group : p.rows * p.heads - 1;
+  if (MODE == kGateHead) {
+    // in_wave heads of `lanes` lanes side by side; or the blockIdx.x % slabs-th wave of a wider head
+    group0 = p.in_wave ? blockIdx.x * p.in_wave : blockIdx.x / p.slabs;
+    const uint32_t groups = p.rows * p.heads, own = p.in_wave ? lane / p.lanes : 0, in = p.in_wave ? lane - own * p.lanes : blockIdx.x % p.slabs * kWave + lane;
+    live = p.in_wave ? own < p.in_wave && group0 + own < groups : in < p.lanes;
+    const uint32_t g = group0 + own < groups && own < (p.in_wave ? p.in_wave : 1) ? group0 + own : group0;
     e = g / p.heads;
-    head = g % p.heads;
-    c = head * p.head + (live ? in : 0);
+    head = g - e * p.heads;
+    c = head * p.head + (live ? in * VEC : 0);
   } else {
+    const uint32_t slot = blockIdx.x * kWave + lane;
     live = slot < p.cols;
     const uint32_t col = live ? slot : p.cols - 1;
     e = col / p.row_cols;
-    c = (col % p.row_cols) * VEC;
+    c = (col - e * p.row_cols) * VEC;
   }
   // lanes that are not live do what another one does and write the same; none lies ahead of the wave's first row e0, from which all count
   const uint32_t e0 = __builtin_amdgcn_readfirstlane(e);
@@ -169,19 +174,27 @@ template <class X, class G, int MODE, int VEC, int W, bool REDUCE> __global__ __
         float sum = 0.f;
 #pragma unroll
         for (int v = 0; v < VEC; ++v) sum = fma_(gt[v], k[v], sum);
-        if (!live) sum = 0.f;
-        const uint32_t width = p.seg < kWave ? p.seg : kWave;
-        for (uint32_t j = width / 2; j > 0; j >>= 1) sum += __shfl_xor(sum, (int)j);
-        if (live && (lane & (width - 1)) == 0) {
-          const uint64_t at = (uint64_t)e * p.heads + head;
-          if (p.slabs == 1) {
-            ((G*)p.dgate)[at + (int64_t)(i + s) * p.dgate_step] = (G)sum;
-          } else {
-            const uint64_t EH = (uint64_t)p.rows * p.heads;
-            p.slab[((slot % p.seg) / kWave) * p.T * EH + (i + s) * EH + at] = sum;
-          }
-        }
+        terms[w][s][lane] = sum;
       }
+    };
+    // dgate of the run's steps: each (step, head) is added up by one lane, or by 2 or 4 where there are fewer such sums than lanes
+    auto add_up = [&]() {
+      const uint32_t heads = p.in_wave ? p.in_wave : 1, each = p.in_wave ? p.lanes : p.lanes - blockIdx.x % p.slabs * kWave < kWave ? p.lanes - blockIdx.x % p.slabs * kWave : kWave;
+      const uint32_t split = heads == 1 ? 4 : heads == 2 ? 2 : 1, share = (each + split - 1) / split;
+      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+      for (uint32_t o = lane / split; o < heads * kSteps; o += kWave / split) {
+        const uint32_t s = o % kSteps, own = o / kSteps, j0 = lane % split * share, j1 = j0 + share < each ? j0 + share : each;
+        float sum = 0.f;
+        for (uint32_t j = j0; j < j1; ++j) sum += terms[w][s][own * each + j];
+        if (split >= 2) sum += __shfl_xor(sum, 1);
+        if (split == 4) sum += __shfl_xor(sum, 2);
+        if (lane % split || (int)s >= n || group0 + own >= p.rows * p.heads) continue;
+        const uint64_t EH = (uint64_t)p.rows * p.heads;
+        if (p.slabs == 1) ((G*)p.dgate)[group0 + own + (int64_t)(i + s) * p.dgate_step] = (G)sum;
+        else p.slab[(blockIdx.x % p.slabs) * p.T * EH + (i + s) * EH + group0 + own] = sum;
+      }
+      __builtin_amdgcn_wave_barrier();
     };
     float k[kSteps][VEC];  // the state that each step multiplies
     bool odd = !plain;
@@ -246,6 +259,7 @@ template <class X, class G, int MODE, int VEC, int W, bool REDUCE> __global__ __
 #pragma unroll
         for (int v = 0; v < VEC; ++v) R[v] = r[v];
     }
+    if (MODE == kGateHead) add_up();
   }
   if (!live || w != 0) return;
   if (REDUCE) {
@@ -268,18 +282,23 @@ template <class G> __global__ __launch_bounds__(256) void k_scan_grad_slabs(Scan
   }
 }
 
-template <class X, class G, int MODE, int VEC> static hipError_t go(const ScanParams& p, hipStream_t stream) {
-  const uint64_t slots = MODE == kGateHead ? (uint64_t)p.rows * p.heads * p.seg : p.cols;
-  const dim3 grid((uint32_t)((slots + kWave - 1) / kWave), p.chunks);
-  if (p.waves == 1) {
-    k_scan_grad<X, G, MODE, VEC, 1, false><<<grid, kWave, 0, stream>>>(p);
-  } else {
-    if (p.chunks > 1) {
-      k_scan_grad<X, G, MODE, VEC, 4, true><<<dim3(grid.x, p.chunks - 1), 4 * kWave, 0, stream>>>(p);
-      if (hipError_t e = hipGetLastError()) return e;
-    }
-    k_scan_grad<X, G, MODE, VEC, 4, false><<<grid, 4 * kWave, 0, stream>>>(p);
+template <class X, class G, int MODE, int VEC, int W> static hipError_t waves(const ScanParams& p, uint32_t x, hipStream_t stream) {
+  if (p.chunks > 1) {
+    k_scan_grad<X, G, MODE, VEC, W, true><<<dim3(x, p.chunks - 1), W * kWave, 0, stream>>>(p);
+    if (hipError_t e = hipGetLastError()) return e;
   }
+  k_scan_grad<X, G, MODE, VEC, W, false><<<dim3(x, p.chunks), W * kWave, 0, stream>>>(p);
+  return hipGetLastError();
+}
+
+template <class X, class G, int MODE, int VEC> static hipError_t go(const ScanParams& p, hipStream_t stream) {
+  // heads of a wave's lanes or fewer lie side by side in it, a wider one takes whole waves
+  const uint64_t columns = MODE != kGateHead ? ((uint64_t)p.cols + kWave - 1) / kWave
+                         : p.in_wave       ? ((uint64_t)p.rows * p.heads + p.in_wave - 1) / p.in_wave
+                                           : (uint64_t)p.rows * p.heads * p.slabs;
+  const uint32_t x = (uint32_t)columns;
+  if (p.waves == 1) k_scan_grad<X, G, MODE, VEC, 1, false><<<x, kWave, 0, stream>>>(p);
+  else if (hipError_t e = p.waves == 4 ? waves<X, G, MODE, VEC, 4>(p, x, stream) : waves<X, G, MODE, VEC, 8>(p, x, stream)) return e;
   if (hipError_t e = hipGetLastError()) return e;
   if (MODE == kGateHead && p.slabs > 1 && p.T > 0) {
     const uint64_t n = p.T * (uint64_t)p.rows * p.heads, blocks = (n + 255) / 256;

@@ -21,36 +21,35 @@ from . import _lib
 _CODE = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16, torch.float16: _lib.F16, torch.float64: _lib.F64, torch.uint8: _lib.U8,
          torch.bool: _lib.U8, torch.int32: _lib.I32, torch.int64: _lib.I64}
 _REAL = (torch.float32, torch.bfloat16, torch.float16)
+_ABI = _lib.POLICY_ABI_VERSION
+_scan_args, _scan_grad_args, _adv_args, _logits_args, _logits_grad_args = (
+    _lib.packer(c) for c in (_lib.CeScan, _lib.CeScanGrad, _lib.CeAdvantage, _lib.CeLogits, _lib.CeLogitsGrad))
+_stream = torch._C._cuda_getCurrentRawStream  # torch's current stream of a device, without the wrapper object around it
 
 
-def _need(cond, what, *args):
-    if not cond:
-        raise ValueError(what % args if args else what)
+def _bad(what, *args):
+    raise ValueError(what % args if args else what)
 
 
-def _device(op, *tensors):
+def _device(op, first, *tensors):
     """the one device that all of a call's tensors live on"""
-    dev = tensors[0].device
-    _need(dev.type == "cuda", "%s: tensors must live on a GPU (there is no CPU path), got %s", op, dev)
-    for t in tensors[1:]:
-        _need(t is None or t.device == dev, "%s: all tensors must live on one device", op)
+    dev = first.device
+    if dev.type != "cuda":
+        _bad("%s: tensors must live on a GPU (there is no CPU path), got %s", op, dev)
+    for t in tensors:
+        if t is not None and t.device != dev:
+            _bad("%s: all tensors must live on one device", op)
     return dev
 
 
 def _ptr(t):
-    return None if t is None or t.numel() == 0 else t.data_ptr()
-
-
-def _stream(dev):
-    return torch.cuda.current_stream(dev).cuda_stream
+    return 0 if t is None else t.data_ptr()
 
 
 def _span(t):
     """first and last byte a tensor reaches"""
-    lo = hi = t.data_ptr()
-    for n, s in zip(t.shape, t.stride()):
-        lo, hi = (lo + (n - 1) * s * t.element_size(), hi) if s < 0 else (lo, hi + (n - 1) * s * t.element_size())
-    return lo, hi + t.element_size()
+    lo = t.data_ptr()
+    return lo, lo + t.element_size() * (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride())))
 
 
 def _apart(op, out, name, *inputs):
@@ -61,59 +60,64 @@ def _apart(op, out, name, *inputs):
     for t in inputs:
         if t is not None and t.numel() and t.device == out.device:
             a, b = _span(t)
-            _need(hi <= a or b <= lo, "%s: %s overlaps an input", op, name)
+            if not (hi <= a or b <= lo):
+                _bad("%s: %s overlaps an input", op, name)
 
 
 def _workspace(fn, dev, *structs):
     nbytes = C.c_uint64()
-    _lib.check_policy(fn(*[C.byref(s) for s in structs], C.byref(nbytes)), fn.__name__)
+    _lib.check_policy(fn(*structs, C.byref(nbytes)), fn.__name__)
     return None if nbytes.value == 0 else torch.empty(nbytes.value, dtype=torch.uint8, device=dev)
 
 
 # ---- linear_scan ---------------------------------------------------------------------------------------------------------------
-def _scan_struct(x, gate, done, reverse):
-    s = _lib.CeScan(abi_version=_lib.POLICY_ABI_VERSION, device=x.device.index, dtype=_CODE[x.dtype], flags=_lib.SCAN_REVERSE * bool(reverse))
-    s.steps, s.rows, s.channels = x.shape
-    s.x_step, s.x_row = x.stride(0), x.stride(1)
-    s.x = _ptr(x)
+def _scan_struct(x, gate, done, reverse, state, y, last, saved, ws):
+    T, E, Ch = x.shape
+    xs, code = x.stride(), _CODE[x.dtype]
     if isinstance(gate, torch.Tensor):
-        s.gate_dtype, s.heads, s.gate_step, s.gate_row, s.gate = _CODE[gate.dtype], gate.shape[2], gate.stride(0), gate.stride(1), gate.data_ptr()
+        gs, gcode, heads, decay, gptr = gate.stride(), _CODE[gate.dtype], gate.shape[2], 0.0, gate.data_ptr()
     else:
-        s.gate_dtype, s.heads, s.decay = s.dtype, s.channels, gate
-    if done is not None:
-        s.done_step, s.done_row, s.done = done.stride(0), done.stride(1), _ptr(done)
-    return s
+        gs, gcode, heads, decay, gptr = (0, 0), code, Ch, gate, 0
+    ds, dptr = (done.stride(), done.data_ptr()) if done is not None else ((0, 0), 0)
+    return _scan_args(_ABI, x.device.index, code, gcode, _lib.SCAN_REVERSE if reverse else 0, 0, T, E, Ch, heads, xs[0], xs[1], gs[0], gs[1], ds[0], ds[1], decay,
+                      x.data_ptr(), gptr, dptr, _ptr(state), _ptr(y), _ptr(last), _ptr(saved), _ptr(ws), 0 if ws is None else ws.numel())
 
 
 def _scan_forward(x, gate, state, done, reverse, y, last, want_saved):
     L = _lib.load_policy()
     T, E, Ch = x.shape
-    acc = torch.float64 if x.dtype == torch.float64 else torch.float32
-    y = torch.empty((T, E, Ch), dtype=x.dtype, device=x.device) if y is None else y
-    last = torch.empty((E, Ch), dtype=acc, device=x.device) if last is None else last
-    saved = torch.empty((-(-T // _lib.SCAN_SAVED_STEPS), E, Ch), dtype=torch.float32, device=x.device) if want_saved else None
-    s = _scan_struct(x, gate, done, reverse)
-    s.y, s.last, s.state, s.saved = _ptr(y), _ptr(last), _ptr(state), _ptr(saved)
-    ws = _workspace(L.ce_linear_scan_workspace, x.device, s)
-    s.workspace, s.workspace_bytes = _ptr(ws), 0 if ws is None else ws.numel()
-    _lib.check_policy(L.ce_linear_scan(C.byref(s), _stream(x.device)), "linear_scan")
+    dev = x.device
+    if y is None:
+        y = torch.empty((T, E, Ch), dtype=x.dtype, device=dev)
+    if last is None:
+        last = torch.empty((E, Ch), dtype=torch.float64 if x.dtype == torch.float64 else torch.float32, device=dev)
+    saved = torch.empty((-(-T // _lib.SCAN_SAVED_STEPS), E, Ch), dtype=torch.float32, device=dev) if want_saved else None
+    ws = None
+    if T >= _lib.SCAN_SPLIT_STEPS:
+        ws = _workspace(L.ce_linear_scan_workspace, dev, _scan_struct(x, gate, done, reverse, state, y, last, saved, None))
+    rc = L.ce_linear_scan(_scan_struct(x, gate, done, reverse, state, y, last, saved, ws), _stream(dev.index))
+    if rc:
+        _lib.check_policy(rc, "linear_scan")
     return y, last, saved
 
 
 def _scan_backward(x, gate, done, reverse, saved, dy, dlast, need_state):
     L = _lib.load_policy()
     T, E, Ch = x.shape
-    dx = torch.empty((T, E, Ch), dtype=x.dtype, device=x.device)
-    dgate = (torch.empty if x.numel() else torch.zeros)(gate.shape, dtype=gate.dtype, device=x.device) if isinstance(gate, torch.Tensor) else None
-    dstate = torch.empty((E, Ch), dtype=torch.float32, device=x.device) if need_state else None
-    s = _scan_struct(x, gate, done, reverse)
-    s.saved = _ptr(saved)
-    dy = torch.zeros((T, E, Ch), dtype=x.dtype, device=x.device) if dy is None else dy.contiguous()
-    dlast = None if dlast is None else dlast.contiguous()
-    g = _lib.CeScanGrad(dy=_ptr(dy), dlast=_ptr(dlast), dx=_ptr(dx), dgate=_ptr(dgate), dstate=_ptr(dstate))
-    ws = _workspace(L.ce_linear_scan_backward_workspace, x.device, s, g)
-    s.workspace, s.workspace_bytes = _ptr(ws), 0 if ws is None else ws.numel()
-    _lib.check_policy(L.ce_linear_scan_backward(C.byref(s), C.byref(g), _stream(x.device)), "linear_scan_backward")
+    dev = x.device
+    dx = torch.empty((T, E, Ch), dtype=x.dtype, device=dev)
+    dgate = (torch.empty if x.numel() else torch.zeros)(gate.shape, dtype=gate.dtype, device=dev) if isinstance(gate, torch.Tensor) else None
+    dstate = torch.empty((E, Ch), dtype=torch.float32, device=dev) if need_state else None
+    dy = torch.zeros((T, E, Ch), dtype=x.dtype, device=dev) if dy is None else dy if dy.is_contiguous() else dy.contiguous()
+    if dlast is not None and not dlast.is_contiguous():
+        dlast = dlast.contiguous()
+    g = _scan_grad_args(dy.data_ptr(), _ptr(dlast), dx.data_ptr(), _ptr(dgate), _ptr(dstate))
+    ws = None
+    if T >= _lib.SCAN_SPLIT_STEPS or (dgate is not None and gate.shape[2] != Ch):
+        ws = _workspace(L.ce_linear_scan_backward_workspace, dev, _scan_struct(x, gate, done, reverse, None, None, None, saved, None), g)
+    rc = L.ce_linear_scan_backward(_scan_struct(x, gate, done, reverse, None, None, None, saved, ws), g, _stream(dev.index))
+    if rc:
+        _lib.check_policy(rc, "linear_scan_backward")
     return dx, dgate, dstate
 
 
@@ -149,41 +153,55 @@ def linear_scan(x, gate, state=None, done=None, reverse=False, out=None, state_o
     The state is float32 throughout (float64 with x); y is rounded once.  Differentiable in x, gate and state (dy and dlast), from the
     unrounded states: one of every 16 is kept between the passes.  out / state_out: dense tensors to write to, without gradients;
     state_out may be `state`."""
-    _need(isinstance(x, torch.Tensor) and x.dim() == 3, "linear_scan: x must be [T, E, C]")
+    if not isinstance(x, torch.Tensor) or x.dim() != 3:
+        _bad("linear_scan: x must be [T, E, C]")
     tensor_gate = isinstance(gate, torch.Tensor)
-    dev = _device("linear_scan", x, gate if tensor_gate else None, state, done, out, state_out)
-    _need(x.dtype in _REAL or x.dtype == torch.float64, "linear_scan: x must be float32, bfloat16, float16 or float64, not %s", x.dtype)
+    _device("linear_scan", x, gate if tensor_gate else None, state, done, out, state_out)
+    dtype = x.dtype
+    double = dtype == torch.float64
+    if dtype not in _REAL and not double:
+        _bad("linear_scan: x must be float32, bfloat16, float16 or float64, not %s", dtype)
     T, E, Ch = x.shape
-    acc = torch.float64 if x.dtype == torch.float64 else torch.float32
+    acc = torch.float64 if double else torch.float32
+    far = (1 << 28) // (255 // max(Ch, 1) + 1)  # rows that far apart are more than a wave's 32-bit offsets
+    strides = x.stride()
+    grad = x.requires_grad
     if tensor_gate:
-        _need(gate.dim() == 3 and gate.shape[:2] == x.shape[:2] and (gate.shape[2] == Ch or (gate.shape[2] and Ch % gate.shape[2] == 0)),
-              "linear_scan: gate must be [T, E, H] with H dividing C, got %s for x %s", tuple(gate.shape), tuple(x.shape))
-        _need(gate.dtype == x.dtype or (gate.dtype == torch.float32 and x.dtype in _REAL), "linear_scan: gate must be of x's type or float32, not %s", gate.dtype)
+        if gate.dim() != 3 or gate.shape[0] != T or gate.shape[1] != E or not (gate.shape[2] == Ch or (gate.shape[2] and Ch % gate.shape[2] == 0)):
+            _bad("linear_scan: gate must be [T, E, H] with H dividing C, got %s for x %s", tuple(gate.shape), tuple(x.shape))
+        if gate.dtype != dtype and (gate.dtype != torch.float32 or double):
+            _bad("linear_scan: gate must be of x's type or float32, not %s", gate.dtype)
+        grad = grad or gate.requires_grad
+        s = gate.stride()
+        if (s[2] != 1 and gate.shape[2] > 1) or s[1] > far:
+            gate = gate.contiguous()
     else:
         gate = float(gate)
     if state is not None:
-        _need(tuple(state.shape) == (E, Ch) and state.dtype == acc, "linear_scan: state must be %s %s", acc, (E, Ch))
+        if state.dim() != 2 or state.shape[0] != E or state.shape[1] != Ch or state.dtype != acc:
+            _bad("linear_scan: state must be %s %s", acc, (E, Ch))
+        grad = grad or state.requires_grad
     if done is not None:
-        _need(tuple(done.shape) == (T, E) and done.dtype in (torch.bool, torch.uint8), "linear_scan: done must be bool or uint8 [T, E]")
-        done = done.view(torch.uint8) if done.dtype == torch.bool else done
-    grad = torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in (x, gate, state))
-    for name, t, shape, dtype in (("out", out, (T, E, Ch), x.dtype), ("state_out", state_out, (E, Ch), acc)):
-        if t is not None:
-            _need(not grad, "linear_scan: %s cannot be given where gradients are wanted", name)
-            _need(tuple(t.shape) == shape and t.dtype == dtype and t.is_contiguous(), "linear_scan: %s must be a dense %s %s", name, dtype, shape)
-    far = (1 << 28) // (255 // max(Ch, 1) + 1)  # rows that far apart are more than a wave's 32-bit offsets
-    if (x.stride(2) != 1 and Ch > 1) or x.stride(1) > far:
+        if done.dim() != 2 or done.shape[0] != T or done.shape[1] != E or done.dtype not in (torch.bool, torch.uint8):
+            _bad("linear_scan: done must be bool or uint8 [T, E]")
+    if (strides[2] != 1 and Ch > 1) or strides[1] > far:
         x = x.contiguous()
-    if tensor_gate and ((gate.stride(2) != 1 and gate.shape[2] > 1) or gate.stride(1) > far):
-        gate = gate.contiguous()
-    in_place = state_out is not None and state is not None and state_out.data_ptr() == state.data_ptr()
-    _need(not in_place or state.is_contiguous(), "linear_scan: state_out overlaps an input")
-    if state is not None:
+    grad = grad and torch.is_grad_enabled()
+    if out is not None or state_out is not None:
+        if grad:
+            _bad("linear_scan: out and state_out cannot be given where gradients are wanted")
+        for name, t, shape, kind in (("out", out, (T, E, Ch), dtype), ("state_out", state_out, (E, Ch), acc)):
+            if t is not None and (tuple(t.shape) != shape or t.dtype != kind or not t.is_contiguous()):
+                _bad("linear_scan: %s must be a dense %s %s", name, kind, shape)
+        moved = state is not None and state.is_contiguous() and state_out is not None and state_out.data_ptr() == state.data_ptr()  # in place
+        others = (x, gate if tensor_gate else None, done)
+        _apart("linear_scan", out, "out", state, state_out, *others)
+        _apart("linear_scan", state_out, "state_out", None if moved else state, *others)
+    if state is not None and not state.is_contiguous():
         state = state.contiguous()
-    _apart("linear_scan", out, "out", x, gate if tensor_gate else None, state, done, state_out)
-    _apart("linear_scan", state_out, "state_out", x, gate if tensor_gate else None, None if in_place else state, done)
     if grad:
-        _need(x.dtype != torch.float64, "linear_scan: float64 has no backward pass")
+        if double:
+            _bad("linear_scan: float64 has no backward pass")
         return _Scan.apply(x, gate, state, done, bool(reverse))
     y, last, _ = _scan_forward(x, gate, state, done, reverse, out, state_out, False)
     return y, last
@@ -198,30 +216,42 @@ def advantages(reward, value, last_value=None, done=None, gamma=0.99, lam=0.95, 
     last_value: [E, n] in value's type; done: [P, E] (the env's) or [P, E, n] (each agent's), bool or uint8.  Time t lies in plane
     (first_plane + t) % P, as a wrapped `Trajectory` holds it (its oldest plane is `traj.c.first_plane`).  Sums run in float64.
     out: a pair of dense float32 [P, E, n] tensors.  Not differentiable: targets are constants of a policy's loss."""
-    _need(isinstance(reward, torch.Tensor) and reward.dim() == 3, "advantages: reward must be [P, E, n]")
+    if not isinstance(reward, torch.Tensor) or reward.dim() != 3:
+        _bad("advantages: reward must be [P, E, n]")
     adv, ret = (None, None) if out is None else out
     dev = _device("advantages", reward, value, last_value, done, adv, ret)
-    P, E, n = reward.shape
-    _need(reward.dtype in (torch.float64, torch.float32), "advantages: reward must be float64 or float32, not %s", reward.dtype)
-    _need(tuple(value.shape) == (P, E, n) and value.dtype in _REAL, "advantages: value must be float32, bfloat16 or float16 %s", (P, E, n))
-    _need(last_value is None or (tuple(last_value.shape) == (E, n) and last_value.dtype == value.dtype), "advantages: last_value must be %s %s", value.dtype, (E, n))
-    _need(done is None or (tuple(done.shape) in ((P, E), (P, E, n)) and done.dtype in (torch.bool, torch.uint8)), "advantages: done must be bool or uint8 [P, E] or [P, E, n]")
-    _need(0 <= int(first_plane) < max(P, 1), "advantages: first_plane out of range")
-    for t in (adv, ret):
-        _need(t is None or (tuple(t.shape) == (P, E, n) and t.dtype == torch.float32 and t.is_contiguous()), "advantages: out must be two dense float32 %s", (P, E, n))
-    reward, value = reward.detach().contiguous(), value.detach().contiguous()
-    last_value = None if last_value is None else last_value.detach().contiguous()
-    done = None if done is None else done.contiguous()
-    _apart("advantages", adv, "out", reward, value, last_value, done, ret)
-    _apart("advantages", ret, "out", reward, value, last_value, done)
-    adv = torch.empty((P, E, n), dtype=torch.float32, device=dev) if adv is None else adv
-    ret = torch.empty((P, E, n), dtype=torch.float32, device=dev) if ret is None else ret
-    a = _lib.CeAdvantage(abi_version=_lib.POLICY_ABI_VERSION, device=dev.index, reward_dtype=_CODE[reward.dtype], value_dtype=_CODE[value.dtype],
-                         flags=_lib.ADV_DONE_PER_AGENT * (done is not None and done.dim() == 3), first_plane=int(first_plane), planes=P, rows=E, agents=n,
-                         gamma=float(gamma), lam=float(lam), reward=_ptr(reward), value=_ptr(value), last_value=_ptr(last_value), done=_ptr(done),
-                         advantage=_ptr(adv), ret=_ptr(ret))
-    L = _lib.load_policy()
-    _lib.check_policy(L.ce_advantages(C.byref(a), _stream(dev)), "advantages")
+    shape = P, E, n = reward.shape
+    if reward.dtype != torch.float64 and reward.dtype != torch.float32:
+        _bad("advantages: reward must be float64 or float32, not %s", reward.dtype)
+    if value.shape != shape or value.dtype not in _REAL:
+        _bad("advantages: value must be float32, bfloat16 or float16 %s", tuple(shape))
+    if last_value is not None:
+        if last_value.shape != shape[1:] or last_value.dtype != value.dtype:
+            _bad("advantages: last_value must be %s %s", value.dtype, (E, n))
+        last_value = last_value.contiguous()
+    per_agent = False
+    if done is not None:
+        per_agent = done.dim() == 3
+        if done.shape != (shape if per_agent else shape[:2]) or done.dtype not in (torch.bool, torch.uint8):
+            _bad("advantages: done must be bool or uint8 [P, E] or [P, E, n]")
+        done = done.contiguous()
+    first_plane = int(first_plane)
+    if not 0 <= first_plane < max(P, 1):
+        _bad("advantages: first_plane out of range")
+    reward, value = reward.contiguous(), value.contiguous()
+    if out is None:
+        adv, ret = torch.empty(shape, dtype=torch.float32, device=dev), torch.empty(shape, dtype=torch.float32, device=dev)
+    else:
+        for t in out:
+            if t.shape != shape or t.dtype != torch.float32 or not t.is_contiguous():
+                _bad("advantages: out must be two dense float32 %s", tuple(shape))
+        _apart("advantages", adv, "out", reward, value, last_value, done, ret)
+        _apart("advantages", ret, "out", reward, value, last_value, done)
+    a = _adv_args(_ABI, dev.index, _CODE[reward.dtype], _CODE[value.dtype], _lib.ADV_DONE_PER_AGENT if per_agent else 0, first_plane, P, E, n, float(gamma),
+                  float(lam), reward.data_ptr(), value.data_ptr(), _ptr(last_value), _ptr(done), adv.data_ptr(), ret.data_ptr())
+    rc = _lib.load_policy().ce_advantages(a, _stream(dev.index))
+    if rc:
+        _lib.check_policy(rc, "advantages")
     return adv, ret
 
 
@@ -234,38 +264,37 @@ def pack_mask(allowed):
     return torch.where(words >= 2 ** 31, words - 2 ** 32, words).to(torch.int32)
 
 
-def _logits_struct(logits, h, out_dtype):
-    s = _lib.CeLogits(abi_version=_lib.POLICY_ABI_VERSION, device=logits.device.index, dtype=_CODE[logits.dtype], out_dtype=_CODE[out_dtype])
-    s.rows, s.vocab = logits.shape
-    s.logits_row, s.logits = logits.stride(0), _ptr(logits)
-    if h["tokens"] is not None:
-        t = h["tokens"]
-        s.token_dtype, s.history, s.token_row, s.token_step, s.tokens = _CODE[t.dtype], t.shape[1], t.stride(0), t.stride(1), _ptr(t)
-        s.lengths, s.prompt_lengths = (_ptr(h["lengths"]), _ptr(h["prompt_lengths"])) if s.tokens else (None, None)
-        for name in ("repetition", "presence", "frequency"):
-            v = h[name]
-            if isinstance(v, torch.Tensor):
-                setattr(s, name, _ptr(v))
-            else:
-                setattr(s, name + "_all", v)
-    if h["mask"] is not None:
-        s.mask_dtype, s.mask_rows, s.mask, s.mask_index = _CODE[h["mask"].dtype], h["mask"].shape[0], _ptr(h["mask"]), _ptr(h["mask_index"])
-    return s
+class _Shaping:
+    """what scores are shaped with, checked and laid out: everything of a ce_logits but the scores, the bias and the output"""
+    __slots__ = ("tokens", "lengths", "prompt_lengths", "repetition", "presence", "frequency", "mask", "mask_index")
 
-
-def _logits_bias(s, bias):
-    if bias is not None:
-        s.bias_dtype, s.bias_rows, s.bias = _CODE[bias.dtype], bias.shape[0], _ptr(bias)
+    def struct(self, rows, V, logits, row, bias, out_dtype, out, out_row, ws):
+        t, m, scalar, ptr = self.tokens, self.mask, [1.0, 0.0, 0.0], [0, 0, 0]
+        if t is not None and t.numel():
+            for k, v in enumerate((self.repetition, self.presence, self.frequency)):
+                if isinstance(v, torch.Tensor):
+                    ptr[k] = v.data_ptr()
+                else:
+                    scalar[k] = v
+            history = (t.stride(0), t.stride(1), t.shape[1], _CODE[t.dtype], t.data_ptr(), _ptr(self.lengths), _ptr(self.prompt_lengths))
+        else:
+            history = (0, 0, 0, 0, 0, 0, 0)
+        return _logits_args(_ABI, logits.device.index, _CODE[logits.dtype], _CODE[out_dtype], history[3], 0 if bias is None else _CODE[bias.dtype],
+                            0 if m is None else _CODE[m.dtype], 0, rows, V, history[2], row, out_row, history[0], history[1], 0 if bias is None else bias.shape[0],
+                            0 if m is None else m.shape[0], scalar[0], scalar[1], scalar[2], logits.data_ptr(), history[4], history[5], history[6], ptr[0], ptr[1], ptr[2],
+                            _ptr(bias), _ptr(m), _ptr(self.mask_index), _ptr(out), _ptr(ws), 0 if ws is None else ws.numel())
 
 
 class _Logits(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, bias, h):
         ctx.set_materialize_grads(False)
-        ctx.h = {k: v for k, v in h.items() if not isinstance(v, torch.Tensor)}
-        ctx.names = [k for k, v in h.items() if isinstance(v, torch.Tensor)]
-        ctx.save_for_backward(logits, bias, *[h[k] for k in ctx.names])
-        return _logits_forward(logits, bias, h, None)
+        ctx.rest = [(k, v) for k in _Shaping.__slots__ for v in (getattr(h, k),) if not isinstance(v, torch.Tensor)]
+        ctx.names = [k for k in _Shaping.__slots__ if isinstance(getattr(h, k), torch.Tensor)]
+        ctx.save_for_backward(logits, bias, *[getattr(h, k) for k in ctx.names])
+        out = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+        _logits_forward(logits, logits.shape[0], logits.shape[1], logits.stride(0), bias, h, out, logits.shape[1])
+        return out
 
     @staticmethod
     @torch.autograd.function.once_differentiable
@@ -273,40 +302,57 @@ class _Logits(torch.autograd.Function):
         if dz is None:
             return None, None, None
         logits, bias, *rest = ctx.saved_tensors
-        h = dict(ctx.h, **dict(zip(ctx.names, rest)))
+        h = _Shaping()
+        for k, v in ctx.rest:
+            setattr(h, k, v)
+        for k, v in zip(ctx.names, rest):
+            setattr(h, k, v)
         L = _lib.load_policy()
-        dz = dz if dz.stride(1) == 1 or dz.shape[1] == 1 else dz.contiguous()
-        dlogits = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device) if ctx.needs_input_grad[0] else None
-        dbias = torch.zeros_like(bias) if ctx.needs_input_grad[1] and logits.numel() == 0 else torch.empty_like(bias) if ctx.needs_input_grad[1] else None
-        s = _logits_struct(logits, h, dz.dtype)
-        _logits_bias(s, bias)
-        g = _lib.CeLogitsGrad(dout=_ptr(dz), dout_row=dz.stride(0), dlogits=_ptr(dlogits), dbias=_ptr(dbias))
-        ws = _workspace(L.ce_process_logits_backward_workspace, logits.device, s, g)
-        s.workspace, s.workspace_bytes = _ptr(ws), 0 if ws is None else ws.numel()
-        _lib.check_policy(L.ce_process_logits_backward(C.byref(s), C.byref(g), _stream(logits.device)), "process_logits_backward")
+        rows, V = logits.shape
+        dev = logits.device
+        if dz.stride(1) != 1 and V > 1:
+            dz = dz.contiguous()
+        dlogits = torch.empty((rows, V), dtype=logits.dtype, device=dev) if ctx.needs_input_grad[0] else None
+        dbias = (torch.empty_like if logits.numel() else torch.zeros_like)(bias) if ctx.needs_input_grad[1] else None
+        g = _logits_grad_args(dz.data_ptr(), dz.stride(0), _ptr(dlogits), _ptr(dbias))
+        ws = None
+        if dbias is not None:
+            ws = _workspace(L.ce_process_logits_backward_workspace, dev, h.struct(rows, V, logits, logits.stride(0), bias, dz.dtype, None, 0, None), g)
+        rc = L.ce_process_logits_backward(h.struct(rows, V, logits, logits.stride(0), bias, dz.dtype, None, 0, ws), g, _stream(dev.index))
+        if rc:
+            _lib.check_policy(rc, "process_logits_backward")
         return dlogits, dbias, None
 
 
-def _logits_forward(logits, bias, h, out):
-    L = _lib.load_policy()
-    out = torch.empty(logits.shape, dtype=h["out_dtype"], device=logits.device) if out is None else out
-    s = _logits_struct(logits, h, out.dtype)
-    _logits_bias(s, bias)
-    s.out, s.out_row = _ptr(out), out.stride(0)
-    _lib.check_policy(L.ce_process_logits(C.byref(s), _stream(logits.device)), "process_logits")
-    return out
+def _logits_forward(logits, rows, V, row, bias, h, out, out_row):
+    rc = _lib.load_policy().ce_process_logits(h.struct(rows, V, logits, row, bias, out.dtype, out, out_row, None), _stream(logits.device.index))
+    if rc:
+        _lib.check_policy(rc, "process_logits")
 
 
-def _table(op, name, t, lead, width):
-    """a [.., width] table whose rows repeat over the logits' rows, as [B, width]"""
+def _table(name, t, lead, width):
+    """a [.., width] table whose rows repeat over the logits' rows, as a dense [B, width]"""
     k = t.dim() - 1
-    rows = 1
-    for d in lead:
-        rows *= d
-    _need(k >= 0 and t.shape[-1] == width, "%s: %s must end in %d entries, got %s", op, name, width, tuple(t.shape))
-    _need(k == 0 or (k == 1 and (len(lead) <= 1 or t.shape[0] == 1)) or tuple(t.shape[:-1]) == tuple(lead)[len(lead) - k:], "%s: %s's leading axes %s must be the last of the logits' %s", op, name, tuple(t.shape[:-1]), tuple(lead))
-    t = t.reshape(-1, width) if t.numel() else t.reshape(t.shape[0] if k else 1, width)
-    return t.contiguous()
+    if k < 0 or t.shape[-1] != width:
+        _bad("process_logits: %s must end in %d entries, got %s", name, width, tuple(t.shape))
+    if k == 1:
+        if len(lead) > 1 and t.shape[0] != 1 and t.shape[0] != lead[-1]:
+            _bad("process_logits: %s's leading axes %s must be the last of the logits' %s", name, tuple(t.shape[:-1]), tuple(lead))
+        return t if t.is_contiguous() else t.contiguous()
+    if k > 1 and tuple(t.shape[:-1]) != tuple(lead)[len(lead) - k:]:
+        _bad("process_logits: %s's leading axes %s must be the last of the logits' %s", name, tuple(t.shape[:-1]), tuple(lead))
+    return t.reshape(t.shape[:-1].numel(), width).contiguous()
+
+
+def _per_row(name, t, lead, dtype):
+    """one entry a row, dense, in dtype (int64 is narrowed)"""
+    if t.shape != lead:
+        _bad("process_logits: %s must hold one entry a row, %s, got %s", name, tuple(lead), tuple(t.shape))
+    if t.dtype != dtype:
+        if dtype != torch.int32 or t.dtype != torch.int64:
+            _bad("process_logits: %s must be %s, not %s", name, dtype, t.dtype)
+        t = t.clamp(-1, 2 ** 31 - 1).to(torch.int32)
+    return t if t.is_contiguous() else t.contiguous()
 
 
 def process_logits(logits, *, tokens=None, lengths=None, prompt_lengths=None, repetition=1.0, presence=0.0, frequency=0.0, bias=None, mask=None,
@@ -327,59 +373,74 @@ def process_logits(logits, *, tokens=None, lengths=None, prompt_lengths=None, re
                   (`step_policy_device(.., "argmax")` then takes action 0).
     out: float32 or the logits' type, rows dense; it may be `logits` itself; not where gradients are wanted.
     Differentiable in logits and bias: gradients scale as l was, vanish where forbidden; bias gradients sum over rows in float32."""
-    op = "process_logits"
-    _need(isinstance(logits, torch.Tensor) and logits.dim() >= 1, "process_logits: logits must be [..., V]")
-    penal = [v for v in (repetition, presence, frequency) if isinstance(v, torch.Tensor)]
-    dev = _device(op, logits, tokens, lengths, prompt_lengths, bias, mask, mask_index, out, *penal)
-    _need(logits.dtype in _REAL, "process_logits: logits must be float32, bfloat16 or float16, not %s", logits.dtype)
-    lead, V = tuple(logits.shape[:-1]), logits.shape[-1]
-    rows = logits.shape[:-1].numel()
-    h = dict(tokens=None, lengths=None, prompt_lengths=None, mask=None, mask_index=None, out_dtype=logits.dtype)
-
-    def per_row(name, t, dtype):
-        _need(tuple(t.shape) == lead, "process_logits: %s must hold one entry a row, %s, got %s", name, lead, tuple(t.shape))
-        _need(t.dtype in dtype, "process_logits: %s must be %s, not %s", name, dtype[0], t.dtype)
-        return t.detach().to(dtype[0]).reshape(-1).contiguous()
-
+    if not isinstance(logits, torch.Tensor) or logits.dim() < 1:
+        _bad("process_logits: logits must be [..., V]")
+    dtype = logits.dtype
+    if dtype not in _REAL:
+        _bad("process_logits: logits must be float32, bfloat16 or float16, not %s", dtype)
+    dev = _device("process_logits", logits, tokens, lengths, prompt_lengths, bias, mask, mask_index, out)
+    lead, V = logits.shape[:-1], logits.shape[-1]
+    rows = lead.numel()
+    h = _Shaping()
     for name, v in (("repetition", repetition), ("presence", presence), ("frequency", frequency)):
-        h[name] = per_row(name, v, (torch.float32,)) if isinstance(v, torch.Tensor) else float(v)
-    _need(tokens is not None or (lengths is None and prompt_lengths is None), "process_logits: lengths without tokens")
+        if isinstance(v, torch.Tensor):
+            if v.device != dev:
+                _bad("process_logits: all tensors must live on one device")
+            setattr(h, name, _per_row(name, v, lead, torch.float32))
+        else:
+            setattr(h, name, float(v))
+    h.tokens = h.lengths = h.prompt_lengths = h.mask = h.mask_index = None
     if tokens is not None:
-        _need(tokens.dim() == logits.dim() and tuple(tokens.shape[:-1]) == lead, "process_logits: tokens must be %s + [L], got %s", lead, tuple(tokens.shape))
-        _need(tokens.dtype in (torch.uint8, torch.int32, torch.int64), "process_logits: tokens must be uint8, int32 or int64, not %s", tokens.dtype)
-        h["tokens"] = tokens.reshape(rows, tokens.shape[-1])
+        if tokens.dim() != logits.dim() or tokens.shape[:-1] != lead:
+            _bad("process_logits: tokens must be %s + [L], got %s", tuple(lead), tuple(tokens.shape))
+        if tokens.dtype not in (torch.uint8, torch.int32, torch.int64):
+            _bad("process_logits: tokens must be uint8, int32 or int64, not %s", tokens.dtype)
+        h.tokens = tokens if tokens.dim() == 2 else tokens.reshape(rows, tokens.shape[-1])
         if lengths is not None:
-            h["lengths"] = per_row("lengths", lengths, (torch.int32, torch.int64))
+            h.lengths = _per_row("lengths", lengths, lead, torch.int32)
         if prompt_lengths is not None:
-            h["prompt_lengths"] = per_row("prompt_lengths", prompt_lengths, (torch.int32, torch.int64))
+            h.prompt_lengths = _per_row("prompt_lengths", prompt_lengths, lead, torch.int32)
+    elif lengths is not None or prompt_lengths is not None:
+        _bad("process_logits: lengths without tokens")
     if mask is not None:
-        _need(mask.dtype in (torch.bool, torch.uint8, torch.int32), "process_logits: mask must be bool, uint8 or int32 words, not %s", mask.dtype)
-        packed = mask.dtype == torch.int32
+        if mask.dtype not in (torch.bool, torch.uint8, torch.int32):
+            _bad("process_logits: mask must be bool, uint8 or int32 words, not %s", mask.dtype)
         if mask_index is not None:
-            _need(mask.dim() == 2, "process_logits: an indexed mask must be a table [S, ..]")
-            h["mask_index"] = per_row("mask_index", mask_index, (torch.int32, torch.int64))
-        mask = mask.view(torch.uint8) if mask.dtype == torch.bool else mask
-        h["mask"] = _table(op, "mask", mask, lead, -(-V // 32) if packed else V)
-    else:
-        _need(mask_index is None, "process_logits: mask_index without a mask")
+            if mask.dim() != 2:
+                _bad("process_logits: an indexed mask must be a table [S, ..]")
+            h.mask_index = _per_row("mask_index", mask_index, lead, torch.int32)
+        h.mask = _table("mask", mask, () if mask_index is not None else lead, -(-V // 32) if mask.dtype == torch.int32 else V)
+    elif mask_index is not None:
+        _bad("process_logits: mask_index without a mask")
+    grad = logits.requires_grad
     if bias is not None:
-        _need(bias.dtype in (torch.float32, logits.dtype), "process_logits: bias must be float32 or of the logits' type, not %s", bias.dtype)
-        bias = _table(op, "bias", bias, lead, V)
-    flat = logits.reshape(rows, V)
+        if bias.dtype != torch.float32 and bias.dtype != dtype:
+            _bad("process_logits: bias must be float32 or of the logits' type, not %s", bias.dtype)
+        bias = _table("bias", bias, lead, V)
+        grad = grad or bias.requires_grad
+    grad = grad and torch.is_grad_enabled()
+    if grad and out is not None:
+        _bad("process_logits: out cannot be given where gradients are wanted")
+    flat = logits if logits.dim() == 2 else logits.reshape(rows, V)
     if V > 1 and flat.stride(1) != 1:
         flat = flat.contiguous()
-    grad = torch.is_grad_enabled() and (logits.requires_grad or (bias is not None and bias.requires_grad))
-    if out is not None:
-        _need(not grad, "process_logits: out cannot be given where gradients are wanted")
-        _need(out.shape == logits.shape and out.dtype in (torch.float32, logits.dtype), "process_logits: out must be %s, float32 or of the logits' type", tuple(logits.shape))
-        try:
-            to = out.view(rows, V)
-        except RuntimeError:
-            to = None
-        _need(to is not None and (V <= 1 or to.stride(1) == 1), "process_logits: out's leading axes must collapse into one stride, its last be dense")
-        same = to.data_ptr() == flat.data_ptr() and to.dtype == flat.dtype and to.stride() == flat.stride()
-        _apart(op, to, "out", None if same else flat, h["tokens"], h["lengths"], h["prompt_lengths"], h["mask"], h["mask_index"], bias,
-               *[h[k] for k in ("repetition", "presence", "frequency") if isinstance(h[k], torch.Tensor)])
-        _logits_forward(flat, bias, h, to)
+    if grad:
+        z = _Logits.apply(flat, bias, h)
+        return z if logits.dim() == 2 else z.view(logits.shape)
+    if out is None:
+        out = torch.empty(logits.shape, dtype=dtype, device=dev)
+        _logits_forward(flat, rows, V, flat.stride(0), bias, h, out, V)
         return out
-    return (_Logits.apply(flat, bias, h) if grad else _logits_forward(flat, bias, h, None)).view(logits.shape)
+    if out.shape != logits.shape or (out.dtype != torch.float32 and out.dtype != dtype):
+        _bad("process_logits: out must be %s, float32 or of the logits' type", tuple(logits.shape))
+    try:
+        to = out.view(rows, V)
+    except RuntimeError:
+        to = None
+    if to is None or (V > 1 and to.stride(1) != 1):
+        _bad("process_logits: out's leading axes must collapse into one stride, its last be dense")
+    same = to.data_ptr() == flat.data_ptr() and to.dtype == flat.dtype and to.stride() == flat.stride()
+    _apart("process_logits", to, "out", None if same else flat, h.tokens, h.lengths, h.prompt_lengths, h.mask, h.mask_index, bias,
+           *[v for v in (h.repetition, h.presence, h.frequency) if isinstance(v, torch.Tensor)])
+    _logits_forward(flat, rows, V, flat.stride(0), bias, h, to, to.stride(0))
+    return out

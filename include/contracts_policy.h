@@ -45,6 +45,7 @@ const char* ce_policy_error(void);
  * negative, and rows of under 256 channels lie less than 2^28 elements apart per row that a wave of 256 channels spans. */
 #define CE_SCAN_REVERSE 1u
 #define CE_SCAN_SAVED_STEPS 16 /* saved: float [ceil(T / 16)][E][C], what ce_linear_scan_backward starts its tiles from */
+#define CE_SCAN_SPLIT_STEPS 512 /* a call of fewer steps needs no workspace (its time axis is never split over blocks) */
 
 typedef struct ce_scan {
   uint32_t abi_version; /* CE_POLICY_ABI_VERSION */
