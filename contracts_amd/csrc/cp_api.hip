@@ -82,31 +82,29 @@ int check_scan(const ce_scan* s) {
   return CE_OK;
 }
 
-// Lanes, waves and chunks.  The chip wants about 2048 waves in flight (2 on each of its 1024 SIMDs).  Columns give them
-// cheapest: with enough, a wave takes its columns' whole time axis on its own, 8 bytes to a lane.  Then the 4 or 8 waves of a block
-// share the time axis, which costs a second walk in registers; then lanes take fewer channels; and last the time axis is cut into chunks, which costs
-// reading x and the gate twice.  No chunk is under CE_SCAN_SPLIT_STEPS / 2 steps.
-constexpr uint64_t kWavesWanted = 2048;
-
-void share(cp::ScanParams& p, int* vec, int least, uint64_t columns, uint64_t (*blocks)(const cp::ScanParams&, uint64_t columns, int vec)) {
-  p.chunks = 1;
-  p.waves = 1;
+// Lanes, waves and chunks: what the columns leave of the chip is filled along the time axis.  Measured (us, fwd or bwd, done in 2 % of steps):
+//  * 2048 waves of columns and more: a wave takes its columns' whole time axis, 8 bytes to a lane.  [128, 4096, 128] bfloat16 75 (floor 75).
+//  * else the waves of a block share the time axis (a second walk in registers), 8 of them, and lanes take fewer channels as long as that
+//    makes waves: [512, 256, 256] bfloat16 36 with 2 channels a lane, 43 with 4, 40 with 4 waves; the gradients' longer walks do better with 4
+//    waves where 2048 can be had: 75 against 82.
+//  * under 1536 waves that way, the time axis is cut into chunks too, which costs reading x and the gate twice, at least a tile each and
+//    4096 waves in all: [65537, 1, 1024] bfloat16, 16 heads: 78 with 128 chunks and 4 channels a lane, 168 with 16 chunks and 1 channel;
+//    [1000, 37, 360] float keeps whole at 1672 waves: 31 against 36.  Gradients: [2000, 8, 2048] bfloat16 92 with 4 waves and 8 chunks, 97 whole.
+void share(cp::ScanParams& p, int* vec, bool grad, uint64_t columns, uint64_t (*blocks)(const cp::ScanParams&, uint64_t columns, int vec)) {
+  p.chunks = p.waves = 1;
   if (p.T <= CE_SCAN_SAVED_STEPS) return;
-  if (blocks(p, columns, *vec) >= kWavesWanted) return;
-  p.waves = 4;
-  while (*vec > least && blocks(p, columns, *vec) * 4 < kWavesWanted) *vec /= 2;
-  uint64_t have = blocks(p, columns, *vec);
-  if (have * 4 >= kWavesWanted || p.T < 16 * CE_SCAN_SAVED_STEPS) return;
-  p.waves = 8;
-  have *= 8;
-  uint64_t want = have ? kWavesWanted / have : 1;
-  const uint64_t most = p.T / (CE_SCAN_SPLIT_STEPS / 2);
-  want = std::min<uint64_t>({want, most, 64});
-  if (want > 1) {
-    const uint64_t tile = 8 * CE_SCAN_SAVED_STEPS, each = ((p.T + want - 1) / want + tile - 1) / tile * tile;
-    p.chunk = each;
-    p.chunks = (uint32_t)((p.T + each - 1) / each);
-  }
+  const int widest = *vec;
+  if (blocks(p, columns, widest) >= 2048) return;
+  p.waves = p.T <= 4 * CE_SCAN_SAVED_STEPS || (grad && blocks(p, columns, widest) * 4 >= 2048) ? 4 : 8;
+  const uint64_t enough = grad ? 1536 : 4096;
+  while (*vec > 1 && !grad && blocks(p, columns, *vec) * p.waves < enough) *vec /= 2;
+  if (blocks(p, columns, *vec) * p.waves >= 1536 || p.T < CE_SCAN_SPLIT_STEPS) return;
+  *vec = widest;
+  if (grad) p.waves = 4;
+  const uint64_t have = blocks(p, columns, widest) * p.waves, tile = p.waves * CE_SCAN_SAVED_STEPS;
+  const uint64_t want = std::min<uint64_t>((4096 + have - 1) / have, 128), each = ((p.T + want - 1) / want + tile - 1) / tile * tile;
+  p.chunk = each;
+  p.chunks = (uint32_t)((p.T + each - 1) / each);
 }
 
 // Waves side by side that a scan's columns make (with a head's gradient to add up, heads keep to a wave, or take several).
@@ -136,7 +134,7 @@ void plan_scan(const ce_scan* s, const ce_scan_grad* g, Plan* o) {
   p.T = T;
   p.head = (uint32_t)head;
   const bool sums = g && o->mode == cp::kGateHead;
-  share(p, &vec, 1, E * C, sums ? head_waves : flat_waves);
+  share(p, &vec, g != nullptr, E * C, sums ? head_waves : flat_waves);
   o->vec = vec;
   const bool rev = s->flags & CE_SCAN_REVERSE;
   const int64_t sign = rev ? -1 : 1, off = rev && T ? (int64_t)T - 1 : 0;

@@ -37,17 +37,36 @@ template <class X, class G, int MODE, int VEC, int W, bool REDUCE> __global__ __
     if (p.state)
 #pragma unroll
       for (int v = 0; v < VEC; ++v) h[v] = ((const A*)p.state)[ch + v];
+  }
+  int buf = 0;
+  if (!REDUCE && W > 1 && blockIdx.y > 0) {  // the chunks before this one: each wave composes its share of them, then all fold the shares
     const uint64_t EC = (uint64_t)p.cols * VEC;
-    const A* part = (const A*)p.part + ch;
-    for (uint32_t k = 0; k < blockIdx.y; ++k)
+    const uint32_t each = (blockIdx.y + W - 1) / W, k0 = w * each, k1 = k0 + each < blockIdx.y ? k0 + each : blockIdx.y;
+    A cp[VEC], cs[VEC];
 #pragma unroll
-      for (int v = 0; v < VEC; ++v) h[v] = apply(part[(uint64_t)k * 2 * EC + v], part[((uint64_t)k * 2 + 1) * EC + v], h[v]);
+    for (int v = 0; v < VEC; ++v) cp[v] = A(1), cs[v] = A(0);
+#pragma unroll 8
+    for (uint32_t k = k0; k < k1; ++k) {
+      const A* part = (const A*)p.part + (uint64_t)k * 2 * EC + ch;
+#pragma unroll
+      for (int v = 0; v < VEC; ++v) {
+        cs[v] = apply(part[v], part[EC + v], cs[v]);
+        cp[v] *= part[v];
+      }
+    }
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) fold[0][w][0][v][lane] = cp[v], fold[0][w][1][v][lane] = cs[v];
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < W; ++k)
+#pragma unroll
+      for (int v = 0; v < VEC; ++v) h[v] = apply(fold[0][k][0][v][lane], fold[0][k][1][v][lane], h[v]);
+    buf = 1;
   }
   A P[VEC];  // REDUCE: the chunk's product so far
 #pragma unroll
   for (int v = 0; v < VEC; ++v) P[v] = A(1);
 
-  int buf = 0;
   for (uint64_t tile = i0; tile < i1; tile += (uint64_t)W * kSteps) {
     const uint64_t i = tile + (uint64_t)w * kSteps;
     const int n = i >= i1 ? 0 : i1 - i < kSteps ? (int)(i1 - i) : kSteps;  // steps of this wave's run

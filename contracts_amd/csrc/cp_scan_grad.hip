@@ -62,13 +62,32 @@ template <class X, class G, int MODE, int VEC, int W, bool REDUCE> __global__ __
     if (p.dlast && !cut)
 #pragma unroll
       for (int v = 0; v < VEC; ++v) R[v] = ((const float*)p.dlast)[ch + v];
-    const float* part = (const float*)p.part + ch;
-    for (uint32_t k = p.chunks - 1; k > chunk; --k)
+  }
+  int buf = 0;
+  if (!REDUCE && W > 1 && chunk + 1 < p.chunks) {  // the chunks behind this one, last first: each wave composes its share, then all fold the shares
+    const uint32_t behind = p.chunks - 1 - chunk, each = (behind + W - 1) / W, k0 = w * each, k1 = k0 + each < behind ? k0 + each : behind;
+    float cp[VEC], cs[VEC];
 #pragma unroll
-      for (int v = 0; v < VEC; ++v) R[v] = apply(part[(uint64_t)(k - 1) * 2 * EC + v], part[((uint64_t)(k - 1) * 2 + 1) * EC + v], R[v]);
+    for (int v = 0; v < VEC; ++v) cp[v] = 1.f, cs[v] = 0.f;
+#pragma unroll 8
+    for (uint32_t k = k0; k < k1; ++k) {
+      const float* part = (const float*)p.part + (uint64_t)(p.chunks - 2 - k) * 2 * EC + ch;  // of chunk chunks - 1 - k
+#pragma unroll
+      for (int v = 0; v < VEC; ++v) {
+        cs[v] = apply(part[v], part[EC + v], cs[v]);
+        cp[v] *= part[v];
+      }
+    }
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) fold[0][w][0][v][lane] = cp[v], fold[0][w][1][v][lane] = cs[v];
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < W; ++k)
+#pragma unroll
+      for (int v = 0; v < VEC; ++v) R[v] = apply(fold[0][k][0][v][lane], fold[0][k][1][v][lane], R[v]);
+    buf = 1;
   }
 
-  int buf = 0;
   const uint64_t span = (uint64_t)W * kSteps, tiles = i1 > i0 ? (i1 - i0 + span - 1) / span : 0;
   for (uint64_t m = tiles; m-- > 0;) {
     const uint64_t i = i0 + m * span + (uint64_t)w * kSteps;
