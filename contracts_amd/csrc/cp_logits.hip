@@ -14,11 +14,12 @@ constexpr uint32_t kSeen = 0x80000000u;
 constexpr uint32_t kRowsMost = 512;  // short rows of a tile (their parameters lie in LDS too)
 
 struct Row {  // what a row is penalised with
-  float repetition, presence, frequency;
+  float repetition, inverse, presence, frequency;
 };
 __device__ __forceinline__ Row row_of(const ce_logits& s, uint64_t r) {
   Row o;
   o.repetition = s.repetition ? s.repetition[r] : (float)s.repetition_all;
+  o.inverse = 1.f / o.repetition;
   o.presence = s.presence ? s.presence[r] : (float)s.presence_all;
   o.frequency = s.frequency ? s.frequency[r] : (float)s.frequency_all;
   return o;
@@ -90,33 +91,52 @@ __device__ __forceinline__ void bias8(const ce_logits& s, uint64_t at, float (&o
   else if (s.bias_dtype == CE_BF16) load8((const bf16*)s.bias + at, o);
   else load8((const f16*)s.bias + at, o);
 }
+// One score under its table entry, without branches: 11 operations a score, and every lane of a wave runs them where one lane has an
+// entry, so a division (some 12 more) would cost as much as the reads: l / repetition is l times its reciprocal, half a step more off.
 __device__ __forceinline__ float penalise(float l, uint32_t entry, const Row& row) {
-  if (!entry) return l;
-  const uint32_t count = entry & ~kSeen;
-  const float z = l > 0.f ? l / row.repetition : l * row.repetition;
-  return count ? z - row.presence - row.frequency * (float)count : z;
+  const float count = (float)(entry & ~kSeen), scaled = l * (l > 0.f ? row.inverse : row.repetition), z = entry ? scaled : l;
+  return count > 0.f ? z - fma_(row.frequency, count, row.presence) : z;
+}
+// z where bit q says so, else -inf, in two operations
+__device__ __forceinline__ float only(float z, uint32_t ok, int q) {
+  const uint32_t keep = (uint32_t)((int32_t)(ok << (31 - q)) >> 31);
+  return __builtin_bit_cast(float, (__builtin_bit_cast(uint32_t, z) & keep) | (0xff800000u & ~keep));
 }
 
 // ---- a run of one row -----------------------------------------------------------------------------------------------------------
+// What does not wait for something else is read first (a block is a chain of reads: the fewer links, the better): scores, the first tokens of the
+// history whatever its length, the row's own numbers, biases; then the mask, whose place one of these names.
 template <class X, class O, class K> __global__ __launch_bounds__(kBlock) void k_logits_run(ce_logits s, uint64_t row0, uint32_t runs) {
+  constexpr int kGroups = kTile / kBlock / kLane;
+  typedef Pack<X, kLane> Eight;
   __shared__ __attribute__((aligned(16))) uint32_t table[kTile];
   const uint64_t r = row0 + blockIdx.x / runs;
   const uint32_t v0 = blockIdx.x % runs * kTile, V = (uint32_t)s.vocab, n = V - v0 < kTile ? V - v0 : kTile;
   const X* x = (const X*)s.logits + (int64_t)r * s.logits_row + v0;
   O* o = (O*)s.out + (int64_t)r * s.out_row + v0;
-  float l[kTile / kBlock / kLane][kLane];
+  Eight raw[kGroups];
 #pragma unroll
-  for (int g = 0; g < kTile / kBlock / kLane; ++g) {  // in flight while the history is counted
+  for (int g = 0; g < kGroups; ++g) {
     const uint32_t k = (g * kBlock + threadIdx.x) * kLane;
-    if (k + kLane <= n) load8(x + k, l[g]);
+    if (k + kLane <= n) __builtin_memcpy(&raw[g], __builtin_assume_aligned(x + k, alignof(X)), sizeof(Eight));
   }
-  const uint32_t used = used_of(s, r);
+  uint64_t tok = ~0ull;
+  if (threadIdx.x < (s.tokens ? s.history : 0)) tok = token<K>(s, r, threadIdx.x);
+  const uint32_t used = used_of(s, r), prompt = prompt_of(s, r);
+  const int64_t m = mask_row(s, r);
+  const Row row = row_of(s, r);
+  uint32_t ok[kGroups];
+#pragma unroll
+  for (int g = 0; g < kGroups; ++g) {
+    const uint32_t k = (g * kBlock + threadIdx.x) * kLane;
+    ok[g] = k + kLane <= n ? allowed8(s, m, v0 + k) : 0;
+  }
   if (used) {
-    const uint32_t prompt = prompt_of(s, r);
     for (uint32_t k = threadIdx.x; k < kTile / 4; k += kBlock) ((uint4*)table)[k] = uint4{0, 0, 0, 0};
     __syncthreads();
     for (uint32_t i = threadIdx.x; i < used; i += kBlock) {
-      const uint64_t t = token<K>(s, r, i) - v0;
+      const uint64_t t = tok - v0;
+      if (i + kBlock < used) tok = token<K>(s, r, i + kBlock);
       if (t < n) {
         if (i < prompt) atomicOr(&table[t], kSeen);
         else atomicAdd(&table[t], 1u);
@@ -124,30 +144,28 @@ template <class X, class O, class K> __global__ __launch_bounds__(kBlock) void k
     }
     __syncthreads();
   }
-  const Row row = row_of(s, r);
-  const int64_t m = mask_row(s, r);
   const uint64_t b = s.bias ? (s.bias_rows == 1 ? 0 : r % s.bias_rows) * s.vocab + v0 : 0;
 #pragma unroll
-  for (int g = 0; g < kTile / kBlock / kLane; ++g) {
+  for (int g = 0; g < kGroups; ++g) {
     const uint32_t k = (g * kBlock + threadIdx.x) * kLane;
     if (k + kLane <= n) {
+      float l[kLane], add[kLane];
+      if (s.bias) bias8(s, b + k, add);
+#pragma unroll
+      for (int q = 0; q < 8; ++q) l[q] = (float)raw[g].v[q];
       if (used) {
         const uint4 lo = ((const uint4*)table)[k / 4], hi = ((const uint4*)table)[k / 4 + 1];
         const uint32_t e[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
         if (lo.x | lo.y | lo.z | lo.w | hi.x | hi.y | hi.z | hi.w)
 #pragma unroll
-          for (int q = 0; q < 8; ++q) l[g][q] = penalise(l[g][q], e[q], row);
+          for (int q = 0; q < 8; ++q) l[q] = penalise(l[q], e[q], row);
       }
-      if (s.bias) {
-        float add[8];
-        bias8(s, b + k, add);
+      if (s.bias)
 #pragma unroll
-        for (int q = 0; q < 8; ++q) l[g][q] += add[q];
-      }
-      const uint32_t ok = allowed8(s, m, v0 + k);
+        for (int q = 0; q < 8; ++q) l[q] += add[q];
 #pragma unroll
-      for (int q = 0; q < 8; ++q) l[g][q] = (ok >> q) & 1 ? l[g][q] : -__builtin_inff();
-      store8(o + k, l[g]);
+      for (int q = 0; q < 8; ++q) l[q] = only(l[q], ok[g], q);
+      store8(o + k, l);
     } else {
       for (uint32_t j = k; j < n; ++j) {  // the row's last scores
         float z = (float)x[j];
@@ -333,35 +351,55 @@ template <class X, class D, class K> __global__ __launch_bounds__(kBlock) void k
       __syncthreads();
     }
     if (!active) continue;
-#pragma unroll 4
-    for (uint32_t q = 0; q < np; ++q) {
-      const uint64_t lr = (p + q) * w.at_once + sub;
-      if (lr >= w.long_rows) break;
-      const uint32_t seen = history ? ((const uint8_t*)marks)[q * kBlock + threadIdx.x] : 0u;
-      if (run && one_row) {
-        const uint64_t r = lr * w.B + b0;
-        float d[kLane];
-        load8((const D*)g.dout + (int64_t)r * g.dout_row + v0, d);
-        const uint32_t ok = allowed8(s, mask_row(s, r), v0);
+    if (one_row) {
+      constexpr int kAhead = 4;  // long rows read before the first is written (the compiler could not: for all it knows, dlogits is dout)
+      for (uint32_t q0 = 0; q0 < np; q0 += kAhead) {
+        float d[kAhead][kLane];
+        uint32_t ok[kAhead];
+        int64_t m[kAhead];
+        const uint64_t lr0 = (p + q0) * w.at_once + sub;
+        uint32_t there = np - q0 < kAhead ? np - q0 : kAhead;  // the last long rows may be fewer
+        while (there > 0 && lr0 + (uint64_t)(there - 1) * w.at_once >= w.long_rows) --there;
+        if (there == 0) break;
+        auto row = [&](int u) -> uint64_t { return (lr0 + (uint64_t)(u < (int)there ? u : there - 1) * w.at_once) * w.B + b0; };
 #pragma unroll
-        for (int j = 0; j < kLane; ++j) {
-          d[j] = (ok >> j) & 1 ? d[j] : 0.f;
-          sum[j] += d[j];
-        }
-        if (!g.dlogits) continue;
-        if (seen) {
-          const float rep = s.repetition ? s.repetition[r] : (float)s.repetition_all;
-          float l[kLane];
-          load8((const X*)s.logits + (int64_t)r * s.logits_row + v0, l);
+        for (int u = 0; u < kAhead; ++u) m[u] = mask_row(s, row(u));
 #pragma unroll
-          for (int j = 0; j < kLane; ++j)
-            if ((seen >> j) & 1) d[j] = l[j] > 0.f ? d[j] / rep : d[j] * rep;
-        }
-        store8((X*)g.dlogits + lr * w.width + c, d);
-      } else {
+        for (int u = 0; u < kAhead; ++u) load8((const D*)g.dout + (int64_t)row(u) * g.dout_row + v0, d[u]);
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) ok[u] = allowed8(s, m[u], v0);
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u)
+          if (u < (int)there) {
+#pragma unroll
+            for (int j = 0; j < kLane; ++j) {
+              d[u][j] = (ok[u] >> j) & 1 ? d[u][j] : 0.f;
+              sum[j] += d[u][j];
+            }
+            if (!g.dlogits) continue;
+            const uint32_t seen = history ? ((const uint8_t*)marks)[(q0 + u) * kBlock + threadIdx.x] : 0u;
+            if (seen) {
+              const float rep = s.repetition ? s.repetition[row(u)] : (float)s.repetition_all;
+              const float inverse = 1.f / rep;
+              float l[kLane];
+              load8((const X*)s.logits + (int64_t)row(u) * s.logits_row + v0, l);
+#pragma unroll
+              for (int j = 0; j < kLane; ++j) {
+                const float scaled = d[u][j] * (l[j] > 0.f ? inverse : rep);
+                d[u][j] = (seen >> j) & 1 ? scaled : d[u][j];
+              }
+            }
+            store8((X*)g.dlogits + row(u) * V + v0, d[u]);
+          }
+      }
+    } else {  // columns of two rows and more, or a long row's last ones
+      for (uint32_t q = 0; q < np; ++q) {
+        const uint64_t lr = (p + q) * w.at_once + sub;
+        if (lr >= w.long_rows) break;
         uint64_t r = lr * w.B + b0;
         uint32_t v = v0;
         int64_t m = mask_row(s, r);
+        const uint32_t seen = history ? ((const uint8_t*)marks)[q * kBlock + threadIdx.x] : 0u;
         float d[kLane];
         if (run) load8((const D*)g.dout + lr * w.width + c, d);
 #pragma unroll
@@ -372,7 +410,7 @@ template <class X, class D, class K> __global__ __launch_bounds__(kBlock) void k
           sum[j] += d[j];
           if ((seen >> j) & 1) {
             const float rep = s.repetition ? s.repetition[r] : (float)s.repetition_all;
-            d[j] = (float)((const X*)s.logits)[(int64_t)r * s.logits_row + v] > 0.f ? d[j] / rep : d[j] * rep;
+            d[j] *= (float)((const X*)s.logits)[(int64_t)r * s.logits_row + v] > 0.f ? 1.f / rep : rep;
           }
           if (!run && g.dlogits) ((X*)g.dlogits)[lr * w.width + c + j] = (X)d[j];
           if (++v == V && j + 1 < (int)cols) {
