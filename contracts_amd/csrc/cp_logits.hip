@@ -9,8 +9,8 @@
 
 namespace cp {
 
-constexpr int kBlock = 256, kTile = 4096, kLane = 8;
-constexpr uint32_t kSeen = 0x80000000u;
+constexpr int kBlock = 256, kTile = 4096, kLane = 8, kTableBytes = 16384;
+constexpr uint32_t kSeen = 0x80000000u;  // of a 32-bit table entry
 constexpr uint32_t kRowsMost = 512;  // short rows of a tile (their parameters lie in LDS too)
 
 struct Row {  // what a row is penalised with
@@ -36,10 +36,23 @@ __device__ __forceinline__ uint32_t prompt_of(const ce_logits& s, uint64_t r) {
   const int32_t l = s.prompt_lengths[r];
   return l > 0 ? (uint32_t)l : 0u;
 }
-// The token at place i of row r's history; a number past every vocabulary where it is no token.
-template <class K> __device__ __forceinline__ uint64_t token(const ce_logits& s, uint64_t r, uint32_t i) {
-  return (uint64_t)(int64_t)((const K*)s.tokens)[(int64_t)r * s.token_row + (int64_t)i * s.token_step];
+// kTokens places of a history at a time, all read before the first is looked at: i, i + stride, .. below end.
+constexpr int kTokens = 8;
+template <class K, class F> __device__ __forceinline__ void each_token(const ce_logits& s, uint64_t r, uint32_t from, uint32_t stride, uint32_t end, F&& f) {
+  const K* p = (const K*)s.tokens + (int64_t)r * s.token_row;
+  for (uint32_t i = from; i < end; i += kTokens * stride) {
+    K t[kTokens];
+#pragma unroll
+    for (int u = 0; u < kTokens; ++u) t[u] = i + u * stride < end ? p[(int64_t)(i + u * stride) * s.token_step] : K(0);
+#pragma unroll
+    for (int u = 0; u < kTokens; ++u)
+      if (i + u * stride < end) f(t[u], i + u * stride);
+  }
 }
+// Where token t lies in a run of n from v0 on; n or more where it does not.
+__device__ __forceinline__ uint32_t place(uint8_t t, uint32_t v0, uint32_t) { return (uint32_t)t - v0; }
+__device__ __forceinline__ uint32_t place(int32_t t, uint32_t v0, uint32_t) { return (uint32_t)t - v0; }
+__device__ __forceinline__ uint32_t place(int64_t t, uint32_t v0, uint32_t n) { return (uint64_t)t - v0 < n ? (uint32_t)((uint64_t)t - v0) : n; }
 // The mask's row of row r: -1 = everything is allowed, -2 = nothing is.
 __device__ __forceinline__ int64_t mask_row(const ce_logits& s, uint64_t r) {
   if (!s.mask) return -1;
@@ -93,8 +106,8 @@ __device__ __forceinline__ void bias8(const ce_logits& s, uint64_t at, float (&o
 }
 // One score under its table entry, without branches: 11 operations a score, and every lane of a wave runs them where one lane has an
 // entry, so a division (some 12 more) would cost as much as the reads: l / repetition is l times its reciprocal, half a step more off.
-__device__ __forceinline__ float penalise(float l, uint32_t entry, const Row& row) {
-  const float count = (float)(entry & ~kSeen), scaled = l * (l > 0.f ? row.inverse : row.repetition), z = entry ? scaled : l;
+__device__ __forceinline__ float penalise(float l, uint32_t entry, uint32_t times, const Row& row) {
+  const float count = (float)times, scaled = l * (l > 0.f ? row.inverse : row.repetition), z = entry ? scaled : l;
   return count > 0.f ? z - fma_(row.frequency, count, row.presence) : z;
 }
 // z where bit q says so, else -inf, in two operations
@@ -105,13 +118,15 @@ __device__ __forceinline__ float only(float z, uint32_t ok, int q) {
 
 // ---- a run of one row -----------------------------------------------------------------------------------------------------------
 // What does not wait for something else is read first (a block is a chain of reads: the fewer links, the better): scores, the first tokens of the
-// history whatever its length, the row's own numbers, biases; then the mask, whose place one of these names.
-template <class X, class O, class K> __global__ __launch_bounds__(kBlock) void k_logits_run(ce_logits s, uint64_t row0, uint32_t runs) {
-  constexpr int kGroups = kTile / kBlock / kLane;
+// history whatever its length, the row's own numbers; then the mask, whose place one of these names.
+// The table is 16 KB, 8 blocks a CU: 8192 entries of 16 bits (a history of at most 32767 tokens counts in 15), or 4096 of 32.
+template <class X, class O, class K, class E> __global__ __launch_bounds__(kBlock) void k_logits_run(ce_logits s, uint64_t row0, uint32_t runs) {
+  constexpr uint32_t kRun = kTableBytes / sizeof(E);
+  constexpr int kGroups = kRun / kBlock / kLane, kFirst = 4;
   typedef Pack<X, kLane> Eight;
-  __shared__ __attribute__((aligned(16))) uint32_t table[kTile];
+  __shared__ __attribute__((aligned(16))) uint32_t table[kTableBytes / 4];
   const uint64_t r = row0 + blockIdx.x / runs;
-  const uint32_t v0 = blockIdx.x % runs * kTile, V = (uint32_t)s.vocab, n = V - v0 < kTile ? V - v0 : kTile;
+  const uint32_t v0 = blockIdx.x % runs * kRun, V = (uint32_t)s.vocab, n = V - v0 < kRun ? V - v0 : kRun;
   const X* x = (const X*)s.logits + (int64_t)r * s.logits_row + v0;
   O* o = (O*)s.out + (int64_t)r * s.out_row + v0;
   Eight raw[kGroups];
@@ -120,8 +135,14 @@ template <class X, class O, class K> __global__ __launch_bounds__(kBlock) void k
     const uint32_t k = (g * kBlock + threadIdx.x) * kLane;
     if (k + kLane <= n) __builtin_memcpy(&raw[g], __builtin_assume_aligned(x + k, alignof(X)), sizeof(Eight));
   }
-  uint64_t tok = ~0ull;
-  if (threadIdx.x < (s.tokens ? s.history : 0)) tok = token<K>(s, r, threadIdx.x);
+  const uint32_t history = s.tokens ? (uint32_t)s.history : 0;
+  const K* tokens = (const K*)s.tokens + (int64_t)r * s.token_row;
+  K first[kFirst];
+#pragma unroll
+  for (int u = 0; u < kFirst; ++u) {
+    const uint32_t i = u * kBlock + threadIdx.x;
+    first[u] = i < history ? tokens[(int64_t)i * s.token_step] : K(0);
+  }
   const uint32_t used = used_of(s, r), prompt = prompt_of(s, r);
   const int64_t m = mask_row(s, r);
   const Row row = row_of(s, r);
@@ -132,18 +153,31 @@ template <class X, class O, class K> __global__ __launch_bounds__(kBlock) void k
     ok[g] = k + kLane <= n ? allowed8(s, m, v0 + k) : 0;
   }
   if (used) {
-    for (uint32_t k = threadIdx.x; k < kTile / 4; k += kBlock) ((uint4*)table)[k] = uint4{0, 0, 0, 0};
+    for (uint32_t k = threadIdx.x; k < kTableBytes / 16; k += kBlock) ((uint4*)table)[k] = uint4{0, 0, 0, 0};
     __syncthreads();
-    for (uint32_t i = threadIdx.x; i < used; i += kBlock) {
-      const uint64_t t = tok - v0;
-      if (i + kBlock < used) tok = token<K>(s, r, i + kBlock);
-      if (t < n) {
+    auto count = [&](K tok, uint32_t i) {
+      const uint32_t t = place(tok, v0, n);
+      if (t >= n) return;
+      if (sizeof(E) == 4) {
         if (i < prompt) atomicOr(&table[t], kSeen);
         else atomicAdd(&table[t], 1u);
+      } else {
+        if (i < prompt) atomicOr(&table[t / 2], 0x8000u << (t % 2 * 16));
+        else atomicAdd(&table[t / 2], 1u << (t % 2 * 16));
       }
-    }
+    };
+#pragma unroll
+    for (int u = 0; u < kFirst; ++u)
+      if (u * kBlock + threadIdx.x < used) count(first[u], u * kBlock + threadIdx.x);
+    each_token<K>(s, r, kFirst * kBlock + threadIdx.x, kBlock, used, count);
     __syncthreads();
   }
+  // an entry in its 32-bit form
+  auto entry = [&](uint32_t k) -> uint32_t {
+    if (sizeof(E) == 4) return table[k];
+    const uint32_t e = ((const uint16_t*)table)[k];
+    return (e & 0x7fffu) | (e & 0x8000u ? kSeen : 0u);
+  };
   const uint64_t b = s.bias ? (s.bias_rows == 1 ? 0 : r % s.bias_rows) * s.vocab + v0 : 0;
 #pragma unroll
   for (int g = 0; g < kGroups; ++g) {
@@ -154,11 +188,23 @@ template <class X, class O, class K> __global__ __launch_bounds__(kBlock) void k
 #pragma unroll
       for (int q = 0; q < 8; ++q) l[q] = (float)raw[g].v[q];
       if (used) {
-        const uint4 lo = ((const uint4*)table)[k / 4], hi = ((const uint4*)table)[k / 4 + 1];
-        const uint32_t e[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
-        if (lo.x | lo.y | lo.z | lo.w | hi.x | hi.y | hi.z | hi.w)
+        uint4 w[sizeof(E) / 2];
 #pragma unroll
-          for (int q = 0; q < 8; ++q) l[q] = penalise(l[q], e[q], row);
+        for (uint32_t j = 0; j < sizeof(E) / 2; ++j) w[j] = ((const uint4*)table)[k * sizeof(E) / 16 + j];
+        uint32_t any = w[0].x | w[0].y | w[0].z | w[0].w;
+        if (sizeof(E) == 4) any |= w[sizeof(E) / 2 - 1].x | w[sizeof(E) / 2 - 1].y | w[sizeof(E) / 2 - 1].z | w[sizeof(E) / 2 - 1].w;
+        if (any) {
+          const uint32_t* e = (const uint32_t*)w;
+#pragma unroll
+          for (int q = 0; q < 8; ++q) {
+            if (sizeof(E) == 4) {
+              l[q] = penalise(l[q], e[q], e[q] & ~kSeen, row);
+            } else {
+              const uint32_t half = q % 2 ? e[q / 2] >> 16 : e[q / 2] & 0xffffu;
+              l[q] = penalise(l[q], half, half & 0x7fffu, row);
+            }
+          }
+        }
       }
       if (s.bias)
 #pragma unroll
@@ -169,7 +215,7 @@ template <class X, class O, class K> __global__ __launch_bounds__(kBlock) void k
     } else {
       for (uint32_t j = k; j < n; ++j) {  // the row's last scores
         float z = (float)x[j];
-        if (used) z = penalise(z, table[j], row);
+        if (used) z = penalise(z, entry(j), entry(j) & ~kSeen, row);
         if (s.bias) z += bias_at(s, b + j);
         o[j] = (O)(allowed(s, m, v0 + j) ? z : -__builtin_inff());
       }
@@ -195,24 +241,22 @@ template <class X, class O, class K> __global__ __launch_bounds__(kBlock) void k
   if (s.tokens) {
     for (uint32_t k = threadIdx.x; k < (n + 3) / 4; k += kBlock) ((uint4*)table)[k] = uint4{0, 0, 0, 0};
     __syncthreads();
-    auto count = [&](uint32_t j, uint32_t i) {
-      const uint64_t t = token<K>(s, r0 + j, i);
-      if (t < V) {
+    auto count = [&](uint32_t j, uint32_t from, uint32_t stride) {
+      each_token<K>(s, r0 + j, from, stride, used[j], [&](K tok, uint32_t i) {
+        const uint32_t t = place(tok, 0, V);
+        if (t >= V) return;
         if (i < prompt[j]) atomicOr(&table[j * V + t], kSeen);
         else atomicAdd(&table[j * V + t], 1u);
-      }
+      });
     };
     if (s.token_row < s.token_step) {  // planes of actions: the same step of neighbouring rows lies together
-      const uint32_t j = threadIdx.x & (G - 1);
       if (G >= kBlock) {
-        for (uint32_t k = threadIdx.x; k < have; k += kBlock)
-          for (uint32_t i = 0; i < used[k]; ++i) count(k, i);
-      } else if (j < have) {
-        for (uint32_t i = threadIdx.x >> shift; i < used[j]; i += kBlock >> shift) count(j, i);
+        for (uint32_t j = threadIdx.x; j < have; j += kBlock) count(j, 0, 1);
+      } else if ((threadIdx.x & (G - 1)) < have) {
+        count(threadIdx.x & (G - 1), threadIdx.x >> shift, kBlock >> shift);
       }
     } else {  // histories row by row: 16 lanes to a row
-      for (uint32_t j = threadIdx.x / 16; j < have; j += kBlock / 16)
-        for (uint32_t i = threadIdx.x % 16; i < used[j]; i += 16) count(j, i);
+      for (uint32_t j = threadIdx.x / 16; j < have; j += kBlock / 16) count(j, threadIdx.x % 16, 16);
     }
   }
   __syncthreads();
@@ -229,7 +273,7 @@ template <class X, class O, class K> __global__ __launch_bounds__(kBlock) void k
     for (int q = 0; q < 8; ++q) {
       if (k + q < n) {
         if (!(dense && whole)) l[q] = (float)x[(int64_t)jj * s.logits_row + vv];
-        if (s.tokens) l[q] = penalise(l[q], table[k + q], rows[jj]);
+        if (s.tokens) l[q] = penalise(l[q], table[k + q], table[k + q] & ~kSeen, rows[jj]);
         if (s.bias) l[q] += bias_at(s, (B == 1 ? 0 : (uint64_t)((uint32_t)(r0 + jj) % B) * V) + vv);
         if (!allowed(s, masks[jj], vv)) l[q] = -__builtin_inff();
         if (!(dense && whole)) o[(int64_t)jj * s.out_row + vv] = (O)l[q];
@@ -243,10 +287,15 @@ template <class X, class O, class K> __global__ __launch_bounds__(kBlock) void k
 template <class X, class O, class K> static void shapes(const ce_logits& s, hipStream_t st) {
   // Half a tile and longer a row is worth blocks of its own; below, a block takes as many rows as fit.
   if (s.vocab > kTile / 2) {
-    const uint32_t runs = (uint32_t)((s.vocab + kTile - 1) / kTile);
+    // 16-bit entries count a longer run (X us against Y at 256 x 131072 bfloat16), 32-bit ones long histories and few rows, where blocks are short
+    const bool half = s.history < 32768 && s.rows * ((s.vocab + 8191) / 8192) >= 512;
+    const uint32_t run = half ? kTableBytes / 2 : kTableBytes / 4, runs = (uint32_t)((s.vocab + run - 1) / run);
     const uint64_t most = (1u << 23) / runs;  // rows of a launch: fewer than 2^32 threads
-    for (uint64_t r = 0; r < s.rows; r += most)
-      k_logits_run<X, O, K><<<(uint32_t)(s.rows - r < most ? s.rows - r : most) * runs, kBlock, 0, st>>>(s, r, runs);
+    for (uint64_t r = 0; r < s.rows; r += most) {
+      const uint32_t blocks = (uint32_t)(s.rows - r < most ? s.rows - r : most) * runs;
+      if (half) k_logits_run<X, O, K, uint16_t><<<blocks, kBlock, 0, st>>>(s, r, runs);
+      else k_logits_run<X, O, K, uint32_t><<<blocks, kBlock, 0, st>>>(s, r, runs);
+    }
     return;
   }
   uint32_t shift = 0;
@@ -330,14 +379,14 @@ template <class X, class D, class K> __global__ __launch_bounds__(kBlock) void k
         const uint32_t lr = k / touched, b = k - lr * touched;
         const uint64_t r = (first + lr) * w.B + b_lo + b;
         const uint32_t used = used_of(s, r), byte0 = (lr / w.at_once) * kBlock + (lr % w.at_once) * w.lanes;
-        for (uint32_t i = from; i < used; i += stride) {
-          const uint64_t tok = token<K>(s, r, i);
-          if (tok >= V) continue;
-          const uint64_t at = (b_lo + b) * V + tok - c0;  // wraps where it lies ahead of the run
-          if (at >= kCols || at >= w.width - c0) continue;
+        each_token<K>(s, r, from, stride, used, [&](K tok, uint32_t) {
+          const uint32_t t = place(tok, 0, V);
+          if (t >= V) return;
+          const uint64_t at = (b_lo + b) * V + t - c0;  // wraps where it lies ahead of the run
+          if (at >= kCols || at >= w.width - c0) return;
           const uint32_t byte = byte0 + (uint32_t)at / kLane;
           atomicOr(&marks[byte / 4], 1u << (byte % 4 * 8 + (uint32_t)at % kLane));
-        }
+        });
       };
       if (s.token_row < s.token_step) {  // neighbouring rows' tokens of a step lie together: neighbouring lanes take them
         if (n >= kBlock) {
