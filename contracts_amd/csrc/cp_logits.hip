@@ -54,19 +54,19 @@ __device__ __forceinline__ uint32_t place(uint8_t t, uint32_t v0, uint32_t) { re
 __device__ __forceinline__ uint32_t place(int32_t t, uint32_t v0, uint32_t) { return (uint32_t)t - v0; }
 __device__ __forceinline__ uint32_t place(int64_t t, uint32_t v0, uint32_t n) { return (uint64_t)t - v0 < n ? (uint32_t)((uint64_t)t - v0) : n; }
 // The mask's row of row r: -1 = everything is allowed, -2 = nothing is.
-__device__ __forceinline__ int64_t mask_row(const ce_logits& s, uint64_t r) {
+__device__ __forceinline__ int32_t mask_row(const ce_logits& s, uint64_t r) {
   if (!s.mask) return -1;
-  if (!s.mask_index) return s.mask_rows == s.rows ? (int64_t)r : (int64_t)((uint32_t)r % (uint32_t)s.mask_rows);
+  if (!s.mask_index) return s.mask_rows == s.rows ? (int32_t)r : (int32_t)((uint32_t)r % (uint32_t)s.mask_rows);
   const int32_t m = s.mask_index[r];
   return m < 0 ? -1 : (uint64_t)m < s.mask_rows ? m : -2;
 }
-__device__ __forceinline__ bool allowed(const ce_logits& s, int64_t m, uint32_t v) {
+__device__ __forceinline__ bool allowed(const ce_logits& s, int32_t m, uint32_t v) {
   if (m < 0) return m == -1;
   if (s.mask_dtype == CE_U8) return ((const uint8_t*)s.mask)[(uint64_t)m * s.vocab + v] != 0;
   return (((const uint32_t*)s.mask)[(uint64_t)m * ((s.vocab + 31) / 32) + v / 32] >> (v % 32)) & 1u;
 }
 // 8 neighbouring tokens' permissions as bits; all 8 lie inside the row.
-__device__ __forceinline__ uint32_t allowed8(const ce_logits& s, int64_t m, uint32_t v) {
+__device__ __forceinline__ uint32_t allowed8(const ce_logits& s, int32_t m, uint32_t v) {
   if (m < 0) return m == -1 ? 0xffu : 0u;
   if (s.mask_dtype == CE_U8) {
     uint64_t b;
@@ -144,7 +144,7 @@ template <class X, class O, class K, class E> __global__ __launch_bounds__(kBloc
     first[u] = i < history ? tokens[(int64_t)i * s.token_step] : K(0);
   }
   const uint32_t used = used_of(s, r), prompt = prompt_of(s, r);
-  const int64_t m = mask_row(s, r);
+  const int32_t m = mask_row(s, r);
   const Row row = row_of(s, r);
   uint32_t ok[kGroups];
 #pragma unroll
@@ -229,7 +229,7 @@ template <class X, class O, class K> __global__ __launch_bounds__(kBlock) void k
   __shared__ __attribute__((aligned(16))) uint32_t table[kTile];
   __shared__ Row rows[kRowsMost];
   __shared__ uint32_t used[kRowsMost], prompt[kRowsMost];
-  __shared__ int64_t masks[kRowsMost];
+  __shared__ int32_t masks[kRowsMost];
   const uint64_t r0 = (uint64_t)blockIdx.x * G;
   const uint32_t V = (uint32_t)s.vocab, have = s.rows - r0 < G ? (uint32_t)(s.rows - r0) : G, n = have * V;
   for (uint32_t j = threadIdx.x; j < have; j += kBlock) {
@@ -325,9 +325,12 @@ hipError_t launch_logits(const ce_logits& s, hipStream_t st) {
 // ---- gradients ------------------------------------------------------------------------------------------------------------------
 // Where a bias wants a gradient, the B rows that its table covers in turn are one long row of B V columns, so that a lane keeps its 8
 // columns while it walks down the R / B long rows and sums them in float; otherwise a long row is a row.  A block takes a run of
-// 2048 columns, or as many whole long rows at a time as fill its lanes; it marks the tokens seen by kPasses of its steps in LDS
-// (one bit a score) ahead of walking them.  The long rows are cut into parts; a second launch adds their sums in a fixed order.
-constexpr int kPasses = 16, kCols = kBlock * kLane;
+// 2048 columns, or as many whole long rows at a time as fill its lanes.  The long rows are cut into parts; a second launch adds
+// their sums in a fixed order.
+// The few scores that a repetition penalty scaled are put right behind that, one lane to a token of a history: a token that occurs twice
+// is written twice, with the same value.  (Marking them in LDS ahead of the walk, as the forward pass does, took 117 us where this
+// takes X, at 2048 x 32000 bfloat16 with histories of up to 512.)
+constexpr int kCols = kBlock * kLane;
 
 struct GradShape {
   uint64_t B, width, long_rows;  // rows of a long row, its columns, how many there are
@@ -349,125 +352,59 @@ static GradShape grad_shape(const ce_logits& s, const ce_logits_grad& g) {
   return o;
 }
 
-template <class X, class D, class K> __global__ __launch_bounds__(kBlock) void k_logits_grad(ce_logits s, ce_logits_grad g, GradShape w, uint64_t block0) {
-  __shared__ uint32_t marks[kPasses * kBlock / 4];  // a byte for a lane's 8 columns of a pass
+template <class X, class D> __global__ __launch_bounds__(kBlock, 4) void k_logits_grad(ce_logits s, ce_logits_grad g, GradShape w, uint64_t block0) {
   __shared__ float sums[kBlock][kLane + 1];
   const uint64_t block = block0 + blockIdx.x, chunk = block % w.chunks, part = block / w.chunks;
   const uint32_t V = (uint32_t)s.vocab, sub = threadIdx.x / w.lanes, t = threadIdx.x - sub * w.lanes;
-  const uint64_t c0 = chunk * kCols, c = c0 + (uint64_t)t * kLane;
-  const bool active = sub < w.at_once && c < w.width;
-  const uint32_t cols = active ? (uint32_t)(w.width - c < kLane ? w.width - c : kLane) : 0;
+  const uint64_t c = chunk * kCols + (uint64_t)t * kLane;
+  const uint32_t cols = sub < w.at_once && c < w.width ? (uint32_t)(w.width - c < kLane ? w.width - c : kLane) : 0;  // 0: nothing to do
   const uint64_t b0 = c / V;
   const uint32_t v0 = (uint32_t)(c - b0 * V);
-  const bool one_row = cols == kLane && v0 + kLane <= V, run = one_row || (cols == kLane && g.dout_row == (int64_t)V);
   const uint64_t passes = (w.long_rows + w.at_once - 1) / w.at_once;
-  const uint64_t p0 = passes * part / w.parts, p1 = passes * (part + 1) / w.parts;
-  // the rows of a long row that this run of columns touches
-  const uint64_t last = (c0 + kCols < w.width ? c0 + kCols : w.width) - 1, b_lo = c0 / V;
-  const uint32_t touched = (uint32_t)(last / V - b_lo) + 1;
-  const bool history = s.tokens && g.dlogits && (s.repetition || s.repetition_all != 1.0);
+  const uint64_t lr0 = passes * part / w.parts * w.at_once + sub, end = passes * (part + 1) / w.parts * w.at_once, lr1 = end < w.long_rows ? end : w.long_rows;
   float sum[kLane] = {0, 0, 0, 0, 0, 0, 0, 0};
-  for (uint64_t p = p0; p < p1; p += kPasses) {
-    const uint32_t np = p1 - p < kPasses ? (uint32_t)(p1 - p) : kPasses;
-    if (history) {
-      __syncthreads();
-      for (uint32_t k = threadIdx.x; k < np * kBlock / 4; k += kBlock) marks[k] = 0;
-      __syncthreads();
-      const uint64_t first = p * w.at_once, end = first + (uint64_t)np * w.at_once < w.long_rows ? first + (uint64_t)np * w.at_once : w.long_rows;
-      const uint32_t n = (uint32_t)(end - first) * touched;  // rows whose histories matter
-      auto mark = [&](uint32_t k, uint32_t from, uint32_t stride) {
-        const uint32_t lr = k / touched, b = k - lr * touched;
-        const uint64_t r = (first + lr) * w.B + b_lo + b;
-        const uint32_t used = used_of(s, r), byte0 = (lr / w.at_once) * kBlock + (lr % w.at_once) * w.lanes;
-        each_token<K>(s, r, from, stride, used, [&](K tok, uint32_t) {
-          const uint32_t t = place(tok, 0, V);
-          if (t >= V) return;
-          const uint64_t at = (b_lo + b) * V + t - c0;  // wraps where it lies ahead of the run
-          if (at >= kCols || at >= w.width - c0) return;
-          const uint32_t byte = byte0 + (uint32_t)at / kLane;
-          atomicOr(&marks[byte / 4], 1u << (byte % 4 * 8 + (uint32_t)at % kLane));
-        });
-      };
-      if (s.token_row < s.token_step) {  // neighbouring rows' tokens of a step lie together: neighbouring lanes take them
-        if (n >= kBlock) {
-          for (uint32_t k = threadIdx.x; k < n; k += kBlock) mark(k, 0, 1);
-        } else if (threadIdx.x / n < kBlock / n) {
-          mark(threadIdx.x % n, threadIdx.x / n, kBlock / n);
+  if (cols == kLane && v0 + kLane <= V) {  // 8 columns of one row
+    constexpr int kAhead = 8;  // long rows read before the first is written (the compiler could not: for all it knows, dlogits is dout)
+    for (uint64_t lr = lr0; lr < lr1; lr += kAhead * w.at_once) {
+      Pack<D, kLane> raw[kAhead];
+      uint32_t ok[kAhead];
+      int32_t m[kAhead];
+      const uint32_t there = (uint32_t)((lr1 - lr + w.at_once - 1) / w.at_once);  // may be fewer: those past the end read the last one
+      auto row = [&](uint32_t u) -> uint64_t { return (lr + (uint64_t)(u < there ? u : there - 1) * w.at_once) * w.B + b0; };
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) m[u] = mask_row(s, row(u));
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u)
+        __builtin_memcpy(&raw[u], __builtin_assume_aligned((const D*)g.dout + (int64_t)row(u) * g.dout_row + v0, alignof(D)), sizeof(raw[u]));
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) ok[u] = allowed8(s, m[u], v0);
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u)
+        if (u < (int)there) {
+          float d[kLane];
+#pragma unroll
+          for (int j = 0; j < kLane; ++j) {
+            d[j] = (ok[u] >> j) & 1 ? (float)raw[u].v[j] : 0.f;
+            sum[j] += d[j];
+          }
+          if (g.dlogits) store8((X*)g.dlogits + row(u) * V + v0, d);
         }
-      } else {  // 16 lanes to a row
-        for (uint32_t k = threadIdx.x / 16; k < n; k += kBlock / 16) mark(k, threadIdx.x % 16, 16);
-      }
-      __syncthreads();
     }
-    if (!active) continue;
-    if (one_row) {
-      constexpr int kAhead = 4;  // long rows read before the first is written (the compiler could not: for all it knows, dlogits is dout)
-      for (uint32_t q0 = 0; q0 < np; q0 += kAhead) {
-        float d[kAhead][kLane];
-        uint32_t ok[kAhead];
-        int64_t m[kAhead];
-        const uint64_t lr0 = (p + q0) * w.at_once + sub;
-        uint32_t there = np - q0 < kAhead ? np - q0 : kAhead;  // the last long rows may be fewer
-        while (there > 0 && lr0 + (uint64_t)(there - 1) * w.at_once >= w.long_rows) --there;
-        if (there == 0) break;
-        auto row = [&](int u) -> uint64_t { return (lr0 + (uint64_t)(u < (int)there ? u : there - 1) * w.at_once) * w.B + b0; };
+  } else if (cols) {  // columns of two rows and more, or a long row's last ones
+    for (uint64_t lr = lr0; lr < lr1; lr += w.at_once) {
+      uint64_t r = lr * w.B + b0;
+      uint32_t v = v0;
+      int32_t m = mask_row(s, r);
 #pragma unroll
-        for (int u = 0; u < kAhead; ++u) m[u] = mask_row(s, row(u));
-#pragma unroll
-        for (int u = 0; u < kAhead; ++u) load8((const D*)g.dout + (int64_t)row(u) * g.dout_row + v0, d[u]);
-#pragma unroll
-        for (int u = 0; u < kAhead; ++u) ok[u] = allowed8(s, m[u], v0);
-#pragma unroll
-        for (int u = 0; u < kAhead; ++u)
-          if (u < (int)there) {
-#pragma unroll
-            for (int j = 0; j < kLane; ++j) {
-              d[u][j] = (ok[u] >> j) & 1 ? d[u][j] : 0.f;
-              sum[j] += d[u][j];
-            }
-            if (!g.dlogits) continue;
-            const uint32_t seen = history ? ((const uint8_t*)marks)[(q0 + u) * kBlock + threadIdx.x] : 0u;
-            if (seen) {
-              const float rep = s.repetition ? s.repetition[row(u)] : (float)s.repetition_all;
-              const float inverse = 1.f / rep;
-              float l[kLane];
-              load8((const X*)s.logits + (int64_t)row(u) * s.logits_row + v0, l);
-#pragma unroll
-              for (int j = 0; j < kLane; ++j) {
-                const float scaled = d[u][j] * (l[j] > 0.f ? inverse : rep);
-                d[u][j] = (seen >> j) & 1 ? scaled : d[u][j];
-              }
-            }
-            store8((X*)g.dlogits + row(u) * V + v0, d[u]);
-          }
-      }
-    } else {  // columns of two rows and more, or a long row's last ones
-      for (uint32_t q = 0; q < np; ++q) {
-        const uint64_t lr = (p + q) * w.at_once + sub;
-        if (lr >= w.long_rows) break;
-        uint64_t r = lr * w.B + b0;
-        uint32_t v = v0;
-        int64_t m = mask_row(s, r);
-        const uint32_t seen = history ? ((const uint8_t*)marks)[q * kBlock + threadIdx.x] : 0u;
-        float d[kLane];
-        if (run) load8((const D*)g.dout + lr * w.width + c, d);
-#pragma unroll
-        for (int j = 0; j < kLane; ++j) {
-          if (j >= (int)cols) continue;
-          if (!run) d[j] = (float)((const D*)g.dout)[(int64_t)r * g.dout_row + v];
-          if (!allowed(s, m, v)) d[j] = 0.f;
-          sum[j] += d[j];
-          if ((seen >> j) & 1) {
-            const float rep = s.repetition ? s.repetition[r] : (float)s.repetition_all;
-            d[j] *= (float)((const X*)s.logits)[(int64_t)r * s.logits_row + v] > 0.f ? 1.f / rep : rep;
-          }
-          if (!run && g.dlogits) ((X*)g.dlogits)[lr * w.width + c + j] = (X)d[j];
-          if (++v == V && j + 1 < (int)cols) {
-            v = 0;
-            m = mask_row(s, ++r);
-          }
+      for (int j = 0; j < kLane; ++j) {
+        if (j >= (int)cols) continue;
+        const float d = allowed(s, m, v) ? (float)((const D*)g.dout)[(int64_t)r * g.dout_row + v] : 0.f;
+        sum[j] += d;
+        if (g.dlogits) ((X*)g.dlogits)[lr * w.width + c + j] = (X)d;
+        if (++v == V && j + 1 < (int)cols) {
+          v = 0;
+          m = mask_row(s, ++r);
         }
-        if (run && g.dlogits) store8((X*)g.dlogits + lr * w.width + c, d);
       }
     }
   }
@@ -484,6 +421,47 @@ template <class X, class D, class K> __global__ __launch_bounds__(kBlock) void k
   }
   for (uint32_t j = 0; j < kLane; ++j)
     if (j < cols) ((float*)s.workspace)[part * w.width + c + j] = sum[j];
+}
+
+// The scores that a repetition penalty scaled.  kTokensBlock places of the histories to a block, neighbouring lanes where tokens lie together.
+constexpr uint32_t kTokensBlock = kBlock * 4;
+template <class X, class D, class K> __global__ __launch_bounds__(kBlock) void k_logits_repeats(ce_logits s, ce_logits_grad g, uint64_t block0) {
+  const bool planes = s.token_row < s.token_step;
+  const uint64_t inner = planes ? s.rows : s.history, outer = planes ? s.history : s.rows, n = inner * outer;
+  const uint64_t first = (block0 + blockIdx.x) * kTokensBlock, o0 = first / inner;
+  const uint32_t i0 = (uint32_t)(first - o0 * inner);
+  // what depends on nothing, then what depends on that, for all four places at once; places that do not count read another's
+  const uint32_t V = (uint32_t)s.vocab;
+  uint64_t r[4];
+  uint32_t t[4], ok[4];
+  int32_t m[4];
+  float rep[4], d[4], l[4];
+  bool good[4];
+#pragma unroll
+  for (int u = 0; u < 4; ++u) {
+    const uint32_t k = u * kBlock + threadIdx.x;
+    good[u] = first + k < n;
+    const uint32_t at = good[u] ? i0 + k : i0, over = at / (uint32_t)inner, in = at - over * (uint32_t)inner;
+    r[u] = planes ? in : o0 + over;
+    const uint32_t i = planes ? (uint32_t)o0 + over : in;
+    good[u] = good[u] && i < used_of(s, r[u]);
+    t[u] = place(((const K*)s.tokens)[(int64_t)r[u] * s.token_row + (int64_t)i * s.token_step], 0, V);
+    m[u] = mask_row(s, r[u]);
+    rep[u] = s.repetition ? s.repetition[r[u]] : (float)s.repetition_all;
+  }
+#pragma unroll
+  for (int u = 0; u < 4; ++u) {
+    good[u] = good[u] && t[u] < V;
+    ok[u] = d[u] = l[u] = 0;
+    if (good[u]) {
+      ok[u] = allowed(s, m[u], t[u]);
+      d[u] = (float)((const D*)g.dout)[(int64_t)r[u] * g.dout_row + t[u]];
+      l[u] = (float)((const X*)s.logits)[(int64_t)r[u] * s.logits_row + t[u]];
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < 4; ++u)
+    if (ok[u]) ((X*)g.dlogits)[r[u] * V + t[u]] = (X)(l[u] > 0.f ? d[u] / rep[u] : d[u] * rep[u]);
 }
 
 // 64 columns to a block, each 4th part to a wave, the waves' sums in their order
@@ -507,19 +485,23 @@ uint64_t logits_grad_workspace(const ce_logits& s, const ce_logits_grad& g) {
 
 constexpr uint64_t kBlocksMost = 1u << 23;  // of a launch: fewer than 2^32 threads
 
-template <class X, class D, class K> static void grad_go(const ce_logits& s, const ce_logits_grad& g, const GradShape& w, hipStream_t st) {
+template <class X, class D, class K> static void repeats_go(const ce_logits& s, const ce_logits_grad& g, hipStream_t st) {
+  const uint64_t blocks = (s.rows * s.history + kTokensBlock - 1) / kTokensBlock;
+  for (uint64_t b = 0; b < blocks; b += kBlocksMost)
+    k_logits_repeats<X, D, K><<<(uint32_t)(blocks - b < kBlocksMost ? blocks - b : kBlocksMost), kBlock, 0, st>>>(s, g, b);
+}
+template <class X, class D> static void grad_go(const ce_logits& s, const ce_logits_grad& g, const GradShape& w, hipStream_t st) {
   const uint64_t blocks = w.chunks * w.parts;
   for (uint64_t b = 0; b < blocks; b += kBlocksMost)
-    k_logits_grad<X, D, K><<<(uint32_t)(blocks - b < kBlocksMost ? blocks - b : kBlocksMost), kBlock, 0, st>>>(s, g, w, b);
-}
-template <class X, class D> static void grad_tokens(const ce_logits& s, const ce_logits_grad& g, const GradShape& w, hipStream_t st) {
-  if (s.tokens && s.token_dtype == CE_I32) grad_go<X, D, int32_t>(s, g, w, st);
-  else if (s.tokens && s.token_dtype == CE_I64) grad_go<X, D, int64_t>(s, g, w, st);
-  else grad_go<X, D, uint8_t>(s, g, w, st);
+    k_logits_grad<X, D><<<(uint32_t)(blocks - b < kBlocksMost ? blocks - b : kBlocksMost), kBlock, 0, st>>>(s, g, w, b);
+  if (!s.tokens || !s.history || !g.dlogits || (!s.repetition && s.repetition_all == 1.0)) return;
+  if (s.token_dtype == CE_I32) repeats_go<X, D, int32_t>(s, g, st);
+  else if (s.token_dtype == CE_I64) repeats_go<X, D, int64_t>(s, g, st);
+  else repeats_go<X, D, uint8_t>(s, g, st);
 }
 template <class X> static void grad_outs(const ce_logits& s, const ce_logits_grad& g, const GradShape& w, hipStream_t st) {
-  if (s.out_dtype == s.dtype) grad_tokens<X, X>(s, g, w, st);
-  else grad_tokens<X, float>(s, g, w, st);
+  if (s.out_dtype == s.dtype) grad_go<X, X>(s, g, w, st);
+  else grad_go<X, float>(s, g, w, st);
 }
 template <class T> static void bias_go(const ce_logits& s, const ce_logits_grad& g, const GradShape& w, hipStream_t st) {
   const uint64_t blocks = (w.width + kWave - 1) / kWave;
