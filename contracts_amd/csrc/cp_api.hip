@@ -89,15 +89,19 @@ int check_scan(const ce_scan* s) {
 //    waves where 2048 can be had: 75 against 82.
 //  * under 1536 waves that way, the time axis is cut into chunks too, which costs reading x and the gate twice, at least a tile each and
 //    4096 waves in all: [65537, 1, 1024] bfloat16, 16 heads: 78 with 128 chunks and 4 channels a lane, 168 with 16 chunks and 1 channel;
-//    [1000, 37, 360] float keeps whole at 1672 waves: 31 against 36.  Gradients: [2000, 8, 2048] bfloat16 92 with 4 waves and 8 chunks, 97 whole.
-void share(cp::ScanParams& p, int* vec, bool grad, uint64_t columns, uint64_t (*blocks)(const cp::ScanParams&, uint64_t columns, int vec)) {
+//    [1000, 37, 360] float keeps whole at 1672 waves: 31 against 36.  Gradients: [1000, 37, 360] float, 9 heads: 54 with 8 chunks of pairs of
+//    channels, 60 whole with one; [1000, 64, 256] float 71 whole with one (2048 waves), 81 in chunks.
+void share(cp::ScanParams& p, int* vec, bool grad, bool halves, uint64_t columns, uint64_t (*blocks)(const cp::ScanParams&, uint64_t columns, int vec)) {
   p.chunks = p.waves = 1;
   if (p.T <= CE_SCAN_SAVED_STEPS) return;
   const int widest = *vec;
   if (blocks(p, columns, widest) >= 2048) return;
   p.waves = p.T <= 4 * CE_SCAN_SAVED_STEPS || (grad && blocks(p, columns, widest) * 4 >= 2048) ? 4 : 8;
-  const uint64_t enough = grad ? 1536 : 4096;
-  while (*vec > 1 && !grad && blocks(p, columns, *vec) * p.waves < enough) *vec /= 2;
+  if (grad) {
+    if (!halves && *vec > 1 && blocks(p, columns, *vec) * p.waves < 1536 && columns / 64 * p.waves >= 2048) *vec = 1;
+  } else {
+    while (*vec > 1 && blocks(p, columns, *vec) * p.waves < 4096) *vec /= 2;
+  }
   if (blocks(p, columns, *vec) * p.waves >= 1536 || p.T < CE_SCAN_SPLIT_STEPS) return;
   *vec = widest;
   if (grad) p.waves = 4;
@@ -129,12 +133,12 @@ void plan_scan(const ce_scan* s, const ce_scan_grad* g, Plan* o) {
     return ok && aligned(g->dy, v * b) && aligned(g->dx, v * b) && (o->mode != cp::kGateChannel || aligned(g->dgate, v * gb));
   };
   int vec = b == 8 ? 1 : (int)(8 / b);
-  if (g) vec = b == 2 ? 2 : 1;
+  if (g) vec = std::min(vec, 2);
   while (vec > 1 && !fits(vec)) vec /= 2;
   p.T = T;
   p.head = (uint32_t)head;
   const bool sums = g && o->mode == cp::kGateHead;
-  share(p, &vec, g != nullptr, E * C, sums ? head_waves : flat_waves);
+  share(p, &vec, g != nullptr, b == 2, E * C, sums ? head_waves : flat_waves);
   o->vec = vec;
   const bool rev = s->flags & CE_SCAN_REVERSE;
   const int64_t sign = rev ? -1 : 1, off = rev && T ? (int64_t)T - 1 : 0;

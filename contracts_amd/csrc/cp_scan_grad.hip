@@ -327,7 +327,7 @@ template <class X, class G, int MODE, int VEC> static hipError_t go(const ScanPa
 }
 
 template <class X, class G, int MODE> static hipError_t vecs(const ScanParams& p, int vec, hipStream_t s) {
-  if (sizeof(X) == 2 && vec == 2) return go<X, G, MODE, sizeof(X) == 2 ? 2 : 1>(p, s);
+  if (vec == 2) return go<X, G, MODE, 2>(p, s);
   return go<X, G, MODE, 1>(p, s);
 }
 template <class X, class G> static hipError_t modes(const ScanParams& p, int mode, int vec, hipStream_t s) {
