@@ -9,7 +9,7 @@
 
 namespace cp {
 
-constexpr int kBlock = 256, kTile = 4096, kLane = 8, kTableBytes = 16384;
+constexpr int kBlock = 256, kTile = 4096, kLane = 8;
 constexpr uint32_t kSeen = 0x80000000u;  // of a 32-bit table entry
 constexpr uint32_t kRowsMost = 512;  // short rows of a tile (their parameters lie in LDS too)
 
@@ -106,8 +106,8 @@ __device__ __forceinline__ void bias8(const ce_logits& s, uint64_t at, float (&o
 }
 // One score under its table entry, without branches: 11 operations a score, and every lane of a wave runs them where one lane has an
 // entry, so a division (some 12 more) would cost as much as the reads: l / repetition is l times its reciprocal, half a step more off.
-__device__ __forceinline__ float penalise(float l, uint32_t entry, uint32_t times, const Row& row) {
-  const float count = (float)times, scaled = l * (l > 0.f ? row.inverse : row.repetition), z = entry ? scaled : l;
+__device__ __forceinline__ float penalise(float l, uint32_t entry, const Row& row) {
+  const float count = (float)(entry & ~kSeen), scaled = l * (l > 0.f ? row.inverse : row.repetition), z = entry ? scaled : l;
   return count > 0.f ? z - fma_(row.frequency, count, row.presence) : z;
 }
 // z where bit q says so, else -inf, in two operations
@@ -119,14 +119,14 @@ __device__ __forceinline__ float only(float z, uint32_t ok, int q) {
 // ---- a run of one row -----------------------------------------------------------------------------------------------------------
 // What does not wait for something else is read first (a block is a chain of reads: the fewer links, the better): scores, the first tokens of the
 // history whatever its length, the row's own numbers; then the mask, whose place one of these names.
-// The table is 16 KB, 8 blocks a CU: 8192 entries of 16 bits (a history of at most 32767 tokens counts in 15), or 4096 of 32.
-template <class X, class O, class K, class E> __global__ __launch_bounds__(kBlock) void k_logits_run(ce_logits s, uint64_t row0, uint32_t runs) {
-  constexpr uint32_t kRun = kTableBytes / sizeof(E);
-  constexpr int kGroups = kRun / kBlock / kLane, kFirst = 4;
+// The table is 16 KB, 8 blocks a CU.  (Entries of 16 bits and runs of 8192 gain nothing: 29.7 us against 29.0 at 256 x 131072 bfloat16 with
+// histories of up to 2048, 6.1 against 4.7 at 1 x 50257 float; without a history the same pass takes 22, as a copy does.)
+template <class X, class O, class K> __global__ __launch_bounds__(kBlock) void k_logits_run(ce_logits s, uint64_t row0, uint32_t runs) {
+  constexpr int kGroups = kTile / kBlock / kLane, kFirst = 4;
   typedef Pack<X, kLane> Eight;
-  __shared__ __attribute__((aligned(16))) uint32_t table[kTableBytes / 4];
+  __shared__ __attribute__((aligned(16))) uint32_t table[kTile];
   const uint64_t r = row0 + blockIdx.x / runs;
-  const uint32_t v0 = blockIdx.x % runs * kRun, V = (uint32_t)s.vocab, n = V - v0 < kRun ? V - v0 : kRun;
+  const uint32_t v0 = blockIdx.x % runs * kTile, V = (uint32_t)s.vocab, n = V - v0 < kTile ? V - v0 : kTile;
   const X* x = (const X*)s.logits + (int64_t)r * s.logits_row + v0;
   O* o = (O*)s.out + (int64_t)r * s.out_row + v0;
   Eight raw[kGroups];
@@ -153,18 +153,13 @@ template <class X, class O, class K, class E> __global__ __launch_bounds__(kBloc
     ok[g] = k + kLane <= n ? allowed8(s, m, v0 + k) : 0;
   }
   if (used) {
-    for (uint32_t k = threadIdx.x; k < kTableBytes / 16; k += kBlock) ((uint4*)table)[k] = uint4{0, 0, 0, 0};
+    for (uint32_t k = threadIdx.x; k < kTile / 4; k += kBlock) ((uint4*)table)[k] = uint4{0, 0, 0, 0};
     __syncthreads();
     auto count = [&](K tok, uint32_t i) {
       const uint32_t t = place(tok, v0, n);
       if (t >= n) return;
-      if (sizeof(E) == 4) {
-        if (i < prompt) atomicOr(&table[t], kSeen);
-        else atomicAdd(&table[t], 1u);
-      } else {
-        if (i < prompt) atomicOr(&table[t / 2], 0x8000u << (t % 2 * 16));
-        else atomicAdd(&table[t / 2], 1u << (t % 2 * 16));
-      }
+      if (i < prompt) atomicOr(&table[t], kSeen);
+      else atomicAdd(&table[t], 1u);
     };
 #pragma unroll
     for (int u = 0; u < kFirst; ++u)
@@ -172,12 +167,6 @@ template <class X, class O, class K, class E> __global__ __launch_bounds__(kBloc
     each_token<K>(s, r, kFirst * kBlock + threadIdx.x, kBlock, used, count);
     __syncthreads();
   }
-  // an entry in its 32-bit form
-  auto entry = [&](uint32_t k) -> uint32_t {
-    if (sizeof(E) == 4) return table[k];
-    const uint32_t e = ((const uint16_t*)table)[k];
-    return (e & 0x7fffu) | (e & 0x8000u ? kSeen : 0u);
-  };
   const uint64_t b = s.bias ? (s.bias_rows == 1 ? 0 : r % s.bias_rows) * s.vocab + v0 : 0;
 #pragma unroll
   for (int g = 0; g < kGroups; ++g) {
@@ -188,23 +177,11 @@ template <class X, class O, class K, class E> __global__ __launch_bounds__(kBloc
 #pragma unroll
       for (int q = 0; q < 8; ++q) l[q] = (float)raw[g].v[q];
       if (used) {
-        uint4 w[sizeof(E) / 2];
+        const uint4 lo = ((const uint4*)table)[k / 4], hi = ((const uint4*)table)[k / 4 + 1];
+        const uint32_t e[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+        if (lo.x | lo.y | lo.z | lo.w | hi.x | hi.y | hi.z | hi.w)
 #pragma unroll
-        for (uint32_t j = 0; j < sizeof(E) / 2; ++j) w[j] = ((const uint4*)table)[k * sizeof(E) / 16 + j];
-        uint32_t any = w[0].x | w[0].y | w[0].z | w[0].w;
-        if (sizeof(E) == 4) any |= w[sizeof(E) / 2 - 1].x | w[sizeof(E) / 2 - 1].y | w[sizeof(E) / 2 - 1].z | w[sizeof(E) / 2 - 1].w;
-        if (any) {
-          const uint32_t* e = (const uint32_t*)w;
-#pragma unroll
-          for (int q = 0; q < 8; ++q) {
-            if (sizeof(E) == 4) {
-              l[q] = penalise(l[q], e[q], e[q] & ~kSeen, row);
-            } else {
-              const uint32_t half = q % 2 ? e[q / 2] >> 16 : e[q / 2] & 0xffffu;
-              l[q] = penalise(l[q], half, half & 0x7fffu, row);
-            }
-          }
-        }
+          for (int q = 0; q < 8; ++q) l[q] = penalise(l[q], e[q], row);
       }
       if (s.bias)
 #pragma unroll
@@ -215,7 +192,7 @@ template <class X, class O, class K, class E> __global__ __launch_bounds__(kBloc
     } else {
       for (uint32_t j = k; j < n; ++j) {  // the row's last scores
         float z = (float)x[j];
-        if (used) z = penalise(z, entry(j), entry(j) & ~kSeen, row);
+        if (used) z = penalise(z, table[j], row);
         if (s.bias) z += bias_at(s, b + j);
         o[j] = (O)(allowed(s, m, v0 + j) ? z : -__builtin_inff());
       }
@@ -273,7 +250,7 @@ template <class X, class O, class K> __global__ __launch_bounds__(kBlock) void k
     for (int q = 0; q < 8; ++q) {
       if (k + q < n) {
         if (!(dense && whole)) l[q] = (float)x[(int64_t)jj * s.logits_row + vv];
-        if (s.tokens) l[q] = penalise(l[q], table[k + q], table[k + q] & ~kSeen, rows[jj]);
+        if (s.tokens) l[q] = penalise(l[q], table[k + q], rows[jj]);
         if (s.bias) l[q] += bias_at(s, (B == 1 ? 0 : (uint64_t)((uint32_t)(r0 + jj) % B) * V) + vv);
         if (!allowed(s, masks[jj], vv)) l[q] = -__builtin_inff();
         if (!(dense && whole)) o[(int64_t)jj * s.out_row + vv] = (O)l[q];
@@ -287,15 +264,10 @@ template <class X, class O, class K> __global__ __launch_bounds__(kBlock) void k
 template <class X, class O, class K> static void shapes(const ce_logits& s, hipStream_t st) {
   // Half a tile and longer a row is worth blocks of its own; below, a block takes as many rows as fit.
   if (s.vocab > kTile / 2) {
-    // 16-bit entries count a longer run (X us against Y at 256 x 131072 bfloat16), 32-bit ones long histories and few rows, where blocks are short
-    const bool half = s.history < 32768 && s.rows * ((s.vocab + 8191) / 8192) >= 512;
-    const uint32_t run = half ? kTableBytes / 2 : kTableBytes / 4, runs = (uint32_t)((s.vocab + run - 1) / run);
+    const uint32_t runs = (uint32_t)((s.vocab + kTile - 1) / kTile);
     const uint64_t most = (1u << 23) / runs;  // rows of a launch: fewer than 2^32 threads
-    for (uint64_t r = 0; r < s.rows; r += most) {
-      const uint32_t blocks = (uint32_t)(s.rows - r < most ? s.rows - r : most) * runs;
-      if (half) k_logits_run<X, O, K, uint16_t><<<blocks, kBlock, 0, st>>>(s, r, runs);
-      else k_logits_run<X, O, K, uint32_t><<<blocks, kBlock, 0, st>>>(s, r, runs);
-    }
+    for (uint64_t r = 0; r < s.rows; r += most)
+      k_logits_run<X, O, K><<<(uint32_t)(s.rows - r < most ? s.rows - r : most) * runs, kBlock, 0, st>>>(s, r, runs);
     return;
   }
   uint32_t shift = 0;
@@ -328,8 +300,8 @@ hipError_t launch_logits(const ce_logits& s, hipStream_t st) {
 // 2048 columns, or as many whole long rows at a time as fill its lanes.  The long rows are cut into parts; a second launch adds
 // their sums in a fixed order.
 // The few scores that a repetition penalty scaled are put right behind that, one lane to a token of a history: a token that occurs twice
-// is written twice, with the same value.  (Marking them in LDS ahead of the walk, as the forward pass does, took 117 us where this
-// takes X, at 2048 x 32000 bfloat16 with histories of up to 512.)
+// is written twice, with the same value.  (Marking them in LDS ahead of the walk, as the forward pass does, took 113 us where the walk
+// and this take 58 + 27, at 2048 x 32000 bfloat16 with histories of up to 512.)
 constexpr int kCols = kBlock * kLane;
 
 struct GradShape {
