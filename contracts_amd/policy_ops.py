@@ -173,7 +173,7 @@ def linear_scan(x, gate, state=None, done=None, reverse=False, out=None, state_o
             _bad("linear_scan: gate must be of x's type or float32, not %s", gate.dtype)
         grad = grad or gate.requires_grad
         s = gate.stride()
-        if (s[2] != 1 and gate.shape[2] > 1) or s[1] > far:
+        if (s[2] != 1 and gate.shape[2] > 1) or s[1] >= far:
             gate = gate.contiguous()
     else:
         gate = float(gate)
@@ -184,7 +184,7 @@ def linear_scan(x, gate, state=None, done=None, reverse=False, out=None, state_o
     if done is not None:
         if done.dim() != 2 or done.shape[0] != T or done.shape[1] != E or done.dtype not in (torch.bool, torch.uint8):
             _bad("linear_scan: done must be bool or uint8 [T, E]")
-    if (strides[2] != 1 and Ch > 1) or strides[1] > far:
+    if (strides[2] != 1 and Ch > 1) or strides[1] >= far:
         x = x.contiguous()
     grad = grad and torch.is_grad_enabled()
     if out is not None or state_out is not None:

@@ -61,7 +61,8 @@ def _scan(**kw):
     (dict(abi_version=7), "abi_version"), (dict(dtype=4), "x must be"), (dict(dtype=1, gate_dtype=2), "gate must be"), (dict(gate_dtype=1), "gate must be"),
     (dict(dtype=3, gate_dtype=0), "gate must be"), (dict(flags=2), "flags"), (dict(heads=4), "divide"), (dict(heads=0), "divide"), (dict(heads=12), "divide"),
     (dict(rows=1 << 20, channels=1 << 10, heads=1), "columns"), (dict(rows=1 << 40), "columns"), (dict(steps=1 << 60), "elements"), (dict(x=None), "null"), (dict(y=None), "null"),
-    (dict(x=FAKE + 2), "aligned"), (dict(gate=FAKE + 1), "aligned"), (dict(last=FAKE + 2), "aligned"), (dict(gate=None, decay=float("nan")), "finite"),
+    (dict(x=FAKE + 2), "aligned"), (dict(gate=FAKE + 1), "aligned"), (dict(last=FAKE + 2), "aligned"), (dict(x_row=-6), "far apart"), (dict(gate_row=1 << 27), "far apart"),
+    (dict(gate=None, decay=float("nan")), "finite"),
     (dict(gate=None, decay=float("inf")), "finite")])
 def test_scan_refusals(L, kw, word):
     s, nbytes = _scan(**kw), C.c_uint64()

@@ -58,7 +58,7 @@ def check_scan(ops, x, gate, state, done, reverse, tag, grad=True):
 
 # (T, E, C, H): one step, one run of 16 and its borders, tiles of 64, heads of every width (one lane, odd, a wave, several waves), a split time axis
 SIZES = [(1, 1, 1, 1), (1, 5, 7, 7), (2, 64, 256, 256), (15, 3, 2, 1), (16, 3, 2, 2), (17, 2, 64, 64), (63, 1, 65, 5), (64, 1, 130, 130), (65, 4, 130, 13), (100, 3, 40, 1),
-         (130, 2, 66, 33), (257, 1, 96, 3), (300, 3, 264, 1), (700, 1, 200, 1), (1000, 2, 6, 2), (1303, 1, 24, 3), (2051, 2, 10, 10), (5000, 1, 8, 8)]
+         (130, 2, 66, 33), (257, 1, 96, 3), (300, 3, 264, 1), (700, 1, 200, 1), (1000, 2, 6, 2), (512, 1, 8, 4), (530, 2, 130, 2), (1303, 1, 24, 3), (2051, 2, 10, 10), (5000, 1, 8, 8)]
 
 
 @pytest.mark.parametrize("T,E,C,H", SIZES)
@@ -218,6 +218,36 @@ def test_scan_over_offsets_past_32_bits(ops):
     assert y[0, 0, 0].item() == 3 and y[1, 0, 0].item() == 1.5 and y[0, -1, -1].item() == 1 and y[3, -1, 5].item() == 0.125
     assert last[-1].eq(2 + 2.0 ** -16).all() and last[1:-1].count_nonzero().item() == 0 and last[0].eq(3 * 2.0 ** -16).all()
     assert y[:, 1:-1].view(T, -1)[:, ::4099].count_nonzero().item() == 0
+    # and back: dy at both ends of memory reaches the first step's dx and the state
+    y.zero_()
+    y[-1, -1], y[-1, 0] = 1, 4
+    saved = torch.zeros((2, E, C), device="cuda")
+    done = torch.zeros((T, E), dtype=torch.uint8, device="cuda")
+    done[T - 2, 0] = 1
+    dx, _, dstate = ops._scan_backward(y, 0.5, done, False, saved, y, None, True)
+    assert dx[0, -1].eq(2.0 ** -16).all() and dx[-1, -1].eq(1).all() and dstate[-1].eq(2.0 ** -17).all() and dx[-1, 0].eq(4).all()
+    assert dx[:-1, 0].count_nonzero().item() == 0 and dstate[:-1].count_nonzero().item() == 0 and dx[:, 1:-1].view(T, -1)[:, ::4099].count_nonzero().item() == 0
+
+
+@pytest.mark.parametrize("dt,gt,H", [(BF16, BF16, 256), (F32, F32, 4), (F16, F32, 1), (F32, F32, 256)])
+def test_scan_with_columns_enough_for_waves_of_their_own(ops, dt, gt, H):
+    """2048 waves of columns and more: each walks its whole time axis alone, partial runs and heads wider than a wave included"""
+    x, gate, state, done = scan_inputs(35, 2049, 256, H, dt, gt, 77)
+    check_scan(ops, x, gate, state, done, H == 4, "many columns")
+
+
+def test_scan_takes_rows_far_apart(ops):
+    """rows further apart than a wave's 32-bit offsets reach are laid out anew first"""
+    T, E, C, far = 3, 5, 4, 5_000_000
+    x, gate, state, done = scan_inputs(T, E, C, 4, BF16, BF16, 3)
+    wide = torch.zeros(far * E + T * C, dtype=BF16, device="cuda")
+    xx = wide.as_strided((T, E, C), (C, far, 1))
+    xx.copy_(x)
+    gg = wide.clone().as_strided((T, E, C), (C, far, 1))
+    gg.copy_(gate)
+    want = ops.linear_scan(x, gate, state=state, done=done)
+    got = ops.linear_scan(xx, gg, state=state, done=done)
+    assert got[0].equal(want[0]) and got[1].equal(want[1])
 
 
 def test_scan_refusals(ops):
@@ -260,6 +290,17 @@ def test_advantages_read_nothing_past_a_border(ops):
     v[10], r[12] = float("nan"), float("inf")
     adv, ret = ops.advantages(r, v, torch.full((3, 2), float("nan"), device="cuda"), done, gamma=0.5, lam=0.5)
     assert torch.isfinite(adv[:10]).all() and adv[9].eq(1).all() and ret[8].eq(1.25).all()
+
+
+def test_advantages_over_offsets_past_32_bits(ops):
+    P, E, n = 33, 16_777_216, 8  # 4.4e9 values
+    r = torch.zeros((P, E, n), device="cuda")
+    v = torch.zeros((P, E, n), dtype=F16, device="cuda")
+    r[-1, -1], r[5, 0] = 1, 2
+    adv, ret = ops.advantages(r, v, gamma=0.5, lam=1.0, first_plane=0)
+    del r, v
+    assert adv[0, -1].eq(2.0 ** -32).all() and adv[-1, -1].eq(1).all() and adv[0, 0].eq(2.0 ** -4).all() and adv[6, 0].eq(0).all()
+    assert ret[3, -1].eq(2.0 ** -29).all() and adv[:, 1:-1].view(P, -1)[:, ::65521].count_nonzero().item() == 0
 
 
 def test_advantages_write_into_given_planes_and_refuse_the_rest(ops):
@@ -404,6 +445,50 @@ def test_logits_strides_axes_and_outputs(ops, V):
     assert ops.process_logits(same, out=same, **kw) is same and same.equal(z)
     one = ops.process_logits(l[0, 0], tokens=acts[:, 0, 0], lengths=kw["lengths"][0, 0], repetition=1.25, frequency=0.125, bias=bias[0], mask=mask[0])
     assert one.equal(z[0, 0])
+
+
+def test_logits_over_offsets_past_32_bits(ops):
+    R, V = 33000, 131072  # 4.3e9 bfloat16 scores, shaped in place
+    l = torch.ones((R, V), dtype=BF16, device="cuda")
+    tok = torch.full((R, 3), V - 1, dtype=torch.int32, device="cuda")
+    mask = torch.full((1, V // 32), -1, dtype=torch.int32, device="cuda")
+    mask[0, -1] = 0x7fffffff ^ (1 << 29)  # tokens V - 1 and V - 3 are forbidden
+    tok[-1, 0] = V - 2
+    ops.process_logits(l, tokens=tok, frequency=0.5, repetition=2.0, mask=mask, out=l)
+    assert torch.isneginf(l[:, V - 1]).all() and torch.isneginf(l[:, V - 3]).all() and l[-1, V - 2].item() == 0 and l[:-1, V - 2].eq(1).all() and l[:, :V - 3:509].eq(1).all()
+    leaf, bias = l.fill_(-1).requires_grad_(True), torch.zeros((1, V), device="cuda").requires_grad_(True)
+    z = ops.process_logits(leaf, tokens=tok, repetition=2.0, mask=mask, bias=bias)
+    dl, db = torch.autograd.grad(z, (leaf, bias), torch.ones((), dtype=BF16, device="cuda").expand(R, V))
+    assert dl[-1, V - 2].item() == 2 and dl[:-1, V - 2].eq(1).all() and dl[:, V - 1].eq(0).all() and dl[:, :V - 3:509].eq(1).all()
+    assert db[0, V - 1].item() == 0 and db[0, :V - 3].eq(R).all()
+
+
+@pytest.mark.parametrize("V", [1, 3, 9])
+def test_logits_of_very_many_short_rows(ops, V):
+    R, L = 300_001 if V != 3 else 300_000, 11
+    l, tok, lengths, prompt, pen, u = logits_inputs(R, V, L, F32, V, torch.uint8)
+    bias = torch.randn((1 if V != 3 else 6, V), generator=gen(1), device="cuda").requires_grad_(True)
+    allowed = u(R, V) < 0.7
+    dz = torch.randn((R, V), generator=gen(2), device="cuda")
+    leaf = l.clone().requires_grad_(True)
+    # the plain form on the device (its own rounding steps are those of the oracle's bound), histories row by row and as planes
+    seen, count = torch.zeros((R, V), device="cuda", dtype=torch.bool), torch.zeros((R, V), device="cuda")
+    for i in range(L):
+        there = i < lengths
+        hit = torch.nn.functional.one_hot(tok[:, i].long(), V).bool() & there[:, None]
+        seen |= hit
+        count += hit & (i >= prompt)[:, None]
+    factor = torch.where(seen, torch.where(l > 0, 1 / pen["repetition"][:, None], pen["repetition"][:, None]), 1.0)
+    want = l * factor - (count > 0) * pen["presence"][:, None] - count * pen["frequency"][:, None] + bias.detach().repeat(R // bias.shape[0], 1)
+    size = (l * factor).abs() + (count > 0) * pen["presence"][:, None].abs() + count * pen["frequency"][:, None] + bias.detach().abs().max()
+    for t in (tok, tok.t().contiguous().t()):
+        z = ops.process_logits(leaf, tokens=t, lengths=lengths, prompt_lengths=prompt, bias=bias, mask=allowed, **pen)
+        assert torch.isneginf(z[~allowed]).all() and bool(((z - want).abs() <= 10 * oracle.U32 * size)[allowed].all())
+        dl, db = torch.autograd.grad(z, (leaf, bias), dz)
+        wdl = torch.where(allowed, dz * factor, 0.0)
+        assert bool(((dl - wdl).abs() <= 6 * oracle.U32 * wdl.abs()).all())
+        wdb = torch.where(allowed, dz, 0.0).double().view(-1, *bias.shape).sum(0)
+        assert bool(((db - wdb).abs() <= (R // bias.shape[0]) * oracle.U32 * dz.abs().double().view(-1, *bias.shape).sum(0)).all())
 
 
 def test_logits_gradient_against_differences(ops):
