@@ -76,7 +76,10 @@ int check_scan(const ce_scan* s) {
   if (!aligned(s->x, b) || !aligned(s->y, b) || !aligned(s->state, a) || !aligned(s->last, a) || !aligned(s->saved, 4) || (s->gate && !aligned(s->gate, size_of(s->gate_dtype))))
     return refuse("linear_scan: a pointer is not aligned to its type");
   // a wave's lanes reach each other by 32-bit offsets: rows that far apart exist only where short rows are very long in time
-  const int64_t span = std::min<int64_t>((int64_t)s->rows - 1, 255 / (int64_t)s->channels + 1), reach = (int64_t)kMost;
+  // (none where rows are whole waves: multiples of 256 channels, heads a power of two)
+  const uint64_t head = s->gate ? s->channels / s->heads : 1;
+  const bool whole = s->channels % 256 == 0 && (head & (head - 1)) == 0;
+  const int64_t span = whole ? 0 : std::min<int64_t>((int64_t)s->rows - 1, 255 / (int64_t)s->channels + 1), reach = (int64_t)kMost;
   for (int64_t row : {s->x_row, s->gate ? s->gate_row : 0})
     if (row < 0 || (span && row >= reach / span)) return refuse("linear_scan: rows lie too far apart for a wave; lay x and gate out time-major");
   return CE_OK;

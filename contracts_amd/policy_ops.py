@@ -10,7 +10,8 @@ answers with — float scores, of which the step kernel takes the first maximum 
 
 Tensors live on an MI355X (there is no CPU path) and a call is asynchronous on torch's current stream of their device; outputs
 are new tensors unless `out=` names them, scratch memory comes from torch's allocator, nothing is kept between calls, and every call may
-be captured into a graph.  Ordering against other streams (env slices on side streams) is the caller's, as for the engine's steps.
+be captured into a graph (a backward pass together with its forward pass, and with leaves of its own: torch's engine ends the process where
+a captured backward pass meets the nodes of an eager graph of the same leaves).  Ordering against other streams (env slices on side streams) is the caller's, as for the engine's steps.
 A tensor whose last axis is not dense, or whose leading axes do not collapse into one stride, is copied first."""
 import ctypes as C
 
@@ -163,7 +164,9 @@ def linear_scan(x, gate, state=None, done=None, reverse=False, out=None, state_o
         _bad("linear_scan: x must be float32, bfloat16, float16 or float64, not %s", dtype)
     T, E, Ch = x.shape
     acc = torch.float64 if double else torch.float32
-    far = (1 << 28) // (255 // max(Ch, 1) + 1)  # rows that far apart are more than a wave's 32-bit offsets
+    head = Ch // gate.shape[2] if tensor_gate and gate.dim() == 3 and gate.shape[2] else 1
+    # rows that far apart are more than a wave's 32-bit offsets, unless rows are whole waves
+    far = 1 << 62 if Ch % 256 == 0 and head & (head - 1) == 0 else (1 << 28) // (255 // Ch + 1)
     strides = x.stride()
     grad = x.requires_grad
     if tensor_gate:
@@ -386,6 +389,8 @@ def process_logits(logits, *, tokens=None, lengths=None, prompt_lengths=None, re
         if isinstance(v, torch.Tensor):
             if v.device != dev:
                 _bad("process_logits: all tensors must live on one device")
+            if v.requires_grad and torch.is_grad_enabled():
+                _bad("process_logits: %s has no gradient here: detach it", name)
             setattr(h, name, _per_row(name, v, lead, torch.float32))
         else:
             setattr(h, name, float(v))

@@ -42,7 +42,8 @@ const char* ce_policy_error(void);
  * Types: x and y dtype; gate dtype or CE_F32; state and last float (CE_F64: double throughout, and no backward pass).
  * gate == NULL: the constant `decay`.  state / done / last / saved may be NULL (zeros / none ended / not wanted).
  * `last` may be `state` itself (a state moved on in place); no other overlap of outputs with inputs.  x_row and gate_row are not
- * negative, and the rows that 256 channels span, min(E - 1, 255 / C + 1) of them, lie within 2^28 elements of each other. */
+ * negative, and the rows that 256 channels span, min(E - 1, 255 / C + 1) of them (none where C is a
+ * multiple of 256 and heads a power of two of channels), lie within 2^28 elements of each other. */
 #define CE_SCAN_REVERSE 1u
 #define CE_SCAN_SAVED_STEPS 16 /* saved: float [ceil(T / 16)][E][C], what ce_linear_scan_backward starts its tiles from */
 #define CE_SCAN_SPLIT_STEPS 512 /* a call of fewer steps needs no workspace (its time axis is never split over blocks) */

@@ -78,6 +78,20 @@ def test_scan_under_a_constant_gate_without_state_or_done(ops, T, E, C, dt):
         check_scan(ops, x, gate, state, done, reverse, "state and done", grad=dt != F64)
 
 
+@pytest.mark.parametrize("T", [5, 90, 1000])
+def test_scan_gradients_of_one_output_or_to_one_input(ops, T):
+    x, gate, state, done = scan_inputs(T, 2, 12, 3, F32, F32, 13)
+    for reverse in (False, True):
+        want = oracle.scan(x, gate, state, done, reverse)
+        for dy, dl in ((None, torch.randn((2, 12), device="cuda")), (torch.randn(x.shape, device="cuda"), None)):
+            back = oracle.scan_grad(want, dy, dl, 3, reverse)
+            for k, name in enumerate(("dx", "dgate", "dstate")):
+                leaves = [t.clone().requires_grad_(i == k) for i, t in enumerate((x, gate, state))]
+                y, last = ops.linear_scan(leaves[0], leaves[1], state=leaves[2], done=done, reverse=reverse)
+                got = torch.autograd.grad(last if dy is None else y, leaves[k], dl if dy is None else dy)[0]
+                oracle.close(got, back[name], oracle.rounded(back[name], back[name + "bound"], F32), name)
+
+
 @pytest.mark.parametrize("T", [30, 700])
 def test_scan_in_double(ops, T):
     x, gate, state, done = scan_inputs(T, 3, 6, 2, F64, F64, 8)
@@ -248,6 +262,16 @@ def test_scan_takes_rows_far_apart(ops):
     want = ops.linear_scan(x, gate, state=state, done=done)
     got = ops.linear_scan(xx, gg, state=state, done=done)
     assert got[0].equal(want[0]) and got[1].equal(want[1])
+    # whole waves to a row: read where they lie, 2^28 elements apart and more
+    x, gate, state, done = scan_inputs(40, 3, 256, 8, BF16, BF16, 4)
+    wide, far = torch.zeros(2 * (1 << 29) + 40 * 256, dtype=BF16, device="cuda"), 1 << 29
+    xx = wide.as_strided((40, 3, 256), (256, far, 1))
+    xx.copy_(x)
+    leaf, gleaf = xx.requires_grad_(True), gate.clone().requires_grad_(True)
+    y, last = ops.linear_scan(leaf, gleaf, state=state, done=done)
+    y2, last2 = ops.linear_scan(x.requires_grad_(True), gleaf, state=state, done=done)
+    assert y.equal(y2) and last.equal(last2)
+    assert all(a.equal(b) for a, b in zip(torch.autograd.grad(y.sum(), (leaf, gleaf)), torch.autograd.grad(y2.sum(), (x, gleaf))))
 
 
 def test_scan_refusals(ops):
@@ -523,7 +547,8 @@ def test_logits_empty_and_refusals(ops):
     lg, bg = l[:0].clone().requires_grad_(True), l[0].clone().requires_grad_(True)
     assert torch.autograd.grad(ops.process_logits(lg, bias=bg).sum(), bg)[0].equal(torch.zeros_like(bg))
     ok = torch.ones((6, 10), dtype=torch.bool, device="cuda")
-    for kw in (dict(logits=l.double()), dict(logits=l.cpu()), dict(tokens=tok[:5]), dict(tokens=tok.float()), dict(lengths=tok[:, 0]), dict(tokens=tok, lengths=tok[:5, 0]),
+    rep = torch.ones(6, device="cuda").requires_grad_(True)
+    for kw in (dict(tokens=tok, repetition=rep), dict(logits=l.double()), dict(logits=l.cpu()), dict(tokens=tok[:5]), dict(tokens=tok.float()), dict(lengths=tok[:, 0]), dict(tokens=tok, lengths=tok[:5, 0]),
                dict(tokens=tok, lengths=tok[:, 0].float()), dict(tokens=tok, repetition=l[0, :5]), dict(bias=l[:, :9]), dict(bias=l.double()), dict(bias=l[:1].bfloat16()),
                dict(mask=ok[:, :9]), dict(mask=ok.float()), dict(mask=torch.zeros((6, 2), dtype=torch.int32, device="cuda")), dict(mask_index=tok[:, 0]),
                dict(mask=ok[:3], mask_index=tok[:5, 0]), dict(out=l.half()), dict(out=l[:5]), dict(out=l.t().contiguous().t()), dict(logits=l.clone().requires_grad_(True), out=torch.empty_like(l)),
