@@ -5,7 +5,6 @@ import of the library / creation of an engine fails loudly.
 """
 import ctypes as C
 import os
-import struct
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("CONTRACTS_AMD_LIB") or os.path.join(HERE, "csrc", "libcontracts_engine.so")
@@ -130,7 +129,6 @@ EXPORTS = {
 POLICY_LIB_PATH = os.path.join(HERE, "csrc", "libcontracts_policy.so")
 POLICY_ABI_VERSION = 1
 F32, BF16, F16, F64, U8, I32, I64 = range(7)  # enum ce_dtype
-SCAN_REVERSE, SCAN_SAVED_STEPS, SCAN_SPLIT_STEPS, ADV_DONE_PER_AGENT = 1, 16, 512, 1
 
 
 class CeScan(C.Structure):
@@ -165,27 +163,17 @@ class CeLogitsGrad(C.Structure):
     _fields_ = [("dout", _P), ("dout_row", C.c_int64), ("dlogits", _P), ("dbias", _P)]
 
 
-def packer(cls):
-    """struct.Struct.pack of a flat ctypes structure, fields in order: a call's arguments as one bytes object (several times quicker than
-    filling the structure field by field; a call's latency is mostly the host's)"""
-    code = {C.c_uint32: "I", C.c_int32: "i", C.c_uint64: "Q", C.c_int64: "q", C.c_double: "d", C.c_void_p: "P"}
-    f = struct.Struct("@" + "".join(code[t] for _, t in cls._fields_))
-    assert f.size == C.sizeof(cls)
-    return f.pack
-
-
-# every structure goes in as an address: C.byref(CeScan(..)) or the bytes that packer(CeScan) made
 POLICY_EXPORTS = {
     "ce_policy_abi_version": (C.c_int, []),
     "ce_policy_error": (C.c_char_p, []),
-    "ce_linear_scan_workspace": (C.c_int, [_P, C.POINTER(C.c_uint64)]),
-    "ce_linear_scan": (C.c_int, [_P, _P]),
-    "ce_linear_scan_backward_workspace": (C.c_int, [_P, _P, C.POINTER(C.c_uint64)]),
-    "ce_linear_scan_backward": (C.c_int, [_P, _P, _P]),
-    "ce_advantages": (C.c_int, [_P, _P]),
-    "ce_process_logits": (C.c_int, [_P, _P]),
-    "ce_process_logits_backward_workspace": (C.c_int, [_P, _P, C.POINTER(C.c_uint64)]),
-    "ce_process_logits_backward": (C.c_int, [_P, _P, _P]),
+    "ce_linear_scan_workspace": (C.c_int, [C.POINTER(CeScan), C.POINTER(C.c_uint64)]),
+    "ce_linear_scan": (C.c_int, [C.POINTER(CeScan), C.c_void_p]),
+    "ce_linear_scan_backward_workspace": (C.c_int, [C.POINTER(CeScan), C.POINTER(CeScanGrad), C.POINTER(C.c_uint64)]),
+    "ce_linear_scan_backward": (C.c_int, [C.POINTER(CeScan), C.POINTER(CeScanGrad), C.c_void_p]),
+    "ce_advantages": (C.c_int, [C.POINTER(CeAdvantage), C.c_void_p]),
+    "ce_process_logits": (C.c_int, [C.POINTER(CeLogits), C.c_void_p]),
+    "ce_process_logits_backward_workspace": (C.c_int, [C.POINTER(CeLogits), C.POINTER(CeLogitsGrad), C.POINTER(C.c_uint64)]),
+    "ce_process_logits_backward": (C.c_int, [C.POINTER(CeLogits), C.POINTER(CeLogitsGrad), C.c_void_p]),
 }
 
 _lib = None
@@ -243,9 +231,15 @@ def load_policy():
     return L
 
 
-def check_policy(rc, what):
-    if rc != 0:
-        raise EngineError("%s failed: %s (%d) %s" % (what, ERRORS.get(rc, "?"), rc, (load_policy().ce_policy_error() or b"").decode()))
+def load_policy_torch():
+    """Loads the torch front of the policy operators (csrc/cp_torch.cpp), which is what policy_ops calls."""
+    load_policy()
+    try:
+        from . import _ce_policy
+    except ImportError as exc:
+        raise EngineError("policy operators' torch extension missing or built against another torch: build it with `python -m contracts_amd.build` (%s)" % exc) from exc
+    _ce_policy.set_error(EngineError)
+    return _ce_policy
 
 
 def check(rc, handle=None, what=""):

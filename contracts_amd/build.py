@@ -31,6 +31,7 @@ FLAGS = ["-O3", "--offload-arch=gfx950", "-std=c++17", "-fPIC", "-ffp-contract=o
 POLICY_LIB = os.path.join(CSRC, "libcontracts_policy.so")
 POLICY_SOURCES = ["cp_api.hip", "cp_scan.hip", "cp_scan_grad.hip", "cp_advantage.hip", "cp_logits.hip"]
 POLICY_HEADERS = ["cp_common.h", os.path.join("..", "..", "include", "contracts_policy.h"), os.path.join("..", "..", "include", "contracts_engine.h")]
+POLICY_TORCH_SRC = "cp_torch.cpp"  # their torch front: host code, built against the torch that is installed
 POLICY_FLAGS = ["-O3", "--offload-arch=gfx950", "-std=c++17", "-fPIC", "-fno-fast-math", "-fno-gpu-rdc", "-Wall",
                 "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops", "-mllvm", "-amdgpu-kernarg-preload-count=16"]
 
@@ -78,8 +79,33 @@ def fingerprint():
 
 
 def policy_fingerprint():
-    """what the policy library is a function of"""
-    return {"files": {s: _sha16(os.path.join(CSRC, s)) for s in POLICY_SOURCES + POLICY_HEADERS}, "flags": POLICY_FLAGS}
+    """what the policy library and its torch front are a function of"""
+    from importlib.metadata import version
+    return {"files": {s: _sha16(os.path.join(CSRC, s)) for s in POLICY_SOURCES + POLICY_HEADERS + [POLICY_TORCH_SRC]}, "flags": POLICY_FLAGS, "torch": version("torch")}
+
+
+def policy_torch_path():
+    import sysconfig
+    return os.path.join(HERE, "_ce_policy" + (sysconfig.get_config_var("EXT_SUFFIX") or ".so"))
+
+
+def compile_policy_torch(verbose=False):
+    """starts the compiler on the torch front; the library it is linked with may still be under way"""
+    import sysconfig
+    import torch
+    root = os.path.dirname(torch.__file__)
+    cxx = shutil.which("g++") or shutil.which("c++")
+    if cxx is None:
+        raise RuntimeError("no C++ compiler for contracts_amd/csrc/cp_torch.cpp")
+    obj = os.path.join(CSRC, POLICY_TORCH_SRC.replace(".cpp", ".o"))
+    cmd = [cxx, "-O2", "-fPIC", "-std=c++17", "-Wall", "-Wno-unused-function", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1", "-DTORCH_EXTENSION_NAME=_ce_policy",
+           "-D_GLIBCXX_USE_CXX11_ABI=%d" % torch._C._GLIBCXX_USE_CXX11_ABI, "-I", os.path.join(root, "include"), "-I", os.path.join(root, "include", "torch", "csrc", "api", "include"),
+           "-I", os.path.join(os.environ.get("ROCM_PATH", "/opt/rocm"), "include"), "-I", sysconfig.get_paths()["include"], "-c", os.path.join(CSRC, POLICY_TORCH_SRC), "-o", obj]
+    link = [cxx, "-shared", "-o", policy_torch_path(), obj, "-L", os.path.join(root, "lib"), "-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch", "-ltorch_python",
+            "-L", CSRC, "-lcontracts_policy", "-Wl,-rpath,$ORIGIN/csrc"]
+    if verbose:
+        print(" ".join(cmd))
+    return cmd, subprocess.Popen(cmd), link
 
 
 def kernels_sha16(fp=None):
@@ -130,11 +156,17 @@ def policy_needs_build():
             rec = json.load(f)
     except (OSError, ValueError):
         return True
-    return not os.path.exists(POLICY_LIB) or rec.get("fingerprint") != policy_fingerprint() or rec.get("lib_sha16") != _sha16(POLICY_LIB)
+    return not os.path.exists(POLICY_LIB) or not os.path.exists(policy_torch_path()) or rec.get("fingerprint") != policy_fingerprint() or rec.get("lib_sha16") != _sha16(POLICY_LIB)
 
 
 def build_policy(verbose=False):
+    cmd, front, link = compile_policy_torch(verbose)
     _compile(POLICY_SOURCES, POLICY_FLAGS, POLICY_LIB, "", verbose)
+    if front.wait() != 0:
+        raise subprocess.CalledProcessError(1, cmd)
+    if verbose:
+        print(" ".join(link))
+    subprocess.check_call(link)
     with open(POLICY_INFO, "w") as f:
         json.dump({"fingerprint": policy_fingerprint(), "lib_sha16": _sha16(POLICY_LIB), "offload_arch": "gfx950",
                    "built_at": time.strftime("%Y-%m-%dT%H:%M:%SZ", time.gmtime())}, f, indent=1)
@@ -174,10 +206,15 @@ def build(force=False, verbose=False):
     if not force and not needs_build():
         return LIB
     t0 = time.time()
-    _compile(SOURCES, flags, lib, suffix, verbose)
-    if lib == LIB:
+    if lib != LIB:
+        _compile(SOURCES, flags, lib, suffix, verbose)
+    else:
+        from concurrent.futures import ThreadPoolExecutor
+        with ThreadPoolExecutor(1) as side:  # the policy operators build beside the engine
+            policy = side.submit(build_policy, verbose)
+            _compile(SOURCES, flags, lib, suffix, verbose)
+            policy.result()
         build_pydict(verbose)
-        build_policy(verbose)
         ver = subprocess.run([hipcc(), "--version"], capture_output=True, text=True).stdout.strip().splitlines()
         with open(INFO, "w") as f:
             head, dirty = git_state()

@@ -13,19 +13,19 @@ are new tensors unless `out=` names them, scratch memory comes from torch's allo
 be captured into a graph (a backward pass together with its forward pass, and with leaves of its own: torch's engine ends the process where
 a captured backward pass meets the nodes of an eager graph of the same leaves).  Ordering against other streams (env slices on side streams) is the caller's, as for the engine's steps.
 A tensor whose last axis is not dense, or whose leading axes do not collapse into one stride, is copied first."""
-import ctypes as C
-
 import torch
 
 from . import _lib
 
-_CODE = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16, torch.float16: _lib.F16, torch.float64: _lib.F64, torch.uint8: _lib.U8,
-         torch.bool: _lib.U8, torch.int32: _lib.I32, torch.int64: _lib.I64}
 _REAL = (torch.float32, torch.bfloat16, torch.float16)
-_ABI = _lib.POLICY_ABI_VERSION
-_scan_args, _scan_grad_args, _adv_args, _logits_args, _logits_grad_args = (
-    _lib.packer(c) for c in (_lib.CeScan, _lib.CeScanGrad, _lib.CeAdvantage, _lib.CeLogits, _lib.CeLogitsGrad))
-_stream = torch._C._cuda_getCurrentRawStream  # torch's current stream of a device, without the wrapper object around it
+_loaded = None
+
+
+def _ext():
+    global _loaded
+    if _loaded is None:
+        _loaded = _lib.load_policy_torch()
+    return _loaded
 
 
 def _bad(what, *args):
@@ -41,10 +41,6 @@ def _device(op, first, *tensors):
         if t is not None and t.device != dev:
             _bad("%s: all tensors must live on one device", op)
     return dev
-
-
-def _ptr(t):
-    return 0 if t is None else t.data_ptr()
 
 
 def _span(t):
@@ -65,81 +61,7 @@ def _apart(op, out, name, *inputs):
                 _bad("%s: %s overlaps an input", op, name)
 
 
-def _workspace(fn, dev, *structs):
-    nbytes = C.c_uint64()
-    _lib.check_policy(fn(*structs, C.byref(nbytes)), fn.__name__)
-    return None if nbytes.value == 0 else torch.empty(nbytes.value, dtype=torch.uint8, device=dev)
-
-
 # ---- linear_scan ---------------------------------------------------------------------------------------------------------------
-def _scan_struct(x, gate, done, reverse, state, y, last, saved, ws):
-    T, E, Ch = x.shape
-    xs, code = x.stride(), _CODE[x.dtype]
-    if isinstance(gate, torch.Tensor):
-        gs, gcode, heads, decay, gptr = gate.stride(), _CODE[gate.dtype], gate.shape[2], 0.0, gate.data_ptr()
-    else:
-        gs, gcode, heads, decay, gptr = (0, 0), code, Ch, gate, 0
-    ds, dptr = (done.stride(), done.data_ptr()) if done is not None else ((0, 0), 0)
-    return _scan_args(_ABI, x.device.index, code, gcode, _lib.SCAN_REVERSE if reverse else 0, 0, T, E, Ch, heads, xs[0], xs[1], gs[0], gs[1], ds[0], ds[1], decay,
-                      x.data_ptr(), gptr, dptr, _ptr(state), _ptr(y), _ptr(last), _ptr(saved), _ptr(ws), 0 if ws is None else ws.numel())
-
-
-def _scan_forward(x, gate, state, done, reverse, y, last, want_saved):
-    L = _lib.load_policy()
-    T, E, Ch = x.shape
-    dev = x.device
-    if y is None:
-        y = torch.empty((T, E, Ch), dtype=x.dtype, device=dev)
-    if last is None:
-        last = torch.empty((E, Ch), dtype=torch.float64 if x.dtype == torch.float64 else torch.float32, device=dev)
-    saved = torch.empty((-(-T // _lib.SCAN_SAVED_STEPS), E, Ch), dtype=torch.float32, device=dev) if want_saved else None
-    ws = None
-    if T >= _lib.SCAN_SPLIT_STEPS:
-        ws = _workspace(L.ce_linear_scan_workspace, dev, _scan_struct(x, gate, done, reverse, state, y, last, saved, None))
-    rc = L.ce_linear_scan(_scan_struct(x, gate, done, reverse, state, y, last, saved, ws), _stream(dev.index))
-    if rc:
-        _lib.check_policy(rc, "linear_scan")
-    return y, last, saved
-
-
-def _scan_backward(x, gate, done, reverse, saved, dy, dlast, need_state):
-    L = _lib.load_policy()
-    T, E, Ch = x.shape
-    dev = x.device
-    dx = torch.empty((T, E, Ch), dtype=x.dtype, device=dev)
-    dgate = (torch.empty if x.numel() else torch.zeros)(gate.shape, dtype=gate.dtype, device=dev) if isinstance(gate, torch.Tensor) else None
-    dstate = torch.empty((E, Ch), dtype=torch.float32, device=dev) if need_state else None
-    dy = torch.zeros((T, E, Ch), dtype=x.dtype, device=dev) if dy is None else dy if dy.is_contiguous() else dy.contiguous()
-    if dlast is not None and not dlast.is_contiguous():
-        dlast = dlast.contiguous()
-    g = _scan_grad_args(dy.data_ptr(), _ptr(dlast), dx.data_ptr(), _ptr(dgate), _ptr(dstate))
-    ws = None
-    if T >= _lib.SCAN_SPLIT_STEPS or (dgate is not None and gate.shape[2] != Ch):
-        ws = _workspace(L.ce_linear_scan_backward_workspace, dev, _scan_struct(x, gate, done, reverse, None, None, None, saved, None), g)
-    rc = L.ce_linear_scan_backward(_scan_struct(x, gate, done, reverse, None, None, None, saved, ws), g, _stream(dev.index))
-    if rc:
-        _lib.check_policy(rc, "linear_scan_backward")
-    return dx, dgate, dstate
-
-
-class _Scan(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, gate, state, done, reverse):
-        ctx.set_materialize_grads(False)
-        y, last, saved = _scan_forward(x, gate, state, done, reverse, None, None, True)
-        ctx.reverse, ctx.const = reverse, None if isinstance(gate, torch.Tensor) else gate
-        ctx.save_for_backward(x, gate if ctx.const is None else None, done, saved)
-        return y, last
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, dy, dlast):
-        x, gate, done, saved = ctx.saved_tensors
-        need = ctx.needs_input_grad
-        dx, dgate, dstate = _scan_backward(x, gate if ctx.const is None else ctx.const, done, ctx.reverse, saved, dy, dlast, need[2])
-        return dx if need[0] else None, dgate if need[1] else None, dstate, None, None
-
-
 def linear_scan(x, gate, state=None, done=None, reverse=False, out=None, state_out=None):
     """The gated linear recurrence along the time axis: (y [T, E, C] in x's type, last [E, C] float32).
 
@@ -202,12 +124,9 @@ def linear_scan(x, gate, state=None, done=None, reverse=False, out=None, state_o
         _apart("linear_scan", state_out, "state_out", None if moved else state, *others)
     if state is not None and not state.is_contiguous():
         state = state.contiguous()
-    if grad:
-        if double:
-            _bad("linear_scan: float64 has no backward pass")
-        return _Scan.apply(x, gate, state, done, bool(reverse))
-    y, last, _ = _scan_forward(x, gate, state, done, reverse, out, state_out, False)
-    return y, last
+    if grad and double:
+        _bad("linear_scan: float64 has no backward pass")
+    return _ext().linear_scan(x, gate if tensor_gate else None, 0.0 if tensor_gate else gate, state, done, bool(reverse), out, state_out, grad)
 
 
 # ---- advantages -----------------------------------------------------------------------------------------------------------------
@@ -222,7 +141,7 @@ def advantages(reward, value, last_value=None, done=None, gamma=0.99, lam=0.95, 
     if not isinstance(reward, torch.Tensor) or reward.dim() != 3:
         _bad("advantages: reward must be [P, E, n]")
     adv, ret = (None, None) if out is None else out
-    dev = _device("advantages", reward, value, last_value, done, adv, ret)
+    _device("advantages", reward, value, last_value, done, adv, ret)
     shape = P, E, n = reward.shape
     if reward.dtype != torch.float64 and reward.dtype != torch.float32:
         _bad("advantages: reward must be float64 or float32, not %s", reward.dtype)
@@ -232,7 +151,6 @@ def advantages(reward, value, last_value=None, done=None, gamma=0.99, lam=0.95, 
         if last_value.shape != shape[1:] or last_value.dtype != value.dtype:
             _bad("advantages: last_value must be %s %s", value.dtype, (E, n))
         last_value = last_value.contiguous()
-    per_agent = False
     if done is not None:
         per_agent = done.dim() == 3
         if done.shape != (shape if per_agent else shape[:2]) or done.dtype not in (torch.bool, torch.uint8):
@@ -242,20 +160,13 @@ def advantages(reward, value, last_value=None, done=None, gamma=0.99, lam=0.95, 
     if not 0 <= first_plane < max(P, 1):
         _bad("advantages: first_plane out of range")
     reward, value = reward.contiguous(), value.contiguous()
-    if out is None:
-        adv, ret = torch.empty(shape, dtype=torch.float32, device=dev), torch.empty(shape, dtype=torch.float32, device=dev)
-    else:
+    if out is not None:
         for t in out:
             if t.shape != shape or t.dtype != torch.float32 or not t.is_contiguous():
                 _bad("advantages: out must be two dense float32 %s", tuple(shape))
         _apart("advantages", adv, "out", reward, value, last_value, done, ret)
         _apart("advantages", ret, "out", reward, value, last_value, done)
-    a = _adv_args(_ABI, dev.index, _CODE[reward.dtype], _CODE[value.dtype], _lib.ADV_DONE_PER_AGENT if per_agent else 0, first_plane, P, E, n, float(gamma),
-                  float(lam), reward.data_ptr(), value.data_ptr(), _ptr(last_value), _ptr(done), adv.data_ptr(), ret.data_ptr())
-    rc = _lib.load_policy().ce_advantages(a, _stream(dev.index))
-    if rc:
-        _lib.check_policy(rc, "advantages")
-    return adv, ret
+    return _ext().advantages(reward, value, last_value, done, float(gamma), float(lam), first_plane, adv, ret)
 
 
 # ---- process_logits ---------------------------------------------------------------------------------------------------------------
@@ -265,72 +176,6 @@ def pack_mask(allowed):
     bits = torch.nn.functional.pad(allowed.to(torch.int64), (0, -V % 32)).unflatten(-1, (-1, 32))
     words = (bits << torch.arange(32, device=allowed.device)).sum(-1)
     return torch.where(words >= 2 ** 31, words - 2 ** 32, words).to(torch.int32)
-
-
-class _Shaping:
-    """what scores are shaped with, checked and laid out: everything of a ce_logits but the scores, the bias and the output"""
-    __slots__ = ("tokens", "lengths", "prompt_lengths", "repetition", "presence", "frequency", "mask", "mask_index")
-
-    def struct(self, rows, V, logits, row, bias, out_dtype, out, out_row, ws):
-        t, m, scalar, ptr = self.tokens, self.mask, [1.0, 0.0, 0.0], [0, 0, 0]
-        if t is not None and t.numel():
-            for k, v in enumerate((self.repetition, self.presence, self.frequency)):
-                if isinstance(v, torch.Tensor):
-                    ptr[k] = v.data_ptr()
-                else:
-                    scalar[k] = v
-            history = (t.stride(0), t.stride(1), t.shape[1], _CODE[t.dtype], t.data_ptr(), _ptr(self.lengths), _ptr(self.prompt_lengths))
-        else:
-            history = (0, 0, 0, 0, 0, 0, 0)
-        return _logits_args(_ABI, logits.device.index, _CODE[logits.dtype], _CODE[out_dtype], history[3], 0 if bias is None else _CODE[bias.dtype],
-                            0 if m is None else _CODE[m.dtype], 0, rows, V, history[2], row, out_row, history[0], history[1], 0 if bias is None else bias.shape[0],
-                            0 if m is None else m.shape[0], scalar[0], scalar[1], scalar[2], logits.data_ptr(), history[4], history[5], history[6], ptr[0], ptr[1], ptr[2],
-                            _ptr(bias), _ptr(m), _ptr(self.mask_index), _ptr(out), _ptr(ws), 0 if ws is None else ws.numel())
-
-
-class _Logits(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, logits, bias, h):
-        ctx.set_materialize_grads(False)
-        ctx.rest = [(k, v) for k in _Shaping.__slots__ for v in (getattr(h, k),) if not isinstance(v, torch.Tensor)]
-        ctx.names = [k for k in _Shaping.__slots__ if isinstance(getattr(h, k), torch.Tensor)]
-        ctx.save_for_backward(logits, bias, *[getattr(h, k) for k in ctx.names])
-        out = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
-        _logits_forward(logits, logits.shape[0], logits.shape[1], logits.stride(0), bias, h, out, logits.shape[1])
-        return out
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, dz):
-        if dz is None:
-            return None, None, None
-        logits, bias, *rest = ctx.saved_tensors
-        h = _Shaping()
-        for k, v in ctx.rest:
-            setattr(h, k, v)
-        for k, v in zip(ctx.names, rest):
-            setattr(h, k, v)
-        L = _lib.load_policy()
-        rows, V = logits.shape
-        dev = logits.device
-        if dz.stride(1) != 1 and V > 1:
-            dz = dz.contiguous()
-        dlogits = torch.empty((rows, V), dtype=logits.dtype, device=dev) if ctx.needs_input_grad[0] else None
-        dbias = (torch.empty_like if logits.numel() else torch.zeros_like)(bias) if ctx.needs_input_grad[1] else None
-        g = _logits_grad_args(dz.data_ptr(), dz.stride(0), _ptr(dlogits), _ptr(dbias))
-        ws = None
-        if dbias is not None:
-            ws = _workspace(L.ce_process_logits_backward_workspace, dev, h.struct(rows, V, logits, logits.stride(0), bias, dz.dtype, None, 0, None), g)
-        rc = L.ce_process_logits_backward(h.struct(rows, V, logits, logits.stride(0), bias, dz.dtype, None, 0, ws), g, _stream(dev.index))
-        if rc:
-            _lib.check_policy(rc, "process_logits_backward")
-        return dlogits, dbias, None
-
-
-def _logits_forward(logits, rows, V, row, bias, h, out, out_row):
-    rc = _lib.load_policy().ce_process_logits(h.struct(rows, V, logits, row, bias, out.dtype, out, out_row, None), _stream(logits.device.index))
-    if rc:
-        _lib.check_policy(rc, "process_logits")
 
 
 def _table(name, t, lead, width):
@@ -384,27 +229,29 @@ def process_logits(logits, *, tokens=None, lengths=None, prompt_lengths=None, re
     dev = _device("process_logits", logits, tokens, lengths, prompt_lengths, bias, mask, mask_index, out)
     lead, V = logits.shape[:-1], logits.shape[-1]
     rows = lead.numel()
-    h = _Shaping()
-    for name, v in (("repetition", repetition), ("presence", presence), ("frequency", frequency)):
+    tensors, scalars = [], []
+    for name, v, none in (("repetition", repetition, 1.0), ("presence", presence, 0.0), ("frequency", frequency, 0.0)):
         if isinstance(v, torch.Tensor):
             if v.device != dev:
                 _bad("process_logits: all tensors must live on one device")
             if v.requires_grad and torch.is_grad_enabled():
                 _bad("process_logits: %s has no gradient here: detach it", name)
-            setattr(h, name, _per_row(name, v, lead, torch.float32))
+            tensors.append(_per_row(name, v, lead, torch.float32))
+            scalars.append(none)
         else:
-            setattr(h, name, float(v))
-    h.tokens = h.lengths = h.prompt_lengths = h.mask = h.mask_index = None
+            tensors.append(None)
+            scalars.append(float(v))
     if tokens is not None:
         if tokens.dim() != logits.dim() or tokens.shape[:-1] != lead:
             _bad("process_logits: tokens must be %s + [L], got %s", tuple(lead), tuple(tokens.shape))
         if tokens.dtype not in (torch.uint8, torch.int32, torch.int64):
             _bad("process_logits: tokens must be uint8, int32 or int64, not %s", tokens.dtype)
-        h.tokens = tokens if tokens.dim() == 2 else tokens.reshape(rows, tokens.shape[-1])
+        if tokens.dim() != 2:
+            tokens = tokens.reshape(rows, tokens.shape[-1])
         if lengths is not None:
-            h.lengths = _per_row("lengths", lengths, lead, torch.int32)
+            lengths = _per_row("lengths", lengths, lead, torch.int32)
         if prompt_lengths is not None:
-            h.prompt_lengths = _per_row("prompt_lengths", prompt_lengths, lead, torch.int32)
+            prompt_lengths = _per_row("prompt_lengths", prompt_lengths, lead, torch.int32)
     elif lengths is not None or prompt_lengths is not None:
         _bad("process_logits: lengths without tokens")
     if mask is not None:
@@ -413,8 +260,8 @@ def process_logits(logits, *, tokens=None, lengths=None, prompt_lengths=None, re
         if mask_index is not None:
             if mask.dim() != 2:
                 _bad("process_logits: an indexed mask must be a table [S, ..]")
-            h.mask_index = _per_row("mask_index", mask_index, lead, torch.int32)
-        h.mask = _table("mask", mask, () if mask_index is not None else lead, -(-V // 32) if mask.dtype == torch.int32 else V)
+            mask_index = _per_row("mask_index", mask_index, lead, torch.int32)
+        mask = _table("mask", mask, () if mask_index is not None else lead, -(-V // 32) if mask.dtype == torch.int32 else V)
     elif mask_index is not None:
         _bad("process_logits: mask_index without a mask")
     grad = logits.requires_grad
@@ -429,23 +276,19 @@ def process_logits(logits, *, tokens=None, lengths=None, prompt_lengths=None, re
     flat = logits if logits.dim() == 2 else logits.reshape(rows, V)
     if V > 1 and flat.stride(1) != 1:
         flat = flat.contiguous()
-    if grad:
-        z = _Logits.apply(flat, bias, h)
-        return z if logits.dim() == 2 else z.view(logits.shape)
-    if out is None:
-        out = torch.empty(logits.shape, dtype=dtype, device=dev)
-        _logits_forward(flat, rows, V, flat.stride(0), bias, h, out, V)
+    to = None
+    if out is not None:
+        if out.shape != logits.shape or (out.dtype != torch.float32 and out.dtype != dtype):
+            _bad("process_logits: out must be %s, float32 or of the logits' type", tuple(logits.shape))
+        try:
+            to = out.view(rows, V)
+        except RuntimeError:
+            pass
+        if to is None or (V > 1 and to.stride(1) != 1):
+            _bad("process_logits: out's leading axes must collapse into one stride, its last be dense")
+        same = to.data_ptr() == flat.data_ptr() and to.dtype == flat.dtype and to.stride() == flat.stride()
+        _apart("process_logits", to, "out", None if same else flat, tokens, lengths, prompt_lengths, mask, mask_index, bias, *tensors)
+    z = _ext().process_logits(flat, bias, tokens, lengths, prompt_lengths, mask, mask_index, *tensors, *scalars, to, grad)
+    if out is not None:
         return out
-    if out.shape != logits.shape or (out.dtype != torch.float32 and out.dtype != dtype):
-        _bad("process_logits: out must be %s, float32 or of the logits' type", tuple(logits.shape))
-    try:
-        to = out.view(rows, V)
-    except RuntimeError:
-        to = None
-    if to is None or (V > 1 and to.stride(1) != 1):
-        _bad("process_logits: out's leading axes must collapse into one stride, its last be dense")
-    same = to.data_ptr() == flat.data_ptr() and to.dtype == flat.dtype and to.stride() == flat.stride()
-    _apart("process_logits", to, "out", None if same else flat, h.tokens, h.lengths, h.prompt_lengths, h.mask, h.mask_index, bias,
-           *[v for v in (h.repetition, h.presence, h.frequency) if isinstance(v, torch.Tensor)])
-    _logits_forward(flat, rows, V, flat.stride(0), bias, h, to, to.stride(0))
-    return out
+    return z if logits.dim() == 2 else z.view(logits.shape)

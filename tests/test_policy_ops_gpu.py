@@ -222,6 +222,19 @@ def test_scan_gradient_against_differences(ops):
                 assert abs(up - down - d[i].item()) <= 1e-5 * (1 + abs(d[i].item())) * 8
 
 
+def test_gradients_of_gradients_are_refused_not_wrong(ops):
+    x, gate, state, done = scan_inputs(7, 2, 4, 2, F32, F32, 4)
+    leaf = x.clone().requires_grad_(True)
+    want = torch.autograd.grad(ops.linear_scan(leaf, gate, done=done)[0].sum(), leaf)[0]
+    got = torch.autograd.grad(ops.linear_scan(leaf, gate, done=done)[0].sum(), leaf, create_graph=True)[0]
+    assert got.equal(want)
+    with pytest.raises(RuntimeError, match="no gradients of their own"):
+        got.sum().backward()
+    z = torch.autograd.grad(ops.process_logits(leaf[:, 0], bias=gate[0, 0].repeat(2)).sum(), leaf, create_graph=True)[0]
+    with pytest.raises(RuntimeError, match="no gradients of their own"):
+        z.sum().backward()
+
+
 def test_scan_over_offsets_past_32_bits(ops):
     """a rollout of 2^32 and some elements: the last columns and steps are where a 32-bit offset would wrap"""
     T, E, C = 17, 131072, 1928  # 4.3e9 bfloat16 elements
@@ -235,10 +248,11 @@ def test_scan_over_offsets_past_32_bits(ops):
     # and back: dy at both ends of memory reaches the first step's dx and the state
     y.zero_()
     y[-1, -1], y[-1, 0] = 1, 4
-    saved = torch.zeros((2, E, C), device="cuda")
     done = torch.zeros((T, E), dtype=torch.uint8, device="cuda")
     done[T - 2, 0] = 1
-    dx, _, dstate = ops._scan_backward(y, 0.5, done, False, saved, y, None, True)
+    x, state = torch.zeros((T, E, C), dtype=BF16, device="cuda").requires_grad_(True), torch.zeros((E, C), device="cuda").requires_grad_(True)
+    out = ops.linear_scan(x, 0.5, state=state, done=done)
+    dx, dstate = torch.autograd.grad(out[0], (x, state), y)
     assert dx[0, -1].eq(2.0 ** -16).all() and dx[-1, -1].eq(1).all() and dstate[-1].eq(2.0 ** -17).all() and dx[-1, 0].eq(4).all()
     assert dx[:-1, 0].count_nonzero().item() == 0 and dstate[:-1].count_nonzero().item() == 0 and dx[:, 1:-1].view(T, -1)[:, ::4099].count_nonzero().item() == 0
 
