@@ -180,7 +180,8 @@ void plan_scan(const ce_scan* s, const ce_scan_grad* g, Plan* o) {
       p.slabs = p.in_wave ? 1 : (p.lanes + 63) / 64;
     }
   }
-  p.flags = !s->done ? cp::kFlagsNone : p.row_cols >= cp::kBallotRow ? cp::kFlagsBallot : cp::kFlagsLane;
+  const uint32_t spanned = 62 / p.row_cols + 2;  // rows that 64 lanes can touch
+  p.flags = !s->done ? cp::kFlagsNone : spanned <= 4 ? cp::kFlags4 : spanned <= 16 ? cp::kFlags16 : cp::kFlagsLane;
   // the chunks of a split time axis read the incoming state while the last of them writes the outgoing one
   if (!g && s->last && s->last == s->state) p.chunks = 1;
   if (p.chunks == 1) p.chunk = T;

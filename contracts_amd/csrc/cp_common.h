@@ -48,10 +48,9 @@ template <> __device__ __forceinline__ float step(float a, float h, float x) { r
 template <class A> __device__ __forceinline__ A apply(A P, A H, A h) { return h == A(0) ? H : step(P, h, H); }
 
 // Done flags of a wave's run of 16 steps as 16 bits a lane.  A wave spans at most 4 rows where a row has 21 lanes or more: then each
-// quarter of the lanes reads one row's 16 flags with a single access and a ballot spreads them (kFlagsBallot); shorter rows
-// take an access a step (kFlagsLane).
-enum FlagMode { kFlagsNone = 0, kFlagsBallot = 1, kFlagsLane = 2 };
-constexpr uint32_t kBallotRow = 21;
+// quarter of the lanes reads one row's 16 flags with a single access and a ballot spreads them (kFlags4).  Up to 16 rows (5 lanes and more)
+// take four such accesses of 4 steps (kFlags16), still shorter rows one a step in every lane (kFlagsLane).
+enum FlagMode { kFlagsNone = 0, kFlags4 = 1, kFlags16 = 2, kFlagsLane = 3 };
 
 struct ScanParams {
   uint64_t T;
@@ -89,29 +88,49 @@ struct ScanParams {
 };
 
 // The done flags that cut the state ahead of the n steps i, i + 1, .. of a wave's run; a flag ahead of the first step (index -1, forward
-// in time) or past the run cuts nothing.  kFlagsBallot reads with the run's other loads, long before bits() asks.
+// in time) or past the run cuts nothing.  What ballots spread is read with the run's other loads, long before bits() asks.
 struct Flags {
-  uint8_t d = 0;
+  uint8_t d[4] = {0, 0, 0, 0};
   bool any = false;
+  static __device__ __forceinline__ uint8_t at(const ScanParams& p, uint32_t row, uint64_t i, int s, int n) {
+    const uint64_t flag = i + s + (int64_t)p.cut_off;
+    return s < n && flag < p.T && row < p.rows ? p.done[(int64_t)row * p.done_row + (int64_t)flag * p.done_step] : 0;
+  }
   __device__ __forceinline__ Flags(const ScanParams& p, uint32_t e0, int lane, uint64_t i, int n) {
-    if (p.flags != kFlagsBallot) return;
-    const uint32_t row = e0 + (lane >> 4);
-    const uint64_t flag = i + (lane & 15) + (int64_t)p.cut_off;
-    if ((lane & 15) < n && flag < p.T && row < p.rows) d = p.done[(int64_t)row * p.done_row + (int64_t)flag * p.done_step];
+    if (p.flags == kFlags4) {
+      d[0] = at(p, e0 + (lane >> 4), i, lane & 15, n);
+    } else if (p.flags == kFlags16) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) d[j] = at(p, e0 + (lane >> 2), i, 4 * j + (lane & 3), n);
+    }
   }
   __device__ __forceinline__ uint32_t bits(const ScanParams& p, uint32_t e, uint32_t e0, uint64_t i, int n) {
     uint32_t cut = 0;
-    if (p.flags == kFlagsBallot) {
-      const uint64_t m = __ballot(d != 0);
+    if (p.flags == kFlags4) {
+      const uint64_t m = __ballot(d[0] != 0);
       any = m != 0;
       cut = (uint32_t)(m >> ((e - e0) * 16)) & 0xffffu;
-    } else if (p.flags == kFlagsLane && n > 0) {
-      const uint8_t* row = p.done + (int64_t)e * p.done_row;
+    } else if (p.flags == kFlags16) {
 #pragma unroll
-      for (int s = 0; s < 16; ++s) {
-        const uint64_t flag = i + (s < n ? s : 0) + (int64_t)p.cut_off, at = flag < p.T ? flag : 0;
-        cut |= (row[(int64_t)at * p.done_step] != 0 && flag < p.T && s < n ? 1u : 0u) << s;
+      for (int j = 0; j < 4; ++j) {
+        const uint64_t m = __ballot(d[j] != 0);
+        any |= m != 0;
+        cut |= ((uint32_t)(m >> ((e - e0) * 4)) & 0xfu) << (4 * j);
       }
+    } else if (p.flags == kFlagsLane && n > 0) {
+      const uint64_t row = (uint64_t)(p.done + (int64_t)e * p.done_row);
+      uint8_t f[16];
+#pragma unroll
+      for (int s = 0; s < 16; ++s) {  // which flag is the same for the whole wave: one that does not count is another's, and dropped below
+        const uint64_t flag = i + (s < n ? s : 0) + (int64_t)p.cut_off;
+        uint64_t off = (flag < p.T ? flag : 0) * (uint64_t)p.done_step;
+        hold(off);
+        f[s] = *(const CP_GLOBAL uint8_t*)(row + off);
+      }
+#pragma unroll
+      for (int s = 0; s < 16; ++s) cut |= (f[s] != 0 ? 1u : 0u) << s;
+      const uint32_t ahead = i + (int64_t)p.cut_off < p.T ? 0u : 1u;  // the flag ahead of the first step
+      cut &= ((1u << n) - 1u) & ~ahead;
       any = __any(cut != 0);
     }
     return cut;
