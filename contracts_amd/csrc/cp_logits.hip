@@ -201,7 +201,7 @@ template <class X, class O, class K> __global__ __launch_bounds__(kBlock) void k
 }
 
 // ---- short rows -----------------------------------------------------------------------------------------------------------------
-// G rows (a power of two) of V <= kTile / G scores each; dense rows are one run of memory, 8 scores a lane whatever row they are of.
+// G rows (a power of two) of V < 512 scores each, G V <= kTile; dense rows are one run of memory, 8 scores a lane whatever row they are of.
 template <class X, class O, class K> __global__ __launch_bounds__(kBlock) void k_logits_rows(ce_logits s, uint32_t G, uint32_t shift, int dense) {
   __shared__ __attribute__((aligned(16))) uint32_t table[kTile];
   __shared__ Row rows[kRowsMost];
@@ -262,8 +262,10 @@ template <class X, class O, class K> __global__ __launch_bounds__(kBlock) void k
 }
 
 template <class X, class O, class K> static void shapes(const ce_logits& s, hipStream_t st) {
-  // Half a tile and longer a row is worth blocks of its own; below, a block takes as many rows as fit.
-  if (s.vocab > kTile / 2) {
+  // A row is worth blocks of its own where it is long or there are no more of them than blocks in flight (8 a CU); otherwise a block takes as many rows
+  // as fit and leave 1024 blocks.  us, own blocks against packed: 4.7 / 8.2 at 1000 x 32 float, 6.9 / 13.6 at 2048 x 600, 32.6 / 35.7 at 20000 x 512
+  // bfloat16; 20.9 / 15.5 at 8192 x 300 float, 94 / 19 at 65536 x 64.  Packed, 131072 x 8: 9.4 with 1024 blocks, 10.2 with 512, 13.9 with 2048.
+  if (s.vocab >= 512 || s.rows <= 2048) {
     const uint32_t runs = (uint32_t)((s.vocab + kTile - 1) / kTile);
     const uint64_t most = (1u << 23) / runs;  // rows of a launch: fewer than 2^32 threads
     for (uint64_t r = 0; r < s.rows; r += most)
@@ -271,7 +273,7 @@ template <class X, class O, class K> static void shapes(const ce_logits& s, hipS
     return;
   }
   uint32_t shift = 0;
-  while ((2ull << shift) * s.vocab <= kTile && (2u << shift) <= kRowsMost && (s.rows >> shift) > 512) ++shift;
+  while ((2ull << shift) * s.vocab <= kTile && (2u << shift) <= kRowsMost && (s.rows >> shift) > 1024) ++shift;
   const uint32_t G = 1u << shift;
   const int dense = s.logits_row == (int64_t)s.vocab && s.out_row == (int64_t)s.vocab;
   k_logits_rows<X, O, K><<<(uint32_t)((s.rows + G - 1) / G), kBlock, 0, st>>>(s, G, shift, dense);
