@@ -43,6 +43,11 @@ template <class T = void> T* ptr(const Maybe& t) { return t ? ptr<T>(*t) : nullp
 Tensor bytes(uint64_t n, const Tensor& like) { return n ? at::empty({(int64_t)n}, like.options().dtype(at::kByte)) : Tensor(); }
 void* stream_of(const Tensor& t) { return c10::hip::getCurrentHIPStream(t.get_device()).stream(); }
 
+// A tensor of the caller's that a call wrote to: a graph that had saved it finds out, as after torch's own in-place operations.
+void written(const Maybe& t) {
+  if (t && !t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
+}
+
 // Gradients of these gradients do not exist: whoever asks for one is told so (and nobody else).
 variable_list once(variable_list grads) {
   if (!at::GradMode::is_enabled()) return grads;
@@ -139,6 +144,8 @@ std::tuple<Tensor, Tensor> linear_scan(const Tensor& x, const Maybe& gate, doubl
   }
   Tensor y = out.value_or(Tensor()), last = state_out.value_or(Tensor());
   scan_forward(x, gate.value_or(Tensor()), decay, state.value_or(Tensor()), done.value_or(Tensor()), reverse, y, last, nullptr);
+  written(out);
+  written(state_out);
   return {y, last};
 }
 
@@ -166,6 +173,8 @@ std::tuple<Tensor, Tensor> advantages(const Tensor& reward, const Tensor& value,
   a.advantage = ptr<float>(adv);
   a.ret = ptr<float>(ret);
   check(ce_advantages(&a, stream_of(reward)), "advantages");
+  written(adv_out);
+  written(ret_out);
   return {adv, ret};
 }
 
@@ -262,6 +271,7 @@ Tensor process_logits(const Tensor& logits, const Maybe& bias, const Maybe& toke
   if (grad) return Logits::apply(logits, bias, h);
   const Tensor to = out ? *out : at::empty(logits.sizes(), logits.options());
   logits_forward(logits, bias.value_or(none), h, to);
+  written(out);
   return to;
 }
 

@@ -222,6 +222,16 @@ def test_scan_gradient_against_differences(ops):
                 assert abs(up - down - d[i].item()) <= 1e-5 * (1 + abs(d[i].item())) * 8
 
 
+def test_writing_to_a_saved_tensor_is_found_out(ops):
+    for write in (lambda t: ops.process_logits(t, out=t, repetition=2.0), lambda t: ops.linear_scan(torch.zeros((1, 3, 4), device="cuda"), 0.5, state=t, state_out=t),
+                  lambda t: ops.linear_scan(torch.zeros((1, 3, 4), device="cuda"), 0.5, out=t.view(1, 3, 4)),
+                  lambda t: ops.advantages(torch.zeros((1, 3, 4), device="cuda"), torch.zeros((1, 3, 4), device="cuda"), out=(t.view(1, 3, 4), torch.empty((1, 3, 4), device="cuda")))):
+        kept = torch.randn((3, 4), device="cuda").requires_grad_(True).exp()  # exp's backward pass needs its result
+        write(kept.detach())
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            kept.sum().backward()
+
+
 def test_gradients_of_gradients_are_refused_not_wrong(ops):
     x, gate, state, done = scan_inputs(7, 2, 4, 2, F32, F32, 4)
     leaf = x.clone().requires_grad_(True)
