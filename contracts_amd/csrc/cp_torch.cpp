@@ -1,12 +1,16 @@
 // cp_torch.cpp — the policy operators (include/contracts_policy.h) for torch tensors: allocates outputs and scratch memory, describes the tensors
 // to the C-ABI, and takes gradients through nodes that need no interpreter.
 //
-// Host-side marshalling only, because a call's latency is the host's: a forward call took 11-14 us through ctypes, of which the
-// launch is 3, and a forward and backward pass 120 us, most of it the interpreter in torch's backward thread.  What is checked about the
-// arguments lies in policy_ops.py and, for everything that reaches the device, in the C-ABI itself.
+// Host-side marshalling and the checks of arguments, because a call's latency is the host's: a forward call took 11-14 us through Python and
+// ctypes, of which the launch is 3, and a forward and backward pass 120 us, most of it the interpreter in torch's backward thread.  What
+// reaches the device is checked by the C-ABI once more.  policy_ops.py documents the calls.
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/python_variable.h>
 #include <torch/extension.h>
+#include <ATen/TensorUtils.h>
+
+#include <sstream>
 
 #include "../../include/contracts_policy.h"
 
@@ -24,6 +28,44 @@ void check(int rc, const char* what) {
   if (rc == CE_OK) return;
   const char* name = rc == CE_EINVAL ? "CE_EINVAL" : rc == CE_ENODEV ? "CE_ENODEV" : "?";
   throw Refused(std::string(what) + " failed: " + name + " (" + std::to_string(rc) + ") " + ce_policy_error());
+}
+
+// ---- refusals: ValueError, as the engine's Python layer raises -------------------------------------------------------------------
+template <class... A> [[noreturn]] void bad(const A&... parts) {
+  std::ostringstream text;
+  (text << ... << parts);
+  throw py::value_error(text.str());
+}
+double number(const py::object& o) {
+  const double v = PyFloat_AsDouble(o.ptr());
+  if (v == -1 && PyErr_Occurred()) throw py::error_already_set();
+  return v;
+}
+bool real(at::ScalarType t) { return t == at::kFloat || t == at::kBFloat16 || t == at::kHalf; }
+bool flag(at::ScalarType t) { return t == at::kBool || t == at::kByte; }
+void on_gpu(const char* op, const Tensor& t) {
+  if (!t.is_cuda()) bad(op, ": tensors must live on a GPU (there is no CPU path), got ", t.device());
+}
+void same_device(const char* op, const Tensor& first, std::initializer_list<const Maybe*> rest) {
+  for (const Maybe* t : rest)
+    if (*t && (*t)->device() != first.device()) bad(op, ": all tensors must live on one device");
+}
+// The bytes a tensor reaches.
+std::pair<const char*, const char*> span(const Tensor& t) {
+  int64_t n = 1;
+  for (int64_t d = 0; d < t.dim(); ++d) n += (t.size(d) - 1) * t.stride(d);
+  const char* lo = (const char*)t.data_ptr();
+  return {lo, lo + n * t.element_size()};
+}
+// An output may not overlap an input.
+void apart(const char* op, const Maybe& out, const char* name, std::initializer_list<const Maybe*> inputs) {
+  if (!out || out->numel() == 0) return;
+  const auto o = span(*out);
+  for (const Maybe* t : inputs)
+    if (*t && (*t)->defined() && (*t)->numel()) {
+      const auto i = span(**t);
+      if (o.second > i.first && i.second > o.first) bad(op, ": ", name, " overlaps an input");
+    }
 }
 
 uint32_t code(const Tensor& t) {
@@ -137,8 +179,53 @@ struct Scan : torch::autograd::Function<Scan> {
   }
 };
 
-std::tuple<Tensor, Tensor> linear_scan(const Tensor& x, const Maybe& gate, double decay, const Maybe& state, const Maybe& done, bool reverse, const Maybe& out, const Maybe& state_out, bool grad) {
+std::tuple<Tensor, Tensor> linear_scan(Tensor x, const py::object& gate_or_decay, Maybe state, const Maybe& done, bool reverse, const Maybe& out, const Maybe& state_out) {
+  const char* op = "linear_scan";
+  if (x.dim() != 3) bad("linear_scan: x must be [T, E, C]");
+  on_gpu(op, x);
+  Maybe gate;
+  double decay = 0;
+  if (THPVariable_Check(gate_or_decay.ptr())) gate = THPVariable_Unpack(gate_or_decay.ptr());
+  else decay = number(gate_or_decay);
+  same_device(op, x, {&gate, &state, &done, &out, &state_out});
+  const auto type = x.scalar_type();
+  const bool twice = type == at::kDouble;
+  if (!real(type) && !twice) bad("linear_scan: x must be float32, bfloat16, float16 or float64, not ", type);
+  const int64_t T = x.size(0), E = x.size(1), C = x.size(2);
+  const auto acc = twice ? at::kDouble : at::kFloat;
+  bool grad = x.requires_grad();
+  int64_t head = 1;
+  if (gate) {
+    const int64_t H = gate->dim() == 3 ? gate->size(2) : -1;
+    if (H < 0 || gate->size(0) != T || gate->size(1) != E || !(H == C || (H && C % H == 0)))
+      bad("linear_scan: gate must be [T, E, H] with H dividing C, got ", gate->sizes(), " for x ", x.sizes());
+    if (gate->scalar_type() != type && (gate->scalar_type() != at::kFloat || twice)) bad("linear_scan: gate must be of x's type or float32, not ", gate->scalar_type());
+    grad |= gate->requires_grad();
+    if (H) head = C / H;
+  }
+  // rows that far apart are more than a wave's 32-bit offsets, unless rows are whole waves
+  const int64_t far = C % 256 == 0 && (head & (head - 1)) == 0 ? INT64_MAX : ((int64_t)1 << 28) / (255 / C + 1);
+  if (gate && ((gate->stride(2) != 1 && gate->size(2) > 1) || gate->stride(1) >= far)) gate = gate->contiguous();
+  if ((x.stride(2) != 1 && C > 1) || x.stride(1) >= far) x = x.contiguous();
+  if (state) {
+    if (state->dim() != 2 || state->size(0) != E || state->size(1) != C || state->scalar_type() != acc) bad("linear_scan: state must be ", acc, " [", E, ", ", C, "]");
+    grad |= state->requires_grad();
+  }
+  if (done && (done->dim() != 2 || done->size(0) != T || done->size(1) != E || !flag(done->scalar_type()))) bad("linear_scan: done must be bool or uint8 [T, E]");
+  grad = grad && at::GradMode::is_enabled();
+  if (out || state_out) {
+    if (grad) bad("linear_scan: out and state_out cannot be given where gradients are wanted");
+    if (out && (out->sizes() != x.sizes() || out->scalar_type() != type || !out->is_contiguous())) bad("linear_scan: out must be a dense ", type, " ", x.sizes());
+    if (state_out && (state_out->dim() != 2 || state_out->size(0) != E || state_out->size(1) != C || state_out->scalar_type() != acc || !state_out->is_contiguous()))
+      bad("linear_scan: state_out must be a dense ", acc, " [", E, ", ", C, "]");
+    const bool moved = state && state->is_contiguous() && state_out && state_out->data_ptr() == state->data_ptr();  // in place
+    const Maybe none, mx = x;
+    apart(op, out, "out", {&state, &state_out, &mx, &gate, &done});
+    apart(op, state_out, "state_out", {moved ? &none : &state, &mx, &gate, &done});
+  }
+  if (state && !state->is_contiguous()) state = state->contiguous();
   if (grad) {
+    if (twice) bad("linear_scan: float64 has no backward pass");
     variable_list r = Scan::apply(x, gate, decay, state, done, reverse);
     return {r[0], r[1]};
   }
@@ -150,8 +237,35 @@ std::tuple<Tensor, Tensor> linear_scan(const Tensor& x, const Maybe& gate, doubl
 }
 
 // ---- advantages -----------------------------------------------------------------------------------------------------------------
-std::tuple<Tensor, Tensor> advantages(const Tensor& reward, const Tensor& value, const Maybe& last_value, const Maybe& done, double gamma, double lam, int64_t first, const Maybe& adv_out,
-                                      const Maybe& ret_out) {
+std::tuple<Tensor, Tensor> advantages(Tensor reward, Tensor value, Maybe last_value, Maybe done, double gamma, double lam, int64_t first, const std::optional<std::pair<Tensor, Tensor>>& out) {
+  const char* op = "advantages";
+  if (reward.dim() != 3) bad("advantages: reward must be [P, E, n]");
+  on_gpu(op, reward);
+  Maybe adv_out, ret_out;
+  if (out) adv_out = out->first, ret_out = out->second;
+  const Maybe mv = value;
+  same_device(op, reward, {&mv, &last_value, &done, &adv_out, &ret_out});
+  const int64_t P = reward.size(0), E = reward.size(1), n = reward.size(2);
+  if (reward.scalar_type() != at::kDouble && reward.scalar_type() != at::kFloat) bad("advantages: reward must be float64 or float32, not ", reward.scalar_type());
+  if (value.sizes() != reward.sizes() || !real(value.scalar_type())) bad("advantages: value must be float32, bfloat16 or float16 ", reward.sizes());
+  if (last_value) {
+    if (last_value->sizes() != reward.sizes().slice(1) || last_value->scalar_type() != value.scalar_type()) bad("advantages: last_value must be ", value.scalar_type(), " [", E, ", ", n, "]");
+    last_value = last_value->contiguous();
+  }
+  if (done) {
+    if (done->sizes() != reward.sizes().slice(0, done->dim() == 3 ? 3 : 2) || !flag(done->scalar_type())) bad("advantages: done must be bool or uint8 [P, E] or [P, E, n]");
+    done = done->contiguous();
+  }
+  if (first < 0 || first >= std::max<int64_t>(P, 1)) bad("advantages: first_plane out of range");
+  reward = reward.contiguous();
+  value = value.contiguous();
+  if (out) {
+    for (const Maybe* t : {&adv_out, &ret_out})
+      if ((*t)->sizes() != reward.sizes() || (*t)->scalar_type() != at::kFloat || !(*t)->is_contiguous()) bad("advantages: out must be two dense float32 ", reward.sizes());
+    const Maybe mr = reward, mw = value;
+    apart(op, adv_out, "out", {&mr, &mw, &last_value, &done, &ret_out});
+    apart(op, ret_out, "out", {&mr, &mw, &last_value, &done});
+  }
   const auto f32 = reward.options().dtype(at::kFloat);
   const Tensor adv = adv_out ? *adv_out : at::empty(reward.sizes(), f32), ret = ret_out ? *ret_out : at::empty(reward.sizes(), f32);
   ce_advantage a = {};
@@ -263,16 +377,101 @@ struct Logits : torch::autograd::Function<Logits> {
   }
 };
 
-Tensor process_logits(const Tensor& logits, const Maybe& bias, const Maybe& tokens, const Maybe& lengths, const Maybe& prompt_lengths, const Maybe& mask, const Maybe& mask_index,
-                      const Maybe& repetition, const Maybe& presence, const Maybe& frequency, double repetition_all, double presence_all, double frequency_all, const Maybe& out, bool grad) {
+// A [.., width] table whose rows repeat over the logits' rows, as a dense [B, width].
+Tensor table(const char* name, const Tensor& t, at::IntArrayRef lead, int64_t width) {
+  const int64_t k = t.dim() - 1;
+  if (k < 0 || t.size(k) != width) bad("process_logits: ", name, " must end in ", width, " entries, got ", t.sizes());
+  const auto axes = t.sizes().slice(0, k);
+  const bool fits = k == 0 || (k == 1 && (lead.size() <= 1 || axes[0] == 1)) || (k <= (int64_t)lead.size() && axes == lead.slice(lead.size() - k));
+  if (!fits) bad("process_logits: ", name, "'s leading axes ", axes, " must be the last of the logits' ", lead);
+  return k == 1 ? t.contiguous() : t.reshape({c10::multiply_integers(axes), width}).contiguous();
+}
+// One entry a row, dense, in `type` (int64 is narrowed; what does not fit keeps its meaning: past every end, or before every start).
+Maybe per_row(const char* name, const Maybe& t, at::IntArrayRef lead, at::ScalarType type) {
+  if (!t) return t;
+  if (t->sizes() != lead) bad("process_logits: ", name, " must hold one entry a row, ", lead, ", got ", t->sizes());
+  if (t->scalar_type() == type) return t->contiguous();
+  if (type != at::kInt || t->scalar_type() != at::kLong) bad("process_logits: ", name, " must be ", type, ", not ", t->scalar_type());
+  return t->clamp(-1, INT32_MAX).to(at::kInt).contiguous();
+}
+
+Tensor process_logits(const Tensor& logits, Maybe tokens, Maybe lengths, Maybe prompt_lengths, const py::object& repetition, const py::object& presence, const py::object& frequency, Maybe bias, Maybe mask,
+                      Maybe mask_index, const Maybe& out) {
+  const char* op = "process_logits";
+  if (logits.dim() < 1) bad("process_logits: logits must be [..., V]");
+  if (!real(logits.scalar_type())) bad("process_logits: logits must be float32, bfloat16 or float16, not ", logits.scalar_type());
+  on_gpu(op, logits);
+  const char* names[3] = {"repetition", "presence", "frequency"};
+  const py::object* given[3] = {&repetition, &presence, &frequency};
+  Maybe penalty[3];
+  Shaping h = {{}, {}, {}, {}, {}, {}, {1, 0, 0}};
+  for (int k = 0; k < 3; ++k) {
+    if (THPVariable_Check(given[k]->ptr())) penalty[k] = THPVariable_Unpack(given[k]->ptr());
+    else h.scalar[k] = number(*given[k]);
+  }
+  same_device(op, logits, {&tokens, &lengths, &prompt_lengths, &penalty[0], &penalty[1], &penalty[2], &bias, &mask, &mask_index, &out});
+  const auto lead = logits.sizes().slice(0, logits.dim() - 1);
+  const int64_t V = logits.size(-1), rows = c10::multiply_integers(lead);
+  for (int k = 0; k < 3; ++k)
+    if (penalty[k]) {
+      if (penalty[k]->requires_grad() && at::GradMode::is_enabled()) bad("process_logits: ", names[k], " has no gradient here: detach it");
+      penalty[k] = per_row(names[k], penalty[k], lead, at::kFloat);
+    }
+  if (tokens) {
+    if (tokens->dim() != logits.dim() || tokens->sizes().slice(0, tokens->dim() - 1) != lead) bad("process_logits: tokens must be ", lead, " + [L], got ", tokens->sizes());
+    const auto t = tokens->scalar_type();
+    if (t != at::kByte && t != at::kInt && t != at::kLong) bad("process_logits: tokens must be uint8, int32 or int64, not ", t);
+    if (tokens->dim() != 2) tokens = tokens->reshape({rows, tokens->size(-1)});
+    lengths = per_row("lengths", lengths, lead, at::kInt);
+    prompt_lengths = per_row("prompt_lengths", prompt_lengths, lead, at::kInt);
+  } else if (lengths || prompt_lengths) {
+    bad("process_logits: lengths without tokens");
+  }
+  if (mask) {
+    const auto t = mask->scalar_type();
+    if (!flag(t) && t != at::kInt) bad("process_logits: mask must be bool, uint8 or int32 words, not ", t);
+    if (mask_index && mask->dim() != 2) bad("process_logits: an indexed mask must be a table [S, ..]");
+    mask_index = per_row("mask_index", mask_index, lead, at::kInt);
+    mask = table("mask", *mask, mask_index ? at::IntArrayRef() : lead, t == at::kInt ? (V + 31) / 32 : V);
+  } else if (mask_index) {
+    bad("process_logits: mask_index without a mask");
+  }
+  bool grad = logits.requires_grad();
+  if (bias) {
+    if (bias->scalar_type() != at::kFloat && bias->scalar_type() != logits.scalar_type()) bad("process_logits: bias must be float32 or of the logits' type, not ", bias->scalar_type());
+    bias = table("bias", *bias, lead, V);
+    grad |= bias->requires_grad();
+  }
+  grad = grad && at::GradMode::is_enabled();
+  if (grad && out) bad("process_logits: out cannot be given where gradients are wanted");
+  Tensor flat = logits.dim() == 2 ? logits : logits.reshape({rows, V});
+  if (V > 1 && flat.stride(1) != 1) flat = flat.contiguous();
   const Tensor none;
-  const Shaping h = {tokens.value_or(none), lengths.value_or(none), prompt_lengths.value_or(none), mask.value_or(none), mask_index.value_or(none),
-                     {repetition.value_or(none), presence.value_or(none), frequency.value_or(none)}, {repetition_all, presence_all, frequency_all}};
-  if (grad) return Logits::apply(logits, bias, h);
-  const Tensor to = out ? *out : at::empty(logits.sizes(), logits.options());
-  logits_forward(logits, bias.value_or(none), h, to);
-  written(out);
-  return to;
+  h.tokens = tokens.value_or(none);
+  h.lengths = lengths.value_or(none);
+  h.prompt_lengths = prompt_lengths.value_or(none);
+  h.mask = mask.value_or(none);
+  h.mask_index = mask_index.value_or(none);
+  for (int k = 0; k < 3; ++k) h.penalty[k] = penalty[k].value_or(none);
+  Tensor z;
+  if (grad) {
+    z = Logits::apply(flat, bias, h);
+  } else if (!out) {
+    z = at::empty({rows, V}, logits.options());
+    logits_forward(flat, bias.value_or(none), h, z);
+  } else {
+    if (out->sizes() != logits.sizes() || (out->scalar_type() != at::kFloat && out->scalar_type() != logits.scalar_type()))
+      bad("process_logits: out must be ", logits.sizes(), ", float32 or of the logits' type");
+    const auto strides = at::detail::computeStride(out->sizes(), out->strides(), at::DimVector{rows, V});
+    if (!strides || (V > 1 && (*strides)[1] != 1)) bad("process_logits: out's leading axes must collapse into one stride, its last be dense");
+    const Maybe to = out->view({rows, V}), nothing, mf = flat;
+    const bool same = to->data_ptr() == flat.data_ptr() && to->scalar_type() == flat.scalar_type() && to->strides() == flat.strides();
+    apart(op, to, "out", {same ? &nothing : &mf, &tokens, &lengths, &prompt_lengths, &mask, &mask_index, &bias, &penalty[0], &penalty[1], &penalty[2]});
+    logits_forward(flat, bias.value_or(none), h, *to);
+    written(out);
+    return *out;
+  }
+  return logits.dim() == 2 ? z : z.view(logits.sizes());
 }
 
 }  // namespace

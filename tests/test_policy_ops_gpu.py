@@ -565,6 +565,25 @@ def test_logits_gradient_against_differences(ops):
             assert abs((up - down) / 0.5 - d[i].item()) <= 1e-5 * (1 + abs(d[i].item()))
 
 
+def test_arguments_of_other_kinds(ops):
+    """No tensor where one belongs, no number where one belongs: TypeError; nothing to write, whatever its axes: no launch and no refusal"""
+    x, r = torch.zeros((4, 3, 6), device="cuda"), torch.zeros((4, 3, 2), device="cuda")
+    for call in (lambda: ops.linear_scan(x, "half"), lambda: ops.linear_scan(x, None), lambda: ops.linear_scan([1.0], 0.5), lambda: ops.linear_scan(x, 0.5, state=0.0),
+                 lambda: ops.advantages(r, None), lambda: ops.advantages(r, r, out=r), lambda: ops.advantages(r, r, first_plane=0.5),
+                 lambda: ops.process_logits(None), lambda: ops.process_logits(x, repetition="two"), lambda: ops.process_logits(x, mask=[True])):
+        with pytest.raises(TypeError):
+            call()
+    import numpy as np
+    assert ops.linear_scan(x + 1, np.float32(0.5))[0].equal(ops.linear_scan(x + 1, 0.5)[0])
+    for shape in ((0, 3, 5), (2, 0, 5), (2, 3, 0), (0,), (0, 5)):
+        out = torch.empty(shape, device="cuda")
+        assert ops.process_logits(torch.empty(shape, device="cuda"), out=out) is out
+    for shape in ((0, 3, 5), (2, 0, 5), (2, 3, 0)):
+        out = torch.empty(shape, device="cuda"), torch.empty(shape, device="cuda")
+        assert ops.linear_scan(torch.empty(shape, device="cuda"), 0.5, out=out[0])[0] is out[0]
+        assert ops.advantages(torch.empty(shape, device="cuda"), torch.empty(shape, device="cuda"), out=out)[1] is out[1]
+
+
 def test_logits_empty_and_refusals(ops):
     l = torch.randn((6, 10), device="cuda")
     tok = torch.zeros((6, 4), dtype=torch.int32, device="cuda")
