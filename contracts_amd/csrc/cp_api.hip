@@ -328,6 +328,7 @@ extern "C" int ce_process_logits(const ce_logits* s, void* stream) {
   if (int rc = check_logits(s)) return rc;
   if (s->rows * s->vocab == 0) return CE_OK;
   if (!s->out) return refuse("process_logits: null output");
+  if (s->rows > 1 && s->out_row < (int64_t)s->vocab && s->out_row > -(int64_t)s->vocab) return refuse("process_logits: the output's rows overlap");
   if (s->out == s->logits && (s->out_dtype != s->dtype || s->out_row != s->logits_row)) return refuse("process_logits: in place needs one type and one stride");
   OnDevice dev(s->device);
   if (dev.err != hipSuccess) return launched(dev.err, "process_logits: device");

@@ -32,7 +32,7 @@ template <class X, class G, int MODE, int VEC, int W, bool REDUCE> __global__ __
     const uint32_t g = group0 + own < groups && own < (p.in_wave ? p.in_wave : 1) ? group0 + own : group0;
     e = g / p.heads;
     head = g - e * p.heads;
-    c = head * p.head + (live ? in * VEC : 0);
+    c = head * p.head + (live ? in : p.in_wave ? 0 : p.lanes - 1) * VEC;
   } else {
     const uint32_t slot = blockIdx.x * kWave + lane;
     live = slot < p.cols;
@@ -40,7 +40,8 @@ template <class X, class G, int MODE, int VEC, int W, bool REDUCE> __global__ __
     e = col / p.row_cols;
     c = (col - e * p.row_cols) * VEC;
   }
-  // lanes that are not live do what another one does and write the same; none lies ahead of the wave's first row e0, from which all count
+  // lanes that are not live do what another one of their wave does and write the same; none lies ahead of the wave's first row e0, from which all
+  // count
   const uint32_t e0 = __builtin_amdgcn_readfirstlane(e);
   const uint64_t EC = (uint64_t)p.cols * VEC, ch = (uint64_t)e * p.row_cols * VEC + c;
   // a lane's offsets from row e0

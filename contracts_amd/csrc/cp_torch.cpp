@@ -46,9 +46,18 @@ bool flag(at::ScalarType t) { return t == at::kBool || t == at::kByte; }
 void on_gpu(const char* op, const Tensor& t) {
   if (!t.is_cuda()) bad(op, ": tensors must live on a GPU (there is no CPU path), got ", t.device());
 }
+// All on one device, and numbers as they lie in memory: not a lazily negated view, not carrying a forward-mode derivative, which a call would drop.
 void same_device(const char* op, const Tensor& first, std::initializer_list<const Maybe*> rest) {
+  auto plain = [&](const Tensor& t) {
+    if (t.is_neg()) bad(op, ": a lazily negated view; call resolve_neg() on it");
+    if (t._fw_grad(0).defined()) bad(op, ": has no forward-mode derivative");
+  };
+  plain(first);
   for (const Maybe* t : rest)
-    if (*t && (*t)->device() != first.device()) bad(op, ": all tensors must live on one device");
+    if (*t) {
+      if ((*t)->device() != first.device()) bad(op, ": all tensors must live on one device");
+      plain(**t);
+    }
 }
 // The bytes a tensor reaches.
 std::pair<const char*, const char*> span(const Tensor& t) {

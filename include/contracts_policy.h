@@ -124,7 +124,7 @@ int ce_advantages(const ce_advantage* a, void* stream);
  * bias: [bias_rows][V] dense, float or the logits' type; row r takes row r mod bias_rows (bias_rows divides R).
  * mask: CE_U8 [mask_rows][V], nonzero = allowed, or CE_I32 [mask_rows][ceil(V / 32)], bit v % 32 of word v / 32.  Row r takes
  * row mask_index[r] — negative: everything is allowed; past the end: nothing is — or, without an index, row r mod mask_rows.
- * out: logits' type or CE_F32, [R][V] with row stride out_row; it may be `logits` itself (same type and stride). */
+ * out: logits' type or CE_F32, [R][V] with row stride out_row (rows do not overlap); it may be `logits` itself (same type and stride). */
 typedef struct ce_logits {
   uint32_t abi_version;
   int32_t device;

@@ -118,7 +118,8 @@ def _logits(**kw):
     (dict(tokens=FAKE, token_dtype=5, history=3, repetition_all=float("nan")), "positive"), (dict(tokens=FAKE, token_dtype=5, history=3, presence_all=float("inf")), "finite"),
     (dict(lengths=FAKE), "without tokens"), (dict(bias=FAKE, bias_dtype=1, bias_rows=1), "bias"), (dict(bias=FAKE, bias_dtype=0, bias_rows=4), "divide"),
     (dict(bias=FAKE, bias_dtype=0, bias_rows=0), "divide"), (dict(mask=FAKE, mask_dtype=0, mask_rows=1), "mask"), (dict(mask=FAKE, mask_dtype=4, mask_rows=5), "divide"),
-    (dict(mask=FAKE, mask_dtype=5, mask_rows=0, mask_index=FAKE), "mask_rows"), (dict(mask_index=FAKE), "without a mask"), (dict(logits_row=12), "in place")])
+    (dict(mask=FAKE, mask_dtype=5, mask_rows=0, mask_index=FAKE), "mask_rows"), (dict(mask_index=FAKE), "without a mask"), (dict(logits_row=12), "in place"),
+    (dict(out_row=9), "overlap"), (dict(out_row=0), "overlap"), (dict(out_row=-9), "overlap")])
 def test_logits_refusals(L, kw, word):
     s = _logits(**kw)
     assert L.ce_process_logits(C.byref(s), None) == EINVAL and word in L.ce_policy_error().decode()

@@ -584,6 +584,26 @@ def test_arguments_of_other_kinds(ops):
         assert ops.advantages(torch.empty(shape, device="cuda"), torch.empty(shape, device="cuda"), out=out)[1] is out[1]
 
 
+def test_tensors_that_hold_something_else_than_their_memory(ops):
+    """Rows of an output that share memory, lazily negated views, forward-mode derivatives: refused, not read as they lie"""
+    import torch.autograd.forward_ad as fwd
+
+    from contracts_amd._lib import EngineError
+    l, x, r = torch.randn((6, 10), device="cuda"), torch.randn((4, 3, 6), device="cuda"), torch.randn((4, 3, 2), device="cuda")
+    for out in (torch.zeros((1, 10), device="cuda").expand(6, 10), torch.zeros(64, device="cuda").as_strided((6, 10), (9, 1))):
+        with pytest.raises(EngineError, match="overlap"):
+            ops.process_logits(l, out=out)
+    neg = torch._neg_view
+    calls = [lambda f: ops.linear_scan(f(x), 0.5), lambda f: ops.linear_scan(x, f(x)), lambda f: ops.linear_scan(x, 0.5, state=f(x[0])), lambda f: ops.advantages(f(r), r),
+             lambda f: ops.advantages(r, f(r)), lambda f: ops.process_logits(f(l)), lambda f: ops.process_logits(l, bias=f(l[0]))]
+    for call in calls:
+        with pytest.raises(ValueError, match="negated"):
+            call(neg)
+        with fwd.dual_level(), pytest.raises(ValueError, match="forward-mode"):
+            call(lambda t: fwd.make_dual(t, torch.ones_like(t)))
+    assert ops.process_logits(neg(l).resolve_neg()).equal(-l)
+
+
 def test_logits_empty_and_refusals(ops):
     l = torch.randn((6, 10), device="cuda")
     tok = torch.zeros((6, 4), dtype=torch.int32, device="cuda")
