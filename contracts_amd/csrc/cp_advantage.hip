@@ -49,7 +49,7 @@ template <class R, class V, int W> __global__ __launch_bounds__(kWave * W) void 
         x[s] = (double)r[s] - now + (d[s] ? 0.0 : a.gamma * after);
         after = now;
         const double g = d[s] ? 0.0 : gl;
-        rp *= g;
+        rp = both(rp, g);
         rh = step(g, rh, x[s]);
       }
     double mine = h;

@@ -46,6 +46,8 @@ template <> __device__ __forceinline__ float step(float a, float h, float x) { r
 // A run of steps as a map of the state before it: h -> P h + H, P the product of its gates.  A zero state takes no part, so
 // that a product past the type's range (gates over 1) does not turn it into NaN.
 template <class A> __device__ __forceinline__ A apply(A P, A H, A h) { return h == A(0) ? H : step(P, h, H); }
+// The product of two such P: one of 0 forgets whatever the other is, past the type's range too (0 times infinity would be NaN).
+template <class A> __device__ __forceinline__ A both(A P, A Q) { return P == A(0) || Q == A(0) ? A(0) : P * Q; }
 
 // Done flags of a wave's run of 16 steps as 16 bits a lane.  A wave spans at most 4 rows where a row has 21 lanes or more: then each
 // quarter of the lanes reads one row's 16 flags with a single access and a ballot spreads them (kFlags4).  Up to 16 rows (5 lanes and more)

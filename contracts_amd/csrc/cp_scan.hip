@@ -54,7 +54,7 @@ template <class X, class G, int MODE, int VEC, int W, bool REDUCE> __global__ __
 #pragma unroll
       for (int v = 0; v < VEC; ++v) {
         cs[v] = apply(part[v], part[EC + v], cs[v]);
-        cp[v] *= part[v];
+        cp[v] = both(cp[v], part[v]);
       }
     }
 #pragma unroll
@@ -119,7 +119,7 @@ template <class X, class G, int MODE, int VEC, int W, bool REDUCE> __global__ __
 #pragma unroll
         for (int v = 0; v < VEC; ++v) {
           if (MODE == kGateHead && v > 0) rp[v] = rp[0];
-          bad |= !finite(rh[v]);
+          bad |= !finite(rh[v]) || !finite(rp[v]);
         }
         odd = __any(bad);
       }
@@ -131,7 +131,7 @@ template <class X, class G, int MODE, int VEC, int W, bool REDUCE> __global__ __
           if (s < n)
 #pragma unroll
             for (int v = 0; v < VEC; ++v) {
-              rp[v] *= (cut >> s) & 1 ? A(0) : gate_of(s, v);
+              rp[v] = both(rp[v], (cut >> s) & 1 ? A(0) : gate_of(s, v));
               rh[v] = careful(s, v, rh[v]);
             }
       }
@@ -146,7 +146,7 @@ template <class X, class G, int MODE, int VEC, int W, bool REDUCE> __global__ __
 #pragma unroll
         for (int v = 0; v < VEC; ++v) {
           h[v] = apply(fold[buf][k][0][v][lane], fold[buf][k][1][v][lane], h[v]);
-          if (REDUCE) P[v] *= fold[buf][k][0][v][lane];
+          if (REDUCE) P[v] = both(P[v], fold[buf][k][0][v][lane]);
         }
       }
       buf ^= W > 1;

@@ -77,7 +77,7 @@ template <class X, class G, int MODE, int VEC, int W, bool REDUCE> __global__ __
 #pragma unroll
       for (int v = 0; v < VEC; ++v) {
         cs[v] = apply(part[v], part[EC + v], cs[v]);
-        cp[v] *= part[v];
+        cp[v] = both(cp[v], part[v]);
       }
     }
 #pragma unroll
@@ -142,7 +142,7 @@ template <class X, class G, int MODE, int VEC, int W, bool REDUCE> __global__ __
 #pragma unroll
         for (int v = 0; v < VEC; ++v) {
           if (MODE == kGateHead && v > 0) rp[v] = rp[0];
-          bad |= !finite(rq[v]);
+          bad |= !finite(rq[v]) || !finite(rp[v]);
         }
         odd = __any(bad);
       }
@@ -155,7 +155,7 @@ template <class X, class G, int MODE, int VEC, int W, bool REDUCE> __global__ __
 #pragma unroll
             for (int v = 0; v < VEC; ++v) {
               const float a = cut_gate(s, v);
-              rp[v] *= a;
+              rp[v] = both(rp[v], a);
               rq[v] = a == 0.f ? 0.f : a * ((float)ty[s].v[v] + rq[v]);
             }
       }
@@ -170,7 +170,7 @@ template <class X, class G, int MODE, int VEC, int W, bool REDUCE> __global__ __
 #pragma unroll
         for (int v = 0; v < VEC; ++v) {
           R[v] = apply(fold[buf][k][0][v][lane], fold[buf][k][1][v][lane], R[v]);
-          if (REDUCE) P[v] *= fold[buf][k][0][v][lane];
+          if (REDUCE) P[v] = both(P[v], fold[buf][k][0][v][lane]);
         }
       }
       buf ^= W > 1;

@@ -37,7 +37,8 @@ const char* ce_policy_error(void);
  *   CE_SCAN_REVERSE:   h_t = a_t * k_t + x_t,  k_t = h_{t+1}, or 0 where done_t;      k_{T-1} = state (0 where done_{T-1});  last = h_0
  * so that an episode that ends with step t hands nothing over the border between t and t + 1 in either direction, and cutting
  * the time axis into calls (`last` of one is `state` of the next) changes nothing.  A gate of exactly 0 forgets the
- * state whatever it held (infinities and NaN included), as done does.  The state is carried in float (double for CE_F64); each
+ * state whatever it held (infinities and NaN included), as done does.  The product of the gates over any stretch of steps without a
+ * border has to stay in the state's range (a stretch is composed as a map h -> P h + H; a P under that range counts as 0).  The state is carried in float (double for CE_F64); each
  * y is rounded once to its own type and the rounded value is not used again.  T = 0 hands the state on.
  * Types: x and y dtype; gate dtype or CE_F32; state and last float (CE_F64: double throughout, and no backward pass).
  * gate == NULL: the constant `decay`.  state / done / last / saved may be NULL (zeros / none ended / not wanted).

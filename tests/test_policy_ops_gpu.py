@@ -138,6 +138,41 @@ def test_scan_forgets_what_done_or_a_zero_gate_closes_off(ops, T):
             assert bool((dx[other] == 0).all()) and bool((dx[keep] >= 1).all())
 
 
+@pytest.mark.parametrize("T", [40, 1400])
+def test_a_border_forgets_gates_whose_product_overflowed(ops, T):
+    """gates of 1e8 ahead of a border (their product, as the state, is past float's range) leave nothing behind it: not 0 times infinity"""
+    t = T // 2
+    for reverse in (False, True):
+        for by_gate in (False, True):
+            x, gate, state, done = scan_inputs(T, 2, 6, 6, F32, F32, 4, done=0)
+            done = torch.zeros((T, 2), dtype=torch.uint8, device="cuda")
+            first, behind = (slice(t + 1, t + 19), slice(0, t + 1)) if reverse else (slice(t - 17, t + 1), slice(t + 1, T))
+            gate[first] = 1e8
+            if by_gate:
+                gate[t if reverse else t + 1] = 0
+            else:
+                done[t] = 1
+            want = oracle.scan(x, gate, state, done, reverse)
+            y, last = ops.linear_scan(x, gate, state=state, done=done, reverse=reverse)
+            assert bool(torch.isfinite(y[behind]).all()) and bool(torch.isfinite(last).all())
+            oracle.close(y[behind], want["y"][behind], oracle.rounded(want["y"], want["ybound"], F32)[behind])
+            # the gradient runs the other way: gates of 1e8 on this side of the border, steps ahead of it on the other
+            x, gate, state, done = scan_inputs(T, 2, 6, 6, F32, F32, 5, done=0)
+            done = torch.zeros((T, 2), dtype=torch.uint8, device="cuda")
+            first, ahead = (slice(t - 17, t + 1), slice(t + 1, T)) if reverse else (slice(t + 1, t + 19), slice(0, t + 1))
+            gate[first], x[behind] = 1e8, 0  # the states there are 0
+            if by_gate:
+                gate[t if reverse else t + 1] = 0
+            else:
+                done[t] = 1
+            leaf = x.requires_grad_(True)
+            y, _ = ops.linear_scan(leaf, gate, state=state, done=done, reverse=reverse)
+            dx = torch.autograd.grad(y.sum(), leaf)[0]
+            f = oracle.scan(x, gate, state, done, reverse)
+            w = oracle.scan_grad(f, torch.ones_like(y), None, 6, reverse)
+            oracle.close(dx[ahead], w["dx"][ahead], oracle.rounded(w["dx"], w["dxbound"], F32)[ahead])
+
+
 def test_scan_gates_past_one_over_a_zero_state(ops):
     """products of gates leave float's range while the state is 0: the state stays 0, no NaN"""
     x = torch.zeros((2000, 1, 3), device="cuda")
