@@ -18,8 +18,8 @@ constexpr int kSteps = CE_SCAN_SAVED_STEPS;
 
 template <class X, class G, int MODE, int VEC, int W, bool REDUCE> __global__ __launch_bounds__(kWave * W) void k_scan(ScanParams p) {
   typedef typename AccOf<X>::type A;
-  constexpr int GV = MODE == kGateChannel ? VEC : 1;
-  __shared__ A fold[W > 1 ? 2 : 1][W][2][VEC][kWave];
+  constexpr int GV = MODE == kGateChannel ? VEC : 1;  // gates of a lane; its channels under one gate have one product P too
+  __shared__ A fold[W > 1 ? 2 : 1][W][GV + VEC][kWave];  // P, then H
   const int lane = threadIdx.x & 63, w = W > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : 0;
   const uint32_t col = blockIdx.x * kWave + lane;
   const uint32_t colc = col < p.cols ? col : p.cols - 1;  // lanes past the end do what the last one does, and write the same
@@ -45,30 +45,30 @@ template <class X, class G, int MODE, int VEC, int W, bool REDUCE> __global__ __
   if (!REDUCE && W > 1 && blockIdx.y > 0) {  // the chunks before this one: each wave composes its share of them, then all fold the shares
     const uint64_t EC = (uint64_t)p.cols * VEC;
     const uint32_t each = (blockIdx.y + W - 1) / W, k0 = w * each, k1 = k0 + each < blockIdx.y ? k0 + each : blockIdx.y;
-    A cp[VEC], cs[VEC];
+    A cp[GV], cs[VEC];
 #pragma unroll
-    for (int v = 0; v < VEC; ++v) cp[v] = A(1), cs[v] = A(0);
+    for (int v = 0; v < VEC; ++v) cp[v % GV] = A(1), cs[v] = A(0);
 #pragma unroll 8
     for (uint32_t k = k0; k < k1; ++k) {
       const A* part = (const A*)p.part + (uint64_t)k * 2 * EC + ch;
 #pragma unroll
       for (int v = 0; v < VEC; ++v) {
-        cs[v] = apply(part[v], part[EC + v], cs[v]);
-        cp[v] = both(cp[v], part[v]);
+        cs[v] = apply(part[v % GV], part[EC + v], cs[v]);
+        if (v < GV) cp[v] = both(cp[v], part[v]);
       }
     }
 #pragma unroll
-    for (int v = 0; v < VEC; ++v) fold[0][w][0][v][lane] = cp[v], fold[0][w][1][v][lane] = cs[v];
+    for (int v = 0; v < VEC; ++v) fold[0][w][v % GV][lane] = cp[v % GV], fold[0][w][GV + v][lane] = cs[v];
     __syncthreads();
 #pragma unroll
     for (int k = 0; k < W; ++k)
 #pragma unroll
-      for (int v = 0; v < VEC; ++v) h[v] = apply(fold[0][k][0][v][lane], fold[0][k][1][v][lane], h[v]);
+      for (int v = 0; v < VEC; ++v) h[v] = apply(fold[0][k][v % GV][lane], fold[0][k][GV + v][lane], h[v]);
     buf = 1;
   }
-  A P[VEC];  // REDUCE: the chunk's product so far
+  A P[GV];  // REDUCE: the chunk's product so far
 #pragma unroll
-  for (int v = 0; v < VEC; ++v) P[v] = A(1);
+  for (int v = 0; v < GV; ++v) P[v] = A(1);
 
   for (uint64_t tile = i0; tile < i1; tile += (uint64_t)W * kSteps) {
     const uint64_t i = tile + (uint64_t)w * kSteps;
@@ -103,40 +103,39 @@ template <class X, class G, int MODE, int VEC, int W, bool REDUCE> __global__ __
 #pragma unroll
     for (int v = 0; v < VEC; ++v) mine[v] = h[v];
     if (W > 1 || REDUCE) {
-      A rp[VEC], rh[VEC];
+      A rp[GV], rh[VEC];
 #pragma unroll
-      for (int v = 0; v < VEC; ++v) rp[v] = A(1), rh[v] = A(0);
+      for (int v = 0; v < VEC; ++v) rp[v % GV] = A(1), rh[v] = A(0);
       bool odd = !plain;
       if (plain) {
 #pragma unroll
         for (int s = 0; s < kSteps; ++s)
 #pragma unroll
           for (int v = 0; v < VEC; ++v) {
-            if (MODE != kGateHead || v == 0) rp[v] *= gate_of(s, v);
+            if (v < GV) rp[v] *= gate_of(s, v);
             rh[v] = fma_(gate_of(s, v), rh[v], A(tx[s].v[v]));
           }
         bool bad = false;
 #pragma unroll
         for (int v = 0; v < VEC; ++v) {
-          if (MODE == kGateHead && v > 0) rp[v] = rp[0];
-          bad |= !finite(rh[v]) || !finite(rp[v]);
+          bad |= !finite(rh[v]) || !finite(rp[v % GV]);
         }
         odd = __any(bad);
       }
       if (odd) {
 #pragma unroll
-        for (int v = 0; v < VEC; ++v) rp[v] = A(1), rh[v] = A(0);
+        for (int v = 0; v < VEC; ++v) rp[v % GV] = A(1), rh[v] = A(0);
 #pragma unroll
         for (int s = 0; s < kSteps; ++s)
           if (s < n)
 #pragma unroll
             for (int v = 0; v < VEC; ++v) {
-              rp[v] = both(rp[v], (cut >> s) & 1 ? A(0) : gate_of(s, v));
+              if (v < GV) rp[v] = both(rp[v], (cut >> s) & 1 ? A(0) : gate_of(s, v));
               rh[v] = careful(s, v, rh[v]);
             }
       }
 #pragma unroll
-      for (int v = 0; v < VEC; ++v) fold[buf][w][0][v][lane] = rp[v], fold[buf][w][1][v][lane] = rh[v];
+      for (int v = 0; v < VEC; ++v) fold[buf][w][v % GV][lane] = rp[v % GV], fold[buf][w][GV + v][lane] = rh[v];
       if (W > 1) __syncthreads();
 #pragma unroll
       for (int k = 0; k < W; ++k) {
@@ -145,8 +144,8 @@ template <class X, class G, int MODE, int VEC, int W, bool REDUCE> __global__ __
           for (int v = 0; v < VEC; ++v) mine[v] = h[v];
 #pragma unroll
         for (int v = 0; v < VEC; ++v) {
-          h[v] = apply(fold[buf][k][0][v][lane], fold[buf][k][1][v][lane], h[v]);
-          if (REDUCE) P[v] = both(P[v], fold[buf][k][0][v][lane]);
+          h[v] = apply(fold[buf][k][v % GV][lane], fold[buf][k][GV + v][lane], h[v]);
+          if (REDUCE && v < GV) P[v] = both(P[v], fold[buf][k][v][lane]);
         }
       }
       buf ^= W > 1;
@@ -203,7 +202,7 @@ template <class X, class G, int MODE, int VEC, int W, bool REDUCE> __global__ __
   if (REDUCE) {
     A* part = (A*)p.part + (uint64_t)blockIdx.y * 2 * p.cols * VEC + ch;
 #pragma unroll
-    for (int v = 0; v < VEC; ++v) part[v] = P[v], part[(uint64_t)p.cols * VEC + v] = h[v];
+    for (int v = 0; v < VEC; ++v) part[v] = P[v % GV], part[(uint64_t)p.cols * VEC + v] = h[v];
   } else if (p.last && blockIdx.y + 1 == gridDim.y) {
     // forward in time the flag of the last step closes the border behind it
     const bool cut = p.flags && p.cut_off < 0 && p.T > 0 && p.done[(int64_t)e * p.done_row + (int64_t)(p.T - 1) * p.done_step];

@@ -17,8 +17,8 @@ namespace cp {
 constexpr int kSteps = CE_SCAN_SAVED_STEPS;
 
 template <class X, class G, int MODE, int VEC, int W, bool REDUCE> __global__ __launch_bounds__(kWave * W) void k_scan_grad(ScanParams p) {
-  constexpr int GV = MODE == kGateChannel ? VEC : 1;
-  __shared__ float fold[W > 1 ? 2 : 1][W][2][VEC][kWave];
+  constexpr int GV = MODE == kGateChannel ? VEC : 1;  // gates of a lane; its channels under one gate have one product P too
+  __shared__ float fold[W > 1 ? 2 : 1][W][GV + VEC][kWave];  // P, then H
   // a run's terms of dgate, a row of lanes to a step; rows are 65 apart, so that lanes which add up different steps read different banks
   __shared__ float terms[MODE == kGateHead && !REDUCE ? W : 1][MODE == kGateHead && !REDUCE ? kSteps : 1][kWave + 1];
   const int lane = threadIdx.x & 63, w = W > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : 0;
@@ -56,9 +56,9 @@ template <class X, class G, int MODE, int VEC, int W, bool REDUCE> __global__ __
   const uint32_t chunk = blockIdx.y + (REDUCE ? 1 : 0);  // nobody folds chunk 0
   const uint64_t i0 = chunk * p.chunk, i1 = i0 + p.chunk < p.T ? i0 + p.chunk : p.T;
 
-  float R[VEC], P[VEC];
+  float R[VEC], P[GV];
 #pragma unroll
-  for (int v = 0; v < VEC; ++v) R[v] = 0.f, P[v] = 1.f;
+  for (int v = 0; v < VEC; ++v) R[v] = 0.f, P[v % GV] = 1.f;
   if (!REDUCE) {
     const bool cut = p.flags && p.cut_off < 0 && p.T > 0 && p.done[(int64_t)e * p.done_row + (int64_t)(p.T - 1) * p.done_step];
     if (p.dlast && !cut)
@@ -68,25 +68,25 @@ template <class X, class G, int MODE, int VEC, int W, bool REDUCE> __global__ __
   int buf = 0;
   if (!REDUCE && W > 1 && chunk + 1 < p.chunks) {  // the chunks behind this one, last first: each wave composes its share, then all fold the shares
     const uint32_t behind = p.chunks - 1 - chunk, each = (behind + W - 1) / W, k0 = w * each, k1 = k0 + each < behind ? k0 + each : behind;
-    float cp[VEC], cs[VEC];
+    float cp[GV], cs[VEC];
 #pragma unroll
-    for (int v = 0; v < VEC; ++v) cp[v] = 1.f, cs[v] = 0.f;
+    for (int v = 0; v < VEC; ++v) cp[v % GV] = 1.f, cs[v] = 0.f;
 #pragma unroll 8
     for (uint32_t k = k0; k < k1; ++k) {
       const float* part = (const float*)p.part + (uint64_t)(p.chunks - 2 - k) * 2 * EC + ch;  // of chunk chunks - 1 - k
 #pragma unroll
       for (int v = 0; v < VEC; ++v) {
-        cs[v] = apply(part[v], part[EC + v], cs[v]);
-        cp[v] = both(cp[v], part[v]);
+        cs[v] = apply(part[v % GV], part[EC + v], cs[v]);
+        if (v < GV) cp[v] = both(cp[v], part[v]);
       }
     }
 #pragma unroll
-    for (int v = 0; v < VEC; ++v) fold[0][w][0][v][lane] = cp[v], fold[0][w][1][v][lane] = cs[v];
+    for (int v = 0; v < VEC; ++v) fold[0][w][v % GV][lane] = cp[v % GV], fold[0][w][GV + v][lane] = cs[v];
     __syncthreads();
 #pragma unroll
     for (int k = 0; k < W; ++k)
 #pragma unroll
-      for (int v = 0; v < VEC; ++v) R[v] = apply(fold[0][k][0][v][lane], fold[0][k][1][v][lane], R[v]);
+      for (int v = 0; v < VEC; ++v) R[v] = apply(fold[0][k][v % GV][lane], fold[0][k][GV + v][lane], R[v]);
     buf = 1;
   }
 
@@ -126,41 +126,40 @@ template <class X, class G, int MODE, int VEC, int W, bool REDUCE> __global__ __
     for (int v = 0; v < VEC; ++v) mine[v] = R[v];
     // As in the forward pass: a quick walk that the careful one replaces where done cuts the run or a value is not finite.
     if (W > 1 || REDUCE) {
-      float rp[VEC], rq[VEC];
+      float rp[GV], rq[VEC];
 #pragma unroll
-      for (int v = 0; v < VEC; ++v) rp[v] = 1.f, rq[v] = 0.f;
+      for (int v = 0; v < VEC; ++v) rp[v % GV] = 1.f, rq[v] = 0.f;
       bool odd = !plain;
       if (plain) {
 #pragma unroll
         for (int s = kSteps - 1; s >= 0; --s)
 #pragma unroll
           for (int v = 0; v < VEC; ++v) {
-            if (MODE != kGateHead || v == 0) rp[v] *= gate_of(s, v);
+            if (v < GV) rp[v] *= gate_of(s, v);
             rq[v] = gate_of(s, v) * ((float)ty[s].v[v] + rq[v]);
           }
         bool bad = false;
 #pragma unroll
         for (int v = 0; v < VEC; ++v) {
-          if (MODE == kGateHead && v > 0) rp[v] = rp[0];
-          bad |= !finite(rq[v]) || !finite(rp[v]);
+          bad |= !finite(rq[v]) || !finite(rp[v % GV]);
         }
         odd = __any(bad);
       }
       if (odd) {
 #pragma unroll
-        for (int v = 0; v < VEC; ++v) rp[v] = 1.f, rq[v] = 0.f;
+        for (int v = 0; v < VEC; ++v) rp[v % GV] = 1.f, rq[v] = 0.f;
 #pragma unroll
         for (int s = kSteps - 1; s >= 0; --s)
           if (s < n)
 #pragma unroll
             for (int v = 0; v < VEC; ++v) {
               const float a = cut_gate(s, v);
-              rp[v] = both(rp[v], a);
+              if (v < GV) rp[v] = both(rp[v], a);
               rq[v] = a == 0.f ? 0.f : a * ((float)ty[s].v[v] + rq[v]);
             }
       }
 #pragma unroll
-      for (int v = 0; v < VEC; ++v) fold[buf][w][0][v][lane] = rp[v], fold[buf][w][1][v][lane] = rq[v];
+      for (int v = 0; v < VEC; ++v) fold[buf][w][v % GV][lane] = rp[v % GV], fold[buf][w][GV + v][lane] = rq[v];
       if (W > 1) __syncthreads();
 #pragma unroll
       for (int k = W - 1; k >= 0; --k) {
@@ -169,8 +168,8 @@ template <class X, class G, int MODE, int VEC, int W, bool REDUCE> __global__ __
           for (int v = 0; v < VEC; ++v) mine[v] = R[v];
 #pragma unroll
         for (int v = 0; v < VEC; ++v) {
-          R[v] = apply(fold[buf][k][0][v][lane], fold[buf][k][1][v][lane], R[v]);
-          if (REDUCE) P[v] = both(P[v], fold[buf][k][0][v][lane]);
+          R[v] = apply(fold[buf][k][v % GV][lane], fold[buf][k][GV + v][lane], R[v]);
+          if (REDUCE && v < GV) P[v] = both(P[v], fold[buf][k][v][lane]);
         }
       }
       buf ^= W > 1;
@@ -286,7 +285,7 @@ template <class X, class G, int MODE, int VEC, int W, bool REDUCE> __global__ __
   if (REDUCE) {
     float* part = (float*)p.part + (uint64_t)blockIdx.y * 2 * EC + ch;
 #pragma unroll
-    for (int v = 0; v < VEC; ++v) part[v] = P[v], part[EC + v] = R[v];
+    for (int v = 0; v < VEC; ++v) part[v] = P[v % GV], part[EC + v] = R[v];
   } else if (p.dstate && chunk == 0) {
 #pragma unroll
     for (int v = 0; v < VEC; ++v) ((float*)p.dstate)[ch + v] = R[v];
