@@ -349,7 +349,8 @@ def test_scan_refusals(ops):
 
 
 # ---- advantages -------------------------------------------------------------------------------------------------------------------
-@pytest.mark.parametrize("P,E,n", [(1, 1, 1), (2, 3, 2), (16, 5, 8), (17, 33, 2), (64, 9, 1), (100, 70, 3), (333, 4, 5)])
+@pytest.mark.parametrize("P,E,n", [(1, 1, 1), (2, 3, 2), (16, 5, 8), (17, 33, 2), (64, 9, 1), (100, 70, 3), (333, 4, 5), (65, 3, 2), (128, 70, 1), (129, 5, 3), (1000, 2, 3), (70, 4200, 8),
+                                   (140, 2100, 8)])
 @pytest.mark.parametrize("rt,vt", [(F64, F32), (F32, F32), (F64, BF16), (F32, F16)])
 def test_advantages(ops, P, E, n, rt, vt):
     g = gen(P * n)
