@@ -3,7 +3,7 @@
 // A_t = delta_t + gamma lam A_{t+1}: the recurrence of cp_scan.hip run against time, its input delta_t made on the way from reward,
 // value and done.  A lane owns one agent of one env (neighbouring lanes, neighbouring addresses), the W waves of a block share
 // its time axis in runs of kSteps steps.  double throughout: the engine's rewards are, and V_{t+1} - V_t cancels; bound by HBM all the
-// same: 64 planes of 16 384 envs x 8 agents in 34.5 us, 4.9 TB/s.  20 planes of 64 x 2 take 6.3 us, one run's chain of reads and the launch.
+// same: 64 planes of 16 384 envs x 8 agents in 34 us, 5.0 TB/s.  20 planes of 64 x 2 take 6.3 us, one run's chain of reads and the launch.
 #include "cp_common.h"
 
 namespace cp {
@@ -14,10 +14,13 @@ template <class R, class V, int W> __global__ __launch_bounds__(kWave * W) void 
   __shared__ double fold[2][W][2][kWave];
   const int lane = threadIdx.x & 63, w = W > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : 0;
   const uint64_t cols = a.rows * a.agents, col = (uint64_t)blockIdx.x * kWave + lane;
-  const bool live = col < cols, per_agent = a.flags & CE_ADV_DONE_PER_AGENT;
-  const uint64_t j = live ? col : cols - 1, dj = per_agent ? j : j / a.agents, dcols = per_agent ? cols : a.rows;
-  const R* reward = (const R*)a.reward + j;
-  const V* value = (const V*)a.value + j;
+  const bool per_agent = a.flags & CE_ADV_DONE_PER_AGENT;
+  const uint64_t j = col < cols ? col : cols - 1, dj = per_agent ? j : j / a.agents, dcols = per_agent ? cols : a.rows;
+  // A plane's base in scalar registers and a lane's 32-bit offset in it (2^28 columns of 8 bytes at most).  Without done flags the values' bytes
+  // are read in their place, and dropped: a branch there made each step wait for its own read (187 planes of 616 blocks: 53 us, now
+  // 33).
+  const uint64_t reward = (uint64_t)a.reward, value = (uint64_t)a.value, done = (uint64_t)(a.done ? a.done : (const uint8_t*)a.value);
+  const uint32_t r_off = (uint32_t)(j * sizeof(R)), v_off = (uint32_t)(j * sizeof(V)), o_off = (uint32_t)(j * sizeof(float)), ends = a.done ? 0xff : 0;
   const double end = a.last_value ? (double)(float)((const V*)a.last_value)[j] : 0.0, gl = a.gamma * a.lam;
   const uint64_t T = a.planes;
   auto plane = [&](uint64_t i) -> uint64_t {  // processed step i is time T - 1 - i
@@ -32,15 +35,19 @@ template <class R, class V, int W> __global__ __launch_bounds__(kWave * W) void 
     V v[kSteps];
     uint8_t d[kSteps];
     double after = end;
-    if (i > 0 && i < T) after = (double)(float)value[plane(i - 1) * cols];
+    const V before = load<V, 1>(value + plane(i > 0 && i < T ? i - 1 : 0) * cols * sizeof(V), v_off).v[0];
 #pragma unroll
-    for (int s = 0; s < kSteps; ++s)
-      if (i + s < T) {
-        const uint64_t pl = plane(i + s);
-        r[s] = reward[pl * cols];
-        v[s] = value[pl * cols];
-        d[s] = a.done ? a.done[pl * dcols + dj] : 0;
-      }
+    for (int s = 0; s < kSteps; ++s) {  // steps past the end read the last one
+      const uint64_t pl = plane(i + s < T ? i + s : T - 1);
+      r[s] = load<R, 1>(reward + pl * cols * sizeof(R), r_off).v[0];
+      v[s] = load<V, 1>(value + pl * cols * sizeof(V), v_off).v[0];
+      d[s] = load<uint8_t, 1>(done + pl * dcols, (uint32_t)dj).v[0];
+    }
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) d[s] &= ends;
+    float b = (float)before;
+    asm volatile("" : "+v"(b));  // read with the rest, not behind a branch of its own
+    if (i > 0) after = (double)b;
     double x[kSteps], rp = 1, rh = 0;
 #pragma unroll
     for (int s = 0; s < kSteps; ++s)
@@ -68,9 +75,9 @@ template <class R, class V, int W> __global__ __launch_bounds__(kWave * W) void 
     for (int s = 0; s < kSteps; ++s)
       if (i + s < T) {
         mine = step(d[s] ? 0.0 : gl, mine, x[s]);
-        const uint64_t at = plane(i + s) * cols + j;
-        if (live && a.advantage) a.advantage[at] = (float)mine;
-        if (live && a.ret) a.ret[at] = (float)(mine + (double)(float)v[s]);
+        const uint64_t at = plane(i + s) * cols * sizeof(float);  // lanes past the end do what the last one does, and write the same
+        if (a.advantage) store<float, 1>((uint64_t)a.advantage + at, o_off, {(float)mine});
+        if (a.ret) store<float, 1>((uint64_t)a.ret + at, o_off, {(float)(mine + (double)(float)v[s])});
       }
     if (W == 1) h = mine;
   }
@@ -79,11 +86,11 @@ template <class R, class V, int W> __global__ __launch_bounds__(kWave * W) void 
 template <class R, class V> static void go(const ce_advantage& a, hipStream_t s) {
   const uint32_t blocks = (uint32_t)((a.rows * a.agents + kWave - 1) / kWave);
   // Waves that share a block's time axis: as many as have a run, while blocks are too few to fill the chip by themselves.  us with 4 / 8 / 16 waves:
-  // 64 planes x 512 blocks 12.7 / 13.3 / 19.5, 128 x 64 13.5 / 9.4 / 10.0, 187 x 256 40 / 31 / 20, 256 x 512 39 / 36 / 40, 187 x 616 53 / 64 / 57,
-  // 927 x 1 92 / 55 / 40.
+  // 64 planes x 512 blocks 13.0 / 17.2 / 20.2, 128 x 64 12.4 / 9.0 / 10.0, 187 x 256 18.2 / 15.5 / 13.6, 256 x 512 42 / 43 / 38,
+  // 187 x 616 33 / 36 / 36, 927 x 1 74 / 47 / 36.
   if (a.planes <= kSteps) k_advantages<R, V, 1><<<blocks, kWave, 0, s>>>(a);
   else if (a.planes <= 4 * kSteps || blocks > 512) k_advantages<R, V, 4><<<blocks, 4 * kWave, 0, s>>>(a);
-  else if (a.planes <= 8 * kSteps || blocks > 256) k_advantages<R, V, 8><<<blocks, 8 * kWave, 0, s>>>(a);
+  else if (a.planes <= 8 * kSteps) k_advantages<R, V, 8><<<blocks, 8 * kWave, 0, s>>>(a);
   else k_advantages<R, V, 16><<<blocks, 16 * kWave, 0, s>>>(a);
 }
 template <class R> static void values(const ce_advantage& a, hipStream_t s) {
