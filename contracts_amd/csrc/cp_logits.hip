@@ -121,7 +121,8 @@ __device__ __forceinline__ float only(float z, uint32_t ok, int q) {
 
 // ---- a run of one row -----------------------------------------------------------------------------------------------------------
 // What does not wait for something else is read first (a block is a chain of reads: the fewer links, the better): scores, the first tokens of the
-// history whatever its length, the row's own numbers; then the mask, whose place one of these names.
+// history whatever its length, the row's own numbers; then the mask, whose place one of these names.  (Scores taken apart where they are read, or
+// read behind a branch, cost a wait of their own: 36 us against 33 at 256 x 131072 bfloat16, 160 against 153 for both passes at 2048 x 32000.)
 // The table is 16 KB, 8 blocks a CU.  (Entries of 16 bits and runs of 8192 gain nothing: 29.7 us against 29.0 at 256 x 131072 bfloat16 with
 // histories of up to 2048, 6.1 against 4.7 at 1 x 50257 float; without a history the same pass takes 22, as a copy does.)
 template <class X, class O, class K> __global__ __launch_bounds__(kBlock) void k_logits_run(ce_logits s, uint64_t row0, uint32_t runs) {
@@ -132,11 +133,11 @@ template <class X, class O, class K> __global__ __launch_bounds__(kBlock) void k
   const uint32_t v0 = blockIdx.x % runs * kTile, V = (uint32_t)s.vocab, n = V - v0 < kTile ? V - v0 : kTile;
   const X* x = (const X*)s.logits + (int64_t)r * s.logits_row + v0;
   O* o = (O*)s.out + (int64_t)r * s.out_row + v0;
-  Eight raw[kGroups];
+  struct { uint32_t w[sizeof(Eight) / 4]; } raw[kGroups];  // taken apart behind the other reads only
 #pragma unroll
-  for (int g = 0; g < kGroups; ++g) {
-    const uint32_t k = (g * kBlock + threadIdx.x) * kLane;
-    if (k + kLane <= n) __builtin_memcpy(&raw[g], __builtin_assume_aligned(x + k, alignof(X)), sizeof(Eight));
+  for (int g = 0; g < kGroups; ++g) {  // lanes past the end read 8 scores of the row ahead of it (it has 8: shapes()), and drop them
+    const int32_t k = (g * kBlock + threadIdx.x) * kLane, last = (int32_t)n - kLane;
+    __builtin_memcpy(&raw[g], __builtin_assume_aligned(x + (k <= last ? k : last), alignof(X)), sizeof(Eight));
   }
   const uint32_t history = s.tokens ? (uint32_t)s.history : 0;
   const K* tokens = (const K*)s.tokens + (int64_t)r * s.token_row;
@@ -178,7 +179,7 @@ template <class X, class O, class K> __global__ __launch_bounds__(kBlock) void k
       float l[kLane], add[kLane];
       if (s.bias) bias8(s, b + k, add);
 #pragma unroll
-      for (int q = 0; q < 8; ++q) l[q] = (float)raw[g].v[q];
+      for (int q = 0; q < 8; ++q) l[q] = (float)__builtin_bit_cast(Eight, raw[g]).v[q];
       if (used) {
         const uint4 lo = ((const uint4*)table)[k / 4], hi = ((const uint4*)table)[k / 4 + 1];
         const uint32_t e[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
@@ -265,10 +266,10 @@ template <class X, class O, class K> __global__ __launch_bounds__(kBlock) void k
 }
 
 template <class X, class O, class K> static void shapes(const ce_logits& s, hipStream_t st) {
-  // A row is worth blocks of its own where it is long or there are no more of them than blocks in flight (8 a CU); otherwise a block takes as many rows
+  // A row is worth blocks of its own (which read 8 scores at a time, so it has to have 8) where it is long or there are no more of them than blocks in flight (8 a CU); otherwise a block takes as many rows
   // as fit and leave 1024 blocks.  us, own blocks against packed: 4.7 / 8.2 at 1000 x 32 float, 6.9 / 13.6 at 2048 x 600, 32.6 / 35.7 at 20000 x 512
   // bfloat16; 20.9 / 15.5 at 8192 x 300 float, 94 / 19 at 65536 x 64.  Packed, 131072 x 8: 9.4 with 1024 blocks, 10.2 with 512, 13.9 with 2048.
-  if (s.vocab >= 512 || s.rows <= 2048) {
+  if (s.vocab >= 512 || (s.rows <= 2048 && s.vocab >= kLane)) {
     const uint32_t runs = (uint32_t)((s.vocab + kTile - 1) / kTile);
     const uint64_t most = (1u << 23) / runs;  // rows of a launch: fewer than 2^32 threads
     for (uint64_t r = 0; r < s.rows; r += most)
