@@ -76,6 +76,12 @@ void apart(const char* op, const Maybe& out, const char* name, std::initializer_
       if (o.second > i.first && i.second > o.first) bad(op, ": ", name, " overlaps an input");
     }
 }
+// An output that is part of a graph would keep the gradients of what it held before (torch's own out= refuses it too).
+void no_graph(const char* op, std::initializer_list<const Maybe*> outs) {
+  if (!at::GradMode::is_enabled()) return;
+  for (const Maybe* t : outs)
+    if (*t && (*t)->requires_grad()) bad(op, ": an output wants a gradient, which this call would not keep; detach it");
+}
 
 uint32_t code(const Tensor& t) {
   switch (t.scalar_type()) {
@@ -197,6 +203,7 @@ std::tuple<Tensor, Tensor> linear_scan(Tensor x, const py::object& gate_or_decay
   if (THPVariable_Check(gate_or_decay.ptr())) gate = THPVariable_Unpack(gate_or_decay.ptr());
   else decay = number(gate_or_decay);
   same_device(op, x, {&gate, &state, &done, &out, &state_out});
+  no_graph(op, {&out, &state_out});
   const auto type = x.scalar_type();
   const bool twice = type == at::kDouble;
   if (!real(type) && !twice) bad("linear_scan: x must be float32, bfloat16, float16 or float64, not ", type);
@@ -254,6 +261,7 @@ std::tuple<Tensor, Tensor> advantages(Tensor reward, Tensor value, Maybe last_va
   if (out) adv_out = out->first, ret_out = out->second;
   const Maybe mv = value;
   same_device(op, reward, {&mv, &last_value, &done, &adv_out, &ret_out});
+  no_graph(op, {&adv_out, &ret_out});
   const int64_t P = reward.size(0), E = reward.size(1), n = reward.size(2);
   if (reward.scalar_type() != at::kDouble && reward.scalar_type() != at::kFloat) bad("advantages: reward must be float64 or float32, not ", reward.scalar_type());
   if (value.sizes() != reward.sizes() || !real(value.scalar_type())) bad("advantages: value must be float32, bfloat16 or float16 ", reward.sizes());
@@ -419,6 +427,7 @@ Tensor process_logits(const Tensor& logits, Maybe tokens, Maybe lengths, Maybe p
     else h.scalar[k] = number(*given[k]);
   }
   same_device(op, logits, {&tokens, &lengths, &prompt_lengths, &penalty[0], &penalty[1], &penalty[2], &bias, &mask, &mask_index, &out});
+  no_graph(op, {&out});
   const auto lead = logits.sizes().slice(0, logits.dim() - 1);
   const int64_t V = logits.size(-1), rows = c10::multiply_integers(lead);
   for (int k = 0; k < 3; ++k)

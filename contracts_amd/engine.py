@@ -279,7 +279,7 @@ class BatchedEnv:
     def shape_scores(self, scores, out=None, **shaping):
         """scores [E, n, |A|] shaped ahead of step_policy_device(.., "argmax") by policy_ops.process_logits — masks of allowed actions, biases,
         penalties for repeated actions (tokens=[E, n, L] past action ids) — as the float32 plane that mode reads: `out`
-        (float32 [E, n, |A|], may be `scores`) or a new one; on torch's current stream, which the step's stream has to follow"""
+        (float32 [E, n, |A|], may be `scores`) or a new one, without gradients; on torch's current stream, which the step's stream has to follow"""
         import torch
         from . import policy_ops
         if self.num_actions is None:
@@ -291,6 +291,8 @@ class BatchedEnv:
             out = torch.empty(shape, dtype=torch.float32, device=scores.device)
         elif out.dtype != torch.float32 or not out.is_contiguous():
             raise ValueError("shape_scores: out must be a dense float32 tensor")
+        elif out.requires_grad and torch.is_grad_enabled():
+            raise ValueError("shape_scores: out wants a gradient, which this call would not keep; detach it")
         with torch.no_grad():
             return policy_ops.process_logits(scores, out=out, **shaping)
 
