@@ -46,6 +46,19 @@ bool flag(at::ScalarType t) { return t == at::kBool || t == at::kByte; }
 void on_gpu(const char* op, const Tensor& t) {
   if (!t.is_cuda()) bad(op, ": tensors must live on a GPU (there is no CPU path), got ", t.device());
 }
+// Tensors that stand for others: batched, traced or differentiated by a transform, of a subclass that dispatches, zeros that are nowhere.
+bool wrapped(const Tensor& t) {
+  using c10::DispatchKey;
+  constexpr c10::DispatchKeySet keys({DispatchKey::Python, DispatchKey::Batched, DispatchKey::FuncTorchBatched, DispatchKey::FuncTorchGradWrapper, DispatchKey::Functionalize, DispatchKey::ZeroTensor});
+  return t.key_set().has_any(keys);
+}
+// An incoming gradient as numbers that lie in memory; one that carries a forward-mode derivative, or is a batch in one, is refused.
+Tensor incoming(const char* op, const Tensor& t) {
+  if (!t.defined()) return t;
+  if (wrapped(t)) throw Refused(std::string(op) + ": a gradient that is a wrapped tensor (batched, traced, of a subclass) has no memory to read");
+  if (t._fw_grad(0).defined()) throw Refused(std::string(op) + ": has no forward-mode derivative");
+  return t.resolve_neg();
+}
 // All on one device, and numbers as they lie in memory: not a lazily negated view, not carrying a forward-mode derivative, which a call would drop.
 void same_device(const char* op, const Tensor& first, std::initializer_list<const Maybe*> rest) {
   auto plain = [&](const Tensor& t) {
@@ -181,8 +194,9 @@ struct Scan : torch::autograd::Function<Scan> {
     Tensor dx = at::empty({T, E, C}, x.options()), dgate, dstate;
     if (gate.defined()) dgate = x.numel() ? at::empty(gate.sizes(), gate.options()) : at::zeros(gate.sizes(), gate.options());
     if (need & 4) dstate = at::empty({E, C}, x.options().dtype(at::kFloat));
-    const Tensor dy = grads[0].defined() ? grads[0].contiguous() : at::zeros({T, E, C}, x.options());
-    const Tensor dlast = grads[1].defined() ? grads[1].contiguous() : Tensor();
+    Tensor dy = incoming("linear_scan", grads[0]), dlast = incoming("linear_scan", grads[1]);
+    dy = dy.defined() ? dy.contiguous() : at::zeros({T, E, C}, x.options());
+    if (dlast.defined()) dlast = dlast.contiguous();
     ce_scan s = describe(x, gate, ctx->saved_data["decay"].toDouble(), done, ctx->saved_data["reverse"].toBool());
     s.saved = ptr<float>(kept[3]);
     const ce_scan_grad g = {ptr(dy), ptr(dlast), ptr(dx), ptr(dgate), ptr(dstate)};
@@ -372,7 +386,7 @@ struct Logits : torch::autograd::Function<Logits> {
     return out;
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
-    Tensor dz = grads[0];
+    Tensor dz = incoming("process_logits", grads[0]);
     if (!dz.defined()) return {Tensor(), Tensor(), Tensor()};
     const auto kept = ctx->get_saved_variables();
     const Tensor &logits = kept[0], &bias = kept[1];

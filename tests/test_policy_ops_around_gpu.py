@@ -41,3 +41,42 @@ def test_shaped_scores_are_not_written_into_a_graph(ops):
     with torch.no_grad():
         assert env.shape_scores(w * 2, bias=-w, out=(buf := w * 2)) is buf and buf.eq(1).all()
     env.close()
+@pytest.mark.parametrize("T,E,C,H", [(1, 1, 1, 1), (40, 2, 6, 3), (700, 2, 6, 6)])
+def test_scan_takes_gradients_that_are_lazily_negated(ops, T, E, C, H):
+    x, gate, state, done = scan_inputs(T, E, C, H, F32, F32, 3)
+    leaves = [t.requires_grad_(True) for t in (x, gate, state)]
+    dy, dl, neg = torch.randn((T, E, C), device="cuda"), torch.randn((E, C), device="cuda"), torch._neg_view
+    y, last = ops.linear_scan(x, gate, state=state, done=done)
+    want = torch.autograd.grad((y, last), leaves, (-dy, -dl), retain_graph=True)
+    for a, b in ((neg(dy), neg(dl)), (neg(dy), -dl), (-dy, neg(dl))):
+        assert all(g.equal(w) for g, w in zip(torch.autograd.grad((y, last), leaves, (a, b), retain_graph=True), want))
+    got, = torch.autograd.grad(torch.view_as_real(torch.complex(torch.zeros_like(y), y).conj().resolve_conj()), x, torch.stack([dy, dy], -1), retain_graph=True)
+    assert got.equal(torch.autograd.grad(y, x, -dy, retain_graph=True)[0])
+
+
+@pytest.mark.parametrize("R,V", [(1, 1), (7, 1), (5, 9), (3, 5000)])
+def test_logits_take_gradients_that_are_lazily_negated(ops, R, V):
+    l, bias = torch.randn((R, V), device="cuda").requires_grad_(True), torch.randn((1, V), device="cuda").requires_grad_(True)
+    tok = torch.zeros((R, 2), dtype=torch.int32, device="cuda")
+    dz = torch.randn((R, V), device="cuda")
+    z = ops.process_logits(l, tokens=tok, repetition=2.0, bias=bias)
+    want = torch.autograd.grad(z, (l, bias), -dz, retain_graph=True)
+    got = torch.autograd.grad(z, (l, bias), torch._neg_view(dz), retain_graph=True)
+    assert got[0].equal(want[0]) and got[1].equal(want[1])
+    got = torch.autograd.grad(torch.complex(torch.zeros_like(z), z).conj(), (l, bias), torch.complex(torch.zeros_like(dz), dz))
+    assert got[0].equal(want[0]) and got[1].equal(want[1])
+
+
+def test_gradients_that_carry_more_than_numbers_are_refused(ops):
+    """a forward-mode derivative of a gradient would be dropped; a batch of gradients in one has no memory to read"""
+    import torch.autograd.forward_ad as fwd
+    x = torch.randn((5, 2, 4), device="cuda").requires_grad_(True)
+    for out in (*ops.linear_scan(x, 0.5), ops.process_logits(x)):
+        d = torch.ones_like(out)
+        with fwd.dual_level(), pytest.raises(RuntimeError, match="forward-mode"):
+            torch.autograd.grad(out, x, fwd.make_dual(d, d), retain_graph=True)
+        with pytest.raises(RuntimeError, match="wrapped"):
+            torch.autograd.grad(out, x, torch.stack([d, d]), retain_graph=True, is_grads_batched=True)
+        torch.autograd.grad(out, x, d, retain_graph=True)
+
+
