@@ -4,9 +4,11 @@
 // Host-side marshalling and the checks of arguments, because a call's latency is the host's: a forward call took 11-14 us through Python and
 // ctypes, of which the launch is 3, and a forward and backward pass 120 us, most of it the interpreter in torch's backward thread.  What
 // reaches the device is checked by the C-ABI once more.  policy_ops.py documents the calls.
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/extension.h>
 #include <ATen/TensorUtils.h>
 
@@ -43,8 +45,11 @@ double number(const py::object& o) {
 }
 bool real(at::ScalarType t) { return t == at::kFloat || t == at::kBFloat16 || t == at::kHalf; }
 bool flag(at::ScalarType t) { return t == at::kBool || t == at::kByte; }
-void on_gpu(const char* op, const Tensor& t) {
-  if (!t.is_cuda()) bad(op, ": tensors must live on a GPU (there is no CPU path), got ", t.device());
+// Recorded as a graph, a call would leave nothing behind but the allocation of its outputs.
+bool traced() {
+  using Modes = c10::impl::TorchDispatchModeTLS;
+  using Key = c10::impl::TorchDispatchModeKey;
+  return torch::jit::tracer::isTracing() || Modes::get_mode(Key::PROXY) || Modes::get_mode(Key::FAKE);
 }
 // Tensors that stand for others: batched, traced or differentiated by a transform, of a subclass that dispatches, zeros that are nowhere.
 bool wrapped(const Tensor& t) {
@@ -52,8 +57,17 @@ bool wrapped(const Tensor& t) {
   constexpr c10::DispatchKeySet keys({DispatchKey::Python, DispatchKey::Batched, DispatchKey::FuncTorchBatched, DispatchKey::FuncTorchGradWrapper, DispatchKey::Functionalize, DispatchKey::ZeroTensor});
   return t.key_set().has_any(keys);
 }
+void memory(const char* op, const Tensor& t) {
+  if (wrapped(t)) bad(op, ": a wrapped tensor (batched, traced, of a subclass) has no memory to read");
+}
+void on_gpu(const char* op, const Tensor& t) {
+  if (traced()) bad(op, ": cannot be traced or recorded as a graph of operations");
+  memory(op, t);
+  if (!t.is_cuda()) bad(op, ": tensors must live on a GPU (there is no CPU path), got ", t.device());
+}
 // An incoming gradient as numbers that lie in memory; one that carries a forward-mode derivative, or is a batch in one, is refused.
 Tensor incoming(const char* op, const Tensor& t) {
+  if (traced()) throw Refused(std::string(op) + ": the backward pass cannot be traced or recorded as a graph of operations");
   if (!t.defined()) return t;
   if (wrapped(t)) throw Refused(std::string(op) + ": a gradient that is a wrapped tensor (batched, traced, of a subclass) has no memory to read");
   if (t._fw_grad(0).defined()) throw Refused(std::string(op) + ": has no forward-mode derivative");
@@ -62,6 +76,7 @@ Tensor incoming(const char* op, const Tensor& t) {
 // All on one device, and numbers as they lie in memory: not a lazily negated view, not carrying a forward-mode derivative, which a call would drop.
 void same_device(const char* op, const Tensor& first, std::initializer_list<const Maybe*> rest) {
   auto plain = [&](const Tensor& t) {
+    memory(op, t);
     if (t.is_neg()) bad(op, ": a lazily negated view; call resolve_neg() on it");
     if (t._fw_grad(0).defined()) bad(op, ": has no forward-mode derivative");
   };

@@ -12,7 +12,8 @@ Tensors live on an MI355X (there is no CPU path) and a call is asynchronous on t
 are new tensors unless `out=` names them (tensors that want no gradient), scratch memory comes from torch's allocator, nothing is kept between calls, and every call may
 be captured into a graph (a backward pass together with its forward pass, and with leaves of its own: torch's engine ends the process where
 a captured backward pass meets the nodes of an eager graph of the same leaves).  Ordering against other streams (env slices on side streams) is the caller's, as for the engine's steps.
-A tensor whose last axis is not dense, or whose leading axes do not collapse into one stride, is copied first."""
+A tensor whose last axis is not dense, or whose leading axes do not collapse into one stride, is copied first.
+torch's tracers and transforms (jit.trace, fx, vmap, torch.func, fake tensors) are refused: calls are no operations of its dispatcher."""
 import torch
 
 from . import _lib

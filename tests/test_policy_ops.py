@@ -181,3 +181,38 @@ def test_pack_mask_and_the_oracles_gradients():
                 down = value()
                 flat[i] = keep
                 assert abs((up - down) / 0.5 - d.reshape(-1)[i]) < 1e-12 * (1 + np.abs(d).max()) * 100
+
+
+def test_tracers_transforms_and_wrapped_tensors_are_refused():
+    """a call is no operation that they could record: the graph would hold the outputs' allocation alone"""
+    from torch._subclasses import FakeTensorMode
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    from contracts_amd import policy_ops as ops
+    x = torch.zeros(2, 3, 4)
+
+    class Wrapper(torch.Tensor):
+        @staticmethod
+        def __new__(cls, inner):
+            return torch.Tensor._make_wrapper_subclass(cls, inner.size(), dtype=inner.dtype)
+
+        @classmethod
+        def __torch_dispatch__(cls, func, types, args=(), kwargs=None):
+            raise AssertionError("never reached")
+
+    for call in (lambda t: ops.linear_scan(t, 0.5)[0], lambda t: ops.advantages(t, t)[0], lambda t: ops.process_logits(t)):
+        with pytest.raises(ValueError, match="traced"):
+            torch.jit.trace(call, x)
+        for mode in ("real", "fake"):
+            with pytest.raises(ValueError, match="traced"):
+                make_fx(call, tracing_mode=mode)(x)
+        with FakeTensorMode(), pytest.raises(ValueError, match="traced"):
+            call(torch.empty(2, 3, 4))
+        with FakeTensorMode():
+            fake = torch.empty(2, 3, 4)
+        for run in (lambda: torch.vmap(call)(x.expand(2, 2, 3, 4)), lambda: torch.func.grad(lambda t: call(t).sum())(x), lambda: call(fake), lambda: call(torch._efficientzerotensor(2, 3, 4)),
+                    lambda: call(Wrapper(x))):
+            with pytest.raises(ValueError, match="wrapped"):
+                run()
+        with pytest.raises(ValueError, match="no CPU path"):
+            call(torch.nn.Parameter(x))
