@@ -49,25 +49,39 @@ template <class R, class V, int W> __global__ __launch_bounds__(kWave * W) void 
     asm volatile("" : "+v"(b));  // read with the rest, not behind a branch of its own
     if (i > 0) after = (double)b;
     double x[kSteps], rp = 1, rh = 0;
+    bool ended = gl == 0;  // the run's map forgets what comes into it
 #pragma unroll
     for (int s = 0; s < kSteps; ++s)
       if (i + s < T) {
         const double now = (double)(float)v[s];
         x[s] = (double)r[s] - now + (d[s] ? 0.0 : a.gamma * after);
         after = now;
-        const double g = d[s] ? 0.0 : gl;
-        rp = both(rp, g);
-        rh = step(g, rh, x[s]);
+        ended |= d[s] != 0;
+        rp *= gl;
+        rh = step(d[s] ? 0.0 : gl, rh, x[s]);
       }
+    if (ended || rp == 0) rp = product(rp, ended);
     double mine = h;
     if (W > 1) {
       fold[buf][w][0][lane] = rp;
       fold[buf][w][1][lane] = rh;
       __syncthreads();
+      // the waves' maps in turn, by bare multiply-adds: what is not finite stays so to the last of them, and then apply() takes their place
+      double at = h;
 #pragma unroll
       for (int k = 0; k < W; ++k) {
-        if (k == w) mine = h;
-        h = apply(fold[buf][k][0][lane], fold[buf][k][1][lane], h);
+        if (k == w) mine = at;
+        const double P = fold[buf][k][0][lane];
+        at = fma_(magnitude(P) <= kLeast<double> ? 0.0 : P, at, fold[buf][k][1][lane]);
+      }
+      if (rare(!finite(at))) {
+#pragma unroll 1  // the maps are read again: kept, they would cost the 16 waves registers (187 x 16384: 14.7 us, 21.6 so)
+        for (int k = 0; k < W; ++k) {
+          if (k == w) mine = h;
+          h = apply(fold[buf][k][0][lane], fold[buf][k][1][lane], h);
+        }
+      } else {
+        h = at;
       }
       buf ^= 1;
     }

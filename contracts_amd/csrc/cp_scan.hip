@@ -46,17 +46,30 @@ template <class X, class G, int MODE, int VEC, int W, bool REDUCE> __global__ __
   if (!REDUCE && W > 1 && blockIdx.y > 0) {  // the chunks before this one: each wave composes its share of them, then all fold the shares
     const uint64_t EC = (uint64_t)p.cols * VEC;
     const uint32_t each = (blockIdx.y + W - 1) / W, k0 = w * each, k1 = k0 + each < blockIdx.y ? k0 + each : blockIdx.y;
+    auto part_of = [&](uint32_t k) { return (const A*)p.part + (uint64_t)k * 2 * EC + ch; };
     A cp[GV], cs[VEC];
+    bool gone[GV], far = false;
 #pragma unroll
-    for (int v = 0; v < VEC; ++v) cp[v % GV] = A(1), cs[v] = A(0);
+    for (int v = 0; v < VEC; ++v) cp[v % GV] = A(1), cs[v] = A(0), gone[v % GV] = false;
 #pragma unroll 8
-    for (uint32_t k = k0; k < k1; ++k) {
-      const A* part = (const A*)p.part + (uint64_t)k * 2 * EC + ch;
+    for (uint32_t k = k0; k < k1; ++k) {  // bare multiply-adds, as in a tile's fold
+      const A* part = part_of(k);
 #pragma unroll
       for (int v = 0; v < VEC; ++v) {
-        cs[v] = apply(part[v % GV], part[EC + v], cs[v]);
-        if (v < GV) cp[v] = both(cp[v], part[v]);
+        cs[v] = fma_(magnitude(part[v % GV]) <= kLeast<A> ? A(0) : part[v % GV], cs[v], part[EC + v]);
+        if (v < GV) cp[v] *= part[v], gone[v] |= part[v] == A(0);
       }
+    }
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) far |= !finite(cs[v]);
+#pragma unroll
+    for (int v = 0; v < GV; ++v) cp[v] = product(cp[v], gone[v]);
+    if (rare(far)) {
+#pragma unroll
+      for (int v = 0; v < VEC; ++v) cs[v] = A(0);
+      for (uint32_t k = k0; k < k1; ++k)
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) cs[v] = apply(part_of(k)[v % GV], part_of(k)[EC + v], cs[v]);
     }
 #pragma unroll
     for (int v = 0; v < VEC; ++v) fold[0][w][v % GV][lane] = cp[v % GV], fold[0][w][GV + v][lane] = cs[v];
@@ -100,6 +113,13 @@ template <class X, class G, int MODE, int VEC, int W, bool REDUCE> __global__ __
       const A a = (cut >> s) & 1 ? A(0) : gate_of(s, v);
       return step(a, from, A(tx[s].v[v]));
     };
+    // whether a gate of 0, or a border, is in the run
+    auto forgets = [&](int v) -> bool {
+      bool f = cut != 0;
+#pragma unroll
+      for (int s = 0; s < kSteps; ++s) f |= s < n && gate_of(s, v) == A(0);
+      return f;
+    };
     A mine[VEC];
 #pragma unroll
     for (int v = 0; v < VEC; ++v) mine[v] = h[v];
@@ -131,23 +151,77 @@ template <class X, class G, int MODE, int VEC, int W, bool REDUCE> __global__ __
           if (s < n)
 #pragma unroll
             for (int v = 0; v < VEC; ++v) {
-              if (v < GV) rp[v] = both(rp[v], (cut >> s) & 1 ? A(0) : gate_of(s, v));
-              rh[v] = careful(s, v, rh[v]);
+              const A a = (cut >> s) & 1 ? A(0) : gate_of(s, v);
+              if (v < GV) rp[v] *= a;
+              rh[v] = step(a, rh[v], A(tx[s].v[v]));
             }
       }
+      bool ask = false;  // a product that left the range forgets all the same; and of a chunk's it is not known yet what comes into it
+#pragma unroll
+      for (int v = 0; v < GV; ++v) ask |= !finite(rp[v]) || (REDUCE && rp[v] == 0 && cut == 0);
+      if (rare(ask))
+#pragma unroll
+        for (int v = 0; v < GV; ++v)
+          if (REDUCE || !finite(rp[v])) rp[v] = product(rp[v], forgets(v));
 #pragma unroll
       for (int v = 0; v < VEC; ++v) fold[buf][w][v % GV][lane] = rp[v % GV], fold[buf][w][GV + v][lane] = rh[v];
       if (W > 1) __syncthreads();
+      // The waves' maps in turn, by bare multiply-adds: what is not finite stays so to the last of them, and then apply() takes their place, over products
+      // of 0 that are told apart now.  All waves fold the same maps onto the same state, so all of them take this branch or none does.
+      A at[VEC];
+      A Pt[GV];
+      bool far = false;
+#pragma unroll
+      for (int v = 0; v < VEC; ++v) at[v] = h[v], Pt[v % GV] = P[v % GV];
 #pragma unroll
       for (int k = 0; k < W; ++k) {
         if (k == w)
 #pragma unroll
-          for (int v = 0; v < VEC; ++v) mine[v] = h[v];
+          for (int v = 0; v < VEC; ++v) mine[v] = at[v];
 #pragma unroll
         for (int v = 0; v < VEC; ++v) {
-          h[v] = apply(fold[buf][k][v % GV][lane], fold[buf][k][GV + v][lane], h[v]);
-          if (REDUCE && v < GV) P[v] = both(P[v], fold[buf][k][v][lane]);
+          const A Pk = fold[buf][k][v % GV][lane];
+          at[v] = fma_(REDUCE && magnitude(Pk) <= kLeast<A> ? A(0) : Pk, at[v], fold[buf][k][GV + v][lane]);
+          if (REDUCE && v < GV) Pt[v] *= Pk;
         }
+      }
+#pragma unroll
+      for (int v = 0; v < VEC; ++v) far |= !finite(at[v]);
+      if (rare(far)) {
+        if (W > 1) __syncthreads();
+        if (!REDUCE)
+#pragma unroll
+          for (int v = 0; v < GV; ++v) {
+            A& own = fold[buf][w][v][lane];
+            if (own == 0) own = product(own, forgets(v));
+          }
+        if (W > 1) __syncthreads();
+#pragma unroll 1
+        for (int k = 0; k < W; ++k) {
+          if (k == w)
+#pragma unroll
+            for (int v = 0; v < VEC; ++v) mine[v] = h[v];
+#pragma unroll
+          for (int v = 0; v < VEC; ++v) h[v] = apply(fold[buf][k][v % GV][lane], fold[buf][k][GV + v][lane], h[v]);
+        }
+      } else {
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) h[v] = at[v];
+      }
+      if (REDUCE) {  // a product that becomes 0, or leaves the range, in this tile is taken once more
+        bool turns = false;
+#pragma unroll
+        for (int v = 0; v < GV; ++v) turns |= P[v] != 0 && (Pt[v] == 0 || !finite(Pt[v]));
+        if (rare(turns)) {
+#pragma unroll
+          for (int v = 0; v < GV; ++v) Pt[v] = P[v];
+#pragma unroll
+          for (int k = 0; k < W; ++k)
+#pragma unroll
+            for (int v = 0; v < GV; ++v) Pt[v] = both(Pt[v], fold[buf][k][v][lane]);
+        }
+#pragma unroll
+        for (int v = 0; v < GV; ++v) P[v] = P[v] == 0 ? P[v] : Pt[v];
       }
       buf ^= W > 1;
     }

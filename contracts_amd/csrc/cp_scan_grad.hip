@@ -68,17 +68,30 @@ template <class X, class G, int MODE, int VEC, int W, bool REDUCE> __global__ __
   int buf = 0;
   if (!REDUCE && W > 1 && chunk + 1 < p.chunks) {  // the chunks behind this one, last first: each wave composes its share, then all fold the shares
     const uint32_t behind = p.chunks - 1 - chunk, each = (behind + W - 1) / W, k0 = w * each, k1 = k0 + each < behind ? k0 + each : behind;
+    auto part_of = [&](uint32_t k) { return (const float*)p.part + (uint64_t)(p.chunks - 2 - k) * 2 * EC + ch; };
     float cp[GV], cs[VEC];
+    bool gone[GV], far = false;
 #pragma unroll
-    for (int v = 0; v < VEC; ++v) cp[v % GV] = 1.f, cs[v] = 0.f;
+    for (int v = 0; v < VEC; ++v) cp[v % GV] = 1.f, cs[v] = 0.f, gone[v % GV] = false;
 #pragma unroll 8
-    for (uint32_t k = k0; k < k1; ++k) {
-      const float* part = (const float*)p.part + (uint64_t)(p.chunks - 2 - k) * 2 * EC + ch;  // of chunk chunks - 1 - k
+    for (uint32_t k = k0; k < k1; ++k) {  // bare multiply-adds, as in a tile's fold
+      const float* part = part_of(k);
 #pragma unroll
       for (int v = 0; v < VEC; ++v) {
-        cs[v] = apply(part[v % GV], part[EC + v], cs[v]);
-        if (v < GV) cp[v] = both(cp[v], part[v]);
+        cs[v] = fma_(magnitude(part[v % GV]) <= kLeast<float> ? 0.f : part[v % GV], cs[v], part[EC + v]);
+        if (v < GV) cp[v] *= part[v], gone[v] |= part[v] == 0.f;
       }
+    }
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) far |= !finite(cs[v]);
+#pragma unroll
+    for (int v = 0; v < GV; ++v) cp[v] = product(cp[v], gone[v]);
+    if (rare(far)) {
+#pragma unroll
+      for (int v = 0; v < VEC; ++v) cs[v] = 0.f;
+      for (uint32_t k = k0; k < k1; ++k)
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) cs[v] = apply(part_of(k)[v % GV], part_of(k)[EC + v], cs[v]);
     }
 #pragma unroll
     for (int v = 0; v < VEC; ++v) fold[0][w][v % GV][lane] = cp[v % GV], fold[0][w][GV + v][lane] = cs[v];
@@ -121,6 +134,12 @@ template <class X, class G, int MODE, int VEC, int W, bool REDUCE> __global__ __
     const bool plain = n == kSteps && !flags.any;
     auto gate_of = [&](int s, int v) -> float { return MODE == kGateConst ? (float)p.decay : (float)tg[s].v[GV > 1 ? v : 0]; };
     auto cut_gate = [&](int s, int v) -> float { return (cut >> s) & 1 ? 0.f : gate_of(s, v); };
+    auto forgets = [&](int v) -> bool {
+      bool f = cut != 0;
+#pragma unroll
+      for (int s = 0; s < kSteps; ++s) f |= s < n && gate_of(s, v) == 0.f;
+      return f;
+    };
     float mine[VEC];
 #pragma unroll
     for (int v = 0; v < VEC; ++v) mine[v] = R[v];
@@ -154,23 +173,74 @@ template <class X, class G, int MODE, int VEC, int W, bool REDUCE> __global__ __
 #pragma unroll
             for (int v = 0; v < VEC; ++v) {
               const float a = cut_gate(s, v);
-              if (v < GV) rp[v] = both(rp[v], a);
+              if (v < GV) rp[v] *= a;
               rq[v] = a == 0.f ? 0.f : a * ((float)ty[s].v[v] + rq[v]);
             }
       }
+      bool ask = false;  // a product that left the range forgets all the same; and of a chunk's it is not known yet what comes into it
+#pragma unroll
+      for (int v = 0; v < GV; ++v) ask |= !finite(rp[v]) || (REDUCE && rp[v] == 0 && cut == 0);
+      if (rare(ask))
+#pragma unroll
+        for (int v = 0; v < GV; ++v)
+          if (REDUCE || !finite(rp[v])) rp[v] = product(rp[v], forgets(v));
 #pragma unroll
       for (int v = 0; v < VEC; ++v) fold[buf][w][v % GV][lane] = rp[v % GV], fold[buf][w][GV + v][lane] = rq[v];
       if (W > 1) __syncthreads();
+      float at[VEC];  // the waves' maps in turn, as in the forward pass
+      float Pt[GV];
+      bool far = false;
+#pragma unroll
+      for (int v = 0; v < VEC; ++v) at[v] = R[v], Pt[v % GV] = P[v % GV];
 #pragma unroll
       for (int k = W - 1; k >= 0; --k) {
         if (k == w)
 #pragma unroll
-          for (int v = 0; v < VEC; ++v) mine[v] = R[v];
+          for (int v = 0; v < VEC; ++v) mine[v] = at[v];
 #pragma unroll
         for (int v = 0; v < VEC; ++v) {
-          R[v] = apply(fold[buf][k][v % GV][lane], fold[buf][k][GV + v][lane], R[v]);
-          if (REDUCE && v < GV) P[v] = both(P[v], fold[buf][k][v][lane]);
+          const float Pk = fold[buf][k][v % GV][lane];
+          at[v] = fma_(REDUCE && magnitude(Pk) <= kLeast<float> ? 0.f : Pk, at[v], fold[buf][k][GV + v][lane]);
+          if (REDUCE && v < GV) Pt[v] *= Pk;
         }
+      }
+#pragma unroll
+      for (int v = 0; v < VEC; ++v) far |= !finite(at[v]);
+      if (rare(far)) {
+        if (W > 1) __syncthreads();
+        if (!REDUCE)
+#pragma unroll
+          for (int v = 0; v < GV; ++v) {
+            float& own = fold[buf][w][v][lane];
+            if (own == 0) own = product(own, forgets(v));
+          }
+        if (W > 1) __syncthreads();
+#pragma unroll 1
+        for (int k = W - 1; k >= 0; --k) {
+          if (k == w)
+#pragma unroll
+            for (int v = 0; v < VEC; ++v) mine[v] = R[v];
+#pragma unroll
+          for (int v = 0; v < VEC; ++v) R[v] = apply(fold[buf][k][v % GV][lane], fold[buf][k][GV + v][lane], R[v]);
+        }
+      } else {
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) R[v] = at[v];
+      }
+      if (REDUCE) {  // a product that becomes 0, or leaves the range, in this tile is taken once more
+        bool turns = false;
+#pragma unroll
+        for (int v = 0; v < GV; ++v) turns |= P[v] != 0 && (Pt[v] == 0 || !finite(Pt[v]));
+        if (rare(turns)) {
+#pragma unroll
+          for (int v = 0; v < GV; ++v) Pt[v] = P[v];
+#pragma unroll
+          for (int k = W - 1; k >= 0; --k)
+#pragma unroll
+            for (int v = 0; v < GV; ++v) Pt[v] = both(Pt[v], fold[buf][k][v][lane]);
+        }
+#pragma unroll
+        for (int v = 0; v < GV; ++v) P[v] = P[v] == 0 ? P[v] : Pt[v];
       }
       buf ^= W > 1;
     }

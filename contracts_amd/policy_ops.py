@@ -39,7 +39,8 @@ def linear_scan(x, gate, state=None, done=None, reverse=False, out=None, state_o
     x: [T, E, C] float32, bfloat16 or float16 (float64 without gradients).  gate: [T, E, H] of x's type or float32, H
     dividing C (channel c is under gate c // (C // H)); strides of 0 share it along time or rows; or a float, one constant.  A gate
     of exactly 0 forgets the state whatever it held, as done does.  Gates over 1 are taken; their product over any stretch of steps without a
-    border has to stay in the state's range, for stretches are composed as maps h -> P h + H (and a P under that range counts as 0).  state: [E, C] float32 (float64 with x).  done: [T, E] bool or uint8.
+    border may not pass the state's range, for stretches are composed as maps h -> P h + H; one under that range takes nothing of a finite state,
+    while an infinity or NaN shows until a border or a gate of 0, however small the gates.  state: [E, C] float32 (float64 with x).  done: [T, E] bool or uint8.
     The state is float32 throughout (float64 with x); y is rounded once.  Differentiable in x, gate and state (dy and dlast), from the
     unrounded states: one of every 16 is kept between the passes.  out / state_out: dense tensors to write to, without gradients;
     state_out may be `state`."""

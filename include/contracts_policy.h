@@ -38,7 +38,8 @@ const char* ce_policy_error(void);
  * so that an episode that ends with step t hands nothing over the border between t and t + 1 in either direction, and cutting
  * the time axis into calls (`last` of one is `state` of the next) changes nothing.  A gate of exactly 0 forgets the
  * state whatever it held (infinities and NaN included), as done does.  The product of the gates over any stretch of steps without a
- * border has to stay in the state's range (a stretch is composed as a map h -> P h + H; a P under that range counts as 0).  The state is carried in float (double for CE_F64); each
+ * border may not pass the state's range (a stretch is composed as a map h -> P h + H); one under that range takes nothing of a finite
+ * state, while an infinity or NaN shows until a border or a gate of 0, however small the gates.  The state is carried in float (double for CE_F64); each
  * y is rounded once to its own type and the rounded value is not used again.  T = 0 hands the state on.
  * Types: x and y dtype; gate dtype or CE_F32; state and last float (CE_F64: double throughout, and no backward pass).
  * gate == NULL: the constant `decay`.  state / done / last / saved may be NULL (zeros / none ended / not wanted).

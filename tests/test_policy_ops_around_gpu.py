@@ -80,3 +80,69 @@ def test_gradients_that_carry_more_than_numbers_are_refused(ops):
         torch.autograd.grad(out, x, d, retain_graph=True)
 
 
+@pytest.mark.parametrize("E,C", [(1, 3), (2, 260), (600, 256)])
+@pytest.mark.parametrize("T,gate", [(40, 1e-3), (40, -1e-3), (150, 1e-5), (700, 0.5), (1400, -0.875), (40, 2.0 ** -140)])
+def test_a_state_that_is_not_finite_shows_to_the_end(ops, T, gate, E, C):
+    """however small the product of the gates behind it: only done and a gate of 0 forget, whatever waves and chunks the sizes make"""
+    if T > 64 and E * C > 1000:
+        E = 8  # (enough columns for another plan, not more than 64 bits take in a moment)
+    bad = torch.tensor([float("inf"), float("nan"), -float("inf")], device="cuda")
+    gate = float(np.float32(gate))
+    for dt, u in ((F32, oracle.U32), (F64, oracle.U64)):
+        for reverse in (False, True):
+            x, _, state, _ = scan_inputs(T, E, C, 0, dt, dt, 3)
+            full = torch.full((T, E, 1), gate, device="cuda", dtype=dt)
+            at = T - 3 if reverse else 2
+            x[at, 0, :3] = bad[:C].to(dt)
+            state[-1, -1] = -float("inf")
+            done = torch.zeros((T, E), dtype=torch.bool, device="cuda")
+            stop = T // 8 if reverse else T - T // 8  # a border (or a zero gate) far behind forgets
+            for how in ("nothing", "done", "gate", "negative zero"):
+                if how == "done":
+                    done[stop, 0] = True
+                elif how != "nothing":
+                    done[stop, 0] = False
+                    full[stop, 0] = 0.0 if how == "gate" else -0.0
+                for g in ((gate, full, full.expand(T, E, C).contiguous()) if how in ("nothing", "done") else (full, full.expand(T, E, C).contiguous())):
+                    want = oracle.scan(x, g, state, done, reverse, u)
+                    y, last = ops.linear_scan(x, g, state=state, done=done, reverse=reverse)
+                    oracle.close(y, want["y"], oracle.rounded(want["y"], want["ybound"], dt), "%s %s" % (how, reverse))
+                    oracle.close(last, want["last"], want["lastbound"] + np.abs(want["last"]) * u, how)
+
+
+@pytest.mark.parametrize("T,gate", [(40, 1e-3), (150, -1e-5), (700, 0.5)])
+def test_a_gradient_that_is_not_finite_shows_to_the_start(ops, T, gate):
+    for E, C, H in ((1, 3, 3), (2, 130, 1), (3, 24, 4)):
+        for reverse in (False, True):
+            x, _, state, _ = scan_inputs(T, E, C, 0, F32, F32, 3)
+            full = torch.full((T, E, H), gate, device="cuda")
+            done = torch.zeros((T, E), dtype=torch.bool, device="cuda")
+            dy, dl = torch.randn((T, E, C), device="cuda"), torch.zeros((E, C), device="cuda")
+            dy[2 if reverse else T - 3, 0, :3] = torch.tensor([float("inf"), float("nan"), -float("inf")], device="cuda")[:C]
+            dl[-1, -1] = float("inf")
+            for border in (False, True):
+                if border:
+                    done[T - T // 8 if reverse else T // 8, 0] = True
+                leaves = [t.detach().requires_grad_(True) for t in (x, full, state)]
+                y, last = ops.linear_scan(leaves[0], leaves[1], state=leaves[2], done=done, reverse=reverse)
+                dx, _, dstate = torch.autograd.grad((y, last), leaves, (dy, dl))
+                f = oracle.scan(x, full, state, done, reverse)
+                with np.errstate(invalid="ignore"):
+                    want = oracle.scan_grad(f, dy, dl, H, reverse)
+                oracle.close(dx, want["dx"], oracle.rounded(want["dx"], want["dxbound"], F32), "dx")
+                oracle.close(dstate, want["dstate"], want["dstatebound"] + np.abs(np.nan_to_num(want["dstate"])) * oracle.U32, "dstate")
+
+
+@pytest.mark.parametrize("P", [20, 40, 100, 300])
+def test_an_advantage_that_is_not_finite_shows_to_the_start(ops, P):
+    r, v = torch.randn((P, 3, 2), dtype=F64, device="cuda"), torch.randn((P, 3, 2), device="cuda")
+    r[-2, 0, 0], r[-2, 1, 0], r[-2, 2, 1] = float("inf"), float("nan"), -float("inf")
+    done = torch.zeros((P, 3), dtype=torch.bool, device="cuda")
+    for gl in (1e-30, -1e-30, 1e-250):
+        for border in (False, True):
+            done[P // 8] = border
+            got = ops.advantages(r, v, None, done, gamma=0.5, lam=2 * gl)
+            for a, b in zip(got, oracle.advantages(r, v, None, done, 0.5, 2 * gl, 0)):
+                oracle.close(a, b, oracle.rounded(b, 1e-12 * (1 + np.abs(b)), F32), "%g %s" % (gl, border))
+
+
