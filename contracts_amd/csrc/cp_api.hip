@@ -41,6 +41,7 @@ int launched(hipError_t e, const char* what) {
 
 uint64_t size_of(uint32_t t) { return t == CE_U8 ? 1 : t == CE_BF16 || t == CE_F16 ? 2 : t == CE_F32 || t == CE_I32 ? 4 : 8; }
 bool half_or_float(uint32_t t) { return t == CE_F32 || t == CE_BF16 || t == CE_F16; }
+bool finite_float(double v) { return std::isfinite((float)v); }  // as the kernels hold it
 bool aligned(const void* p, uint64_t to) { return (uintptr_t)p % to == 0; }
 
 constexpr uint64_t kMost = 1ull << 28;   // columns of a scan: a launch has fewer than 2^32 threads
@@ -71,7 +72,7 @@ int check_scan(const ce_scan* s) {
   if (s->steps > kFar || (s->steps && s->rows * s->channels > kFar / s->steps)) return refuse("linear_scan: too many elements");
   if (s->rows * s->channels == 0) return CE_OK;
   if (s->steps && (!s->x || !s->y)) return refuse("linear_scan: null x or y");
-  if (!s->gate && !std::isfinite(s->decay)) return refuse("linear_scan: decay must be finite");
+  if (!s->gate && !(s->dtype == CE_F64 ? std::isfinite(s->decay) : finite_float(s->decay))) return refuse("linear_scan: decay must be finite in the state's type");
   const uint64_t b = size_of(s->dtype), a = s->dtype == CE_F64 ? 8 : 4;
   if (!aligned(s->x, b) || !aligned(s->y, b) || !aligned(s->state, a) || !aligned(s->last, a) || !aligned(s->saved, 4) || (s->gate && !aligned(s->gate, size_of(s->gate_dtype))))
     return refuse("linear_scan: a pointer is not aligned to its type");
@@ -275,7 +276,7 @@ extern "C" int ce_advantages(const ce_advantage* a, void* stream) {
   if (a->reward_dtype != CE_F64 && a->reward_dtype != CE_F32) return refuse("advantages: reward must be double or float");
   if (!half_or_float(a->value_dtype)) return refuse("advantages: value must be float, bfloat16 or half");
   if (a->flags & ~CE_ADV_DONE_PER_AGENT) return refuse("advantages: unknown flags %#x", a->flags);
-  if (!std::isfinite(a->gamma) || !std::isfinite(a->lam)) return refuse("advantages: gamma and lam must be finite");
+  if (!std::isfinite(a->gamma) || !std::isfinite(a->lam) || !std::isfinite(a->gamma * a->lam)) return refuse("advantages: gamma, lam and their product must be finite");
   if (a->rows > kMost || a->agents > kMost || a->rows * a->agents > kMost) return refuse("advantages: more than 2^28 columns (rows x agents)");
   if (a->planes > kFar || (a->planes && a->rows * a->agents > kFar / a->planes)) return refuse("advantages: too many elements");
   if (a->planes * a->rows * a->agents == 0) return CE_OK;
@@ -304,8 +305,9 @@ static int check_logits(const ce_logits* s) {
   if (s->tokens) {
     if (s->token_dtype != CE_U8 && s->token_dtype != CE_I32 && s->token_dtype != CE_I64) return refuse("process_logits: tokens must be uint8, int32 or int64");
     if (!aligned(s->tokens, size_of(s->token_dtype))) return refuse("process_logits: tokens are not aligned to their type");
-    if (!s->repetition && !(s->repetition_all > 0 && std::isfinite(s->repetition_all))) return refuse("process_logits: repetition must be positive and finite");
-    if ((!s->presence && !std::isfinite(s->presence_all)) || (!s->frequency && !std::isfinite(s->frequency_all))) return refuse("process_logits: presence and frequency must be finite");
+    // the kernels take the reciprocal too: both are to be normal floats
+    if (!s->repetition && !(s->repetition_all >= 0x1p-126 && s->repetition_all <= 0x1p126)) return refuse("process_logits: repetition must be positive, from 2^-126 to 2^126");
+    if ((!s->presence && !finite_float(s->presence_all)) || (!s->frequency && !finite_float(s->frequency_all))) return refuse("process_logits: presence and frequency must be finite floats");
   } else if (s->lengths || s->prompt_lengths) {
     return refuse("process_logits: lengths without tokens");
   }

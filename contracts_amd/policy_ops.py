@@ -75,7 +75,8 @@ def process_logits(logits, *, tokens=None, lengths=None, prompt_lengths=None, re
                   `lengths` [...] count, the first `prompt_lengths` [...] of these are its prompt; ids outside [0, V) are passed over
       repetition  > 0: l / repetition where l > 0, else l * repetition, for a token seen anywhere in the history
       presence    taken off a token that occurs behind the prompt;  frequency: taken off as often as it occurs there.
-                  Each of the three is a float or a float32 [...] tensor, one for each row
+                  Each of the three is a float or a float32 [...] tensor, one for each row; repetition lies between 2^-126 and 2^126 (a tensor's entries
+                  are not checked), the others are finite
       bias        added: [V], the last axes of the logits ([n, V] for [E, n, V]), or [B, V] for logits [R, V] with B dividing R (row r takes
                   row r mod B); float32 or the logits' type
       mask        -inf where it forbids, whatever stands there; bool / uint8 [.., V] (nonzero = allowed), or int32 [.., ceil(V / 32)] words

@@ -42,7 +42,7 @@ const char* ce_policy_error(void);
  * state, while an infinity or NaN shows until a border or a gate of 0, however small the gates.  The state is carried in float (double for CE_F64); each
  * y is rounded once to its own type and the rounded value is not used again.  T = 0 hands the state on.
  * Types: x and y dtype; gate dtype or CE_F32; state and last float (CE_F64: double throughout, and no backward pass).
- * gate == NULL: the constant `decay`.  state / done / last / saved may be NULL (zeros / none ended / not wanted).
+ * gate == NULL: the constant `decay`, finite in the state's type.  state / done / last / saved may be NULL (zeros / none ended / not wanted).
  * `last` may be `state` itself (a state moved on in place); no other overlap of outputs with inputs.  x_row and gate_row are not
  * negative, and the rows that 256 channels span, min(E - 1, 255 / C + 1) of them (none where C is a
  * multiple of 256 and heads a power of two of channels), lie within 2^28 elements of each other. */
@@ -122,7 +122,8 @@ int ce_advantages(const ce_advantage* a, void* stream);
  * Arithmetic in float, one rounding to the output's type.
  * History: tokens (CE_U8 / CE_I32 / CE_I64) at tokens[r * token_row + i * token_step], i < min(lengths[r], L) (lengths NULL: L;
  * a negative length counts as 0); those with i < prompt_lengths[r] (NULL: none) are the prompt.  A token outside [0, V) is
- * passed over.  repetition / presence / frequency: one float a row, or NULL with the scalar of that name.  repetition > 0.
+ * passed over.  repetition / presence / frequency: one float a row, or NULL with the scalar of that name (a finite float).  repetition lies between
+ * 2^-126 and 2^126; a row's is not checked.
  * bias: [bias_rows][V] dense, float or the logits' type; row r takes row r mod bias_rows (bias_rows divides R).
  * mask: CE_U8 [mask_rows][V], nonzero = allowed, or CE_I32 [mask_rows][ceil(V / 32)], bit v % 32 of word v / 32.  Row r takes
  * row mask_index[r] — negative: everything is allowed; past the end: nothing is — or, without an index, row r mod mask_rows.

@@ -216,3 +216,24 @@ def test_tracers_transforms_and_wrapped_tensors_are_refused():
                 run()
         with pytest.raises(ValueError, match="no CPU path"):
             call(torch.nn.Parameter(x))
+
+
+def test_scalars_are_checked_as_the_kernels_hold_them(L):
+    """finite and positive as a double is not enough where float arithmetic follows: what becomes 0 or infinite there is refused"""
+    from contracts_amd import _lib
+    nbytes = C.c_uint64()
+    for value in (1e-50, 2.0 ** -127, 1e-39, 2.0 ** 126 * 1.0001, 1e39, 1e300):
+        s = _logits(tokens=FAKE, token_dtype=5, history=3, repetition_all=value)
+        assert L.ce_process_logits(C.byref(s), None) == EINVAL and b"repetition must be positive" in L.ce_policy_error()
+    for kw in (dict(presence_all=1e39), dict(frequency_all=-1e300)):
+        s = _logits(tokens=FAKE, token_dtype=5, history=3, **kw)
+        assert L.ce_process_logits(C.byref(s), None) == EINVAL and b"finite" in L.ce_policy_error()
+    g = _lib.CeLogitsGrad(dout=FAKE, dlogits=FAKE + 4096)
+    for kw in (dict(repetition_all=2.0 ** -126), dict(repetition_all=2.0 ** 126), dict(presence_all=-3e38), dict(repetition=FAKE, repetition_all=0.0)):  # (a call that launches nothing)
+        assert L.ce_process_logits_backward_workspace(C.byref(_logits(tokens=FAKE, token_dtype=5, history=3, **kw)), C.byref(g), C.byref(nbytes)) == 0
+    for dtype, ok in ((_lib.F32, 3e38), (_lib.BF16, 3e38), (_lib.F64, 1e300)):
+        for decay, fine in ((ok, True), (1e39, dtype == _lib.F64), (-1e39, dtype == _lib.F64), (float("inf"), False)):
+            rc = L.ce_linear_scan_workspace(C.byref(_scan(dtype=dtype, gate_dtype=dtype, gate=None, decay=decay)), C.byref(nbytes))
+            assert rc == (0 if fine else EINVAL) and (fine or b"finite" in L.ce_policy_error())
+    f = dict(abi_version=1, reward_dtype=_lib.F64, value_dtype=_lib.F32, planes=4, rows=3, agents=2, reward=FAKE, value=FAKE, advantage=FAKE, ret=FAKE)
+    assert L.ce_advantages(C.byref(_lib.CeAdvantage(gamma=1e200, lam=1e200, **f)), None) == EINVAL and b"finite" in L.ce_policy_error()

@@ -146,3 +146,19 @@ def test_an_advantage_that_is_not_finite_shows_to_the_start(ops, P):
                 oracle.close(a, b, oracle.rounded(b, 1e-12 * (1 + np.abs(b)), F32), "%g %s" % (gl, border))
 
 
+
+
+@pytest.mark.parametrize("V", [9, 700])
+def test_repetitions_at_the_borders_of_their_range(ops, V):
+    """2^-126 and 2^126, of which both the number and its reciprocal are normal floats"""
+    R = 4
+    l = torch.rand((R, V), generator=gen(1), device="cuda") + 1
+    l = torch.where(torch.rand((R, V), generator=gen(2), device="cuda") < 0.5, l, -l)
+    tok = torch.randint(0, V, (R, 30), generator=gen(3), device="cuda").to(torch.int32)
+    dz = torch.ones((R, V), device="cuda")
+    for rep in (2.0 ** -126, 2.0 ** 126, torch.tensor([2.0 ** -126, 1.0, 2.0 ** 126, 3.0], device="cuda")):
+        want = oracle.logits(l, tok, repetition=rep, dz=dz)
+        leaf = l.clone().requires_grad_(True)
+        z = ops.process_logits(leaf, tokens=tok, repetition=rep)
+        oracle.close(z, want["z"], oracle.rounded(want["z"], want["bound"], F32), "z")
+        oracle.close(torch.autograd.grad(z, leaf, dz)[0], want["dlogits"], oracle.rounded(want["dlogits"], want["dlogitsbound"], F32), "dlogits")
