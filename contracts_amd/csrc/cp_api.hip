@@ -45,7 +45,7 @@ bool finite_float(double v) { return std::isfinite((float)v); }  // as the kerne
 bool aligned(const void* p, uint64_t to) { return (uintptr_t)p % to == 0; }
 
 constexpr uint64_t kMost = 1ull << 28;   // columns of a scan: a launch has fewer than 2^32 threads
-constexpr uint64_t kMostRows = 1ull << 23;  // rows of scores, for the same reason
+constexpr uint64_t kMostRows = (1ull << 24) - 1;  // rows of scores: short ones are packed, 8 and more to a block; long ones go in parts
 constexpr uint64_t kFar = 1ull << 46;    // elements: products of sizes stay far inside 64 bits
 
 // ---- the scan ---------------------------------------------------------------------------------------------------------------------
@@ -296,7 +296,7 @@ static int check_logits(const ce_logits* s) {
   if (s->abi_version != CE_POLICY_ABI_VERSION) return refuse("ce_logits.abi_version is %u, this library is %d", s->abi_version, CE_POLICY_ABI_VERSION);
   if (!half_or_float(s->dtype)) return refuse("process_logits: logits must be float, bfloat16 or half");
   if (s->out_dtype != s->dtype && s->out_dtype != CE_F32) return refuse("process_logits: the output must be of the logits' type or float");
-  if (s->rows > kMostRows) return refuse("process_logits: more than 2^23 rows");
+  if (s->rows > kMostRows) return refuse("process_logits: 2^24 rows or more");
   if (s->vocab > (1ull << 28)) return refuse("process_logits: more than 2^28 tokens");
   if (s->history > (1ull << 31) - 1) return refuse("process_logits: a history of more than 2^31 - 1 tokens");
   if (s->rows * s->vocab == 0) return CE_OK;

@@ -70,7 +70,7 @@ def process_logits(logits, *, tokens=None, lengths=None, prompt_lengths=None, re
                    mask_index=None, out=None):
     """Scores or logits shaped ahead of a selection: penalties for repeated tokens (or past actions), biases, masks.
 
-    logits: [..., V] float32, bfloat16 or float16; the leading axes are R rows (envs x agents, sequences).  In this order, in float32, rounded once:
+    logits: [..., V] float32, bfloat16 or float16; the leading axes are R rows (envs x agents, sequences), fewer than 2^24 in a call.  In this order, in float32, rounded once:
       tokens      [..., L] uint8, int32 or int64 of any strides (`actions.permute(1, 2, 0)` of [T, E, n] action planes), a row's history; only its first
                   `lengths` [...] count, the first `prompt_lengths` [...] of these are its prompt; ids outside [0, V) are passed over
       repetition  > 0: l / repetition where l > 0, else l * repetition, for a token seen anywhere in the history

@@ -119,7 +119,7 @@ int ce_advantages(const ce_advantage* a, void* stream);
  * For row r and token v, with `seen` = v occurs in the row's history and `count` = how often it occurs behind its prompt:
  *   z = l;  seen: z = l > 0 ? l / repetition : l * repetition;  count > 0: z -= presence;  z -= frequency * count;  z += bias;
  *   a token that the mask forbids: -inf, whatever l and bias hold (a row whose mask leaves nothing is -inf throughout)
- * Arithmetic in float, one rounding to the output's type.
+ * Arithmetic in float, one rounding to the output's type.  Fewer than 2^24 rows, at most 2^28 tokens, histories shorter than 2^31.
  * History: tokens (CE_U8 / CE_I32 / CE_I64) at tokens[r * token_row + i * token_step], i < min(lengths[r], L) (lengths NULL: L;
  * a negative length counts as 0); those with i < prompt_lengths[r] (NULL: none) are the prompt.  A token outside [0, V) is
  * passed over.  repetition / presence / frequency: one float a row, or NULL with the scalar of that name (a finite float).  repetition lies between

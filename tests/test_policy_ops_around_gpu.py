@@ -162,3 +162,39 @@ def test_repetitions_at_the_borders_of_their_range(ops, V):
         z = ops.process_logits(leaf, tokens=tok, repetition=rep)
         oracle.close(z, want["z"], oracle.rounded(want["z"], want["bound"], F32), "z")
         oracle.close(torch.autograd.grad(z, leaf, dz)[0], want["dlogits"], oracle.rounded(want["dlogits"], want["dlogitsbound"], F32), "dlogits")
+
+
+@pytest.mark.parametrize("V", [7, 8])
+def test_logits_of_more_than_two_to_the_23_rows(ops, V):
+    """a learner's batch of 65 steps of 16 384 envs x 8 agents has more; numbers that float32 holds exactly, so that the plain form's equal"""
+    n, L = 4, 3
+    R = (1 << 23) + 3 * n
+    g = gen(V)
+    l = torch.randint(-8, 9, (R, V), generator=g, device="cuda") * 0.5
+    tok = torch.randint(0, V, (R, L), generator=g, device="cuda").to(torch.uint8)
+    bias, allowed = torch.randint(-4, 5, (n, V), generator=g, device="cuda") * 0.25, torch.rand((n, V), generator=g, device="cuda") < 0.7
+    count = torch.zeros((R, V), device="cuda")
+    for i in range(L):
+        count.scatter_add_(1, tok[:, i:i + 1].long(), torch.ones((R, 1), device="cuda"))
+    factor = torch.where(count > 0, torch.where(l > 0, 0.5, 2.0), 1.0)
+    ok = allowed.repeat(R // n, 1)
+    leaf, bleaf = l.clone().requires_grad_(True), bias.clone().requires_grad_(True)
+    z = ops.process_logits(leaf, tokens=tok, repetition=2.0, presence=0.5, frequency=0.25, bias=bleaf, mask=allowed)
+    assert z.equal(torch.where(ok, l * factor - 0.5 * (count > 0) - 0.25 * count + bias.repeat(R // n, 1), -float("inf")))
+    dz = torch.randint(-2, 3, (R, V), generator=g, device="cuda").float()
+    dl, db = torch.autograd.grad(z, (leaf, bleaf), dz)
+    assert dl.equal(torch.where(ok, dz * factor, 0.0)) and db.equal(torch.where(ok, dz, 0.0).double().view(-1, n, V).sum(0).float())
+
+
+def test_long_logits_of_more_than_two_to_the_23_rows(ops):
+    R, V = (1 << 23) + 2, 520
+    l = torch.zeros((R, V), dtype=BF16, device="cuda")
+    l[-1, -1], l[-2, 0], l[1 << 22, 7] = 1, 2, 3
+    bias = torch.arange(V, device="cuda").float()
+    ops.process_logits(l, bias=bias, out=l)
+    l -= bias.to(BF16)
+    # 519 and 1 + 519 are both 520 in bfloat16 (steps of 4 there): the last place is 0 again, like all that held 0
+    assert l[-1, -1].item() == 0 and l[-2, 0].item() == 2 and l[1 << 22, 7].item() == 3 and l[:-2].count_nonzero().item() == 1 and l[-2:, 1:-1].count_nonzero().item() == 0
+    from contracts_amd._lib import EngineError
+    with pytest.raises(EngineError, match="2\\^24 rows"):
+        ops.process_logits(l[:1].expand(1 << 24, V))
