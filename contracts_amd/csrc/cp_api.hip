@@ -337,6 +337,15 @@ extern "C" int ce_process_logits(const ce_logits* s, void* stream) {
   return launched(cp::launch_logits(*s, (hipStream_t)stream), "process_logits");
 }
 
+struct Reach {
+  uintptr_t lo, hi;  // the bytes of [rows][width] elements, rows `row` elements apart
+  bool meets(const Reach& o) const { return lo < o.hi && o.lo < hi; }
+};
+static Reach reach(const void* p, uint64_t rows, int64_t row, uint64_t width, uint64_t size) {
+  const int64_t last = (int64_t)(rows - 1) * row, lo = std::min<int64_t>(last, 0), hi = std::max<int64_t>(last, 0) + (int64_t)width;
+  return {(uintptr_t)p + (uintptr_t)(lo * (int64_t)size), (uintptr_t)p + (uintptr_t)(hi * (int64_t)size)};
+}
+
 static int check_logits_grad(const ce_logits* s, const ce_logits_grad* g) {
   if (!g) return refuse("null ce_logits_grad");
   if (int rc = check_logits(s)) return rc;
@@ -345,6 +354,10 @@ static int check_logits_grad(const ce_logits* s, const ce_logits_grad* g) {
   if (g->dbias && !s->bias) return refuse("process_logits_backward: dbias without a bias");
   if (!aligned(g->dout, size_of(s->out_dtype)) || !aligned(g->dlogits, size_of(s->dtype)) || (g->dbias && !aligned(g->dbias, size_of(s->bias_dtype))))
     return refuse("process_logits_backward: a pointer is not aligned to its type");
+  // the repeats' launch reads both again where the walk has written dlogits
+  const Reach dl = reach(g->dlogits, s->rows, (int64_t)s->vocab, s->vocab, size_of(s->dtype));
+  if (g->dlogits && (dl.meets(reach(g->dout, s->rows, g->dout_row, s->vocab, size_of(s->out_dtype))) || dl.meets(reach(s->logits, s->rows, s->logits_row, s->vocab, size_of(s->dtype)))))
+    return refuse("process_logits_backward: dlogits overlaps dout or the logits");
   return CE_OK;
 }
 

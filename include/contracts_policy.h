@@ -78,7 +78,7 @@ int ce_linear_scan(const ce_scan* s, void* stream);
  *   g_t = dy_t + (the successor's a g, nothing over a border that done closes);  dx = g;  dgate = sum over a head's channels
  *   of g_t k_t;  dstate = a g of the first step
  * dx in dtype, dgate in gate_dtype ([T][E][H] dense, NULL with a constant gate), dstate float (or NULL).
- * Sums run in float, in one fixed order: the same call gives the same bits. */
+ * Outputs overlap no input.  Sums run in float, in one fixed order: the same call gives the same bits. */
 typedef struct ce_scan_grad {
   const void* dy;
   const void* dlast;
@@ -153,9 +153,9 @@ typedef struct ce_logits {
 
 int ce_process_logits(const ce_logits* s, void* stream);
 
-/* Gradient of the output (dout, in logits' type, row stride dout_row) taken back: dlogits (logits' type, [R][V] dense) = dout scaled as l was, 0
+/* Gradient of the output (dout, in out_dtype, row stride dout_row) taken back: dlogits (logits' type, [R][V] dense) = dout scaled as l was, 0
  * where forbidden; dbias (bias_dtype, [bias_rows][V] dense) = the sum over the rows that share a bias row, in float and in one fixed order.
- * Either may be NULL.  fwd->out is not read. */
+ * Either may be NULL.  dlogits overlaps neither dout nor the logits.  fwd->out is not read. */
 typedef struct ce_logits_grad {
   const void* dout;
   int64_t dout_row;

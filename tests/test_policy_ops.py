@@ -237,3 +237,21 @@ def test_scalars_are_checked_as_the_kernels_hold_them(L):
             assert rc == (0 if fine else EINVAL) and (fine or b"finite" in L.ce_policy_error())
     f = dict(abi_version=1, reward_dtype=_lib.F64, value_dtype=_lib.F32, planes=4, rows=3, agents=2, reward=FAKE, value=FAKE, advantage=FAKE, ret=FAKE)
     assert L.ce_advantages(C.byref(_lib.CeAdvantage(gamma=1e200, lam=1e200, **f)), None) == EINVAL and b"finite" in L.ce_policy_error()
+
+
+def test_logits_gradients_do_not_overlap_what_they_are_made_of(L):
+    """dlogits is written before the scores under a repetition penalty are read again: not over dout, nor over the logits"""
+    from contracts_amd import _lib
+    nbytes, size, far = C.c_uint64(), 6 * 10 * 4, FAKE + 8192
+    for dout, logits, dlogits, fine in ((FAKE, far, FAKE, False), (FAKE, far, far, False), (FAKE, far, FAKE + size - 4, False), (FAKE, far, far - size + 4, False), (FAKE, far, FAKE + size, True),
+                                        (FAKE, far, far - size, True), (FAKE, far, far + size, True)):
+        s, g = _logits(tokens=FAKE, token_dtype=5, history=3, logits=logits), _lib.CeLogitsGrad(dout=dout, dout_row=10, dlogits=dlogits)
+        assert L.ce_process_logits_backward_workspace(C.byref(s), C.byref(g), C.byref(nbytes)) == (0 if fine else EINVAL)
+        if not fine:
+            assert b"overlaps" in L.ce_policy_error() and L.ce_process_logits_backward(C.byref(s), C.byref(g), None) == EINVAL
+    # rows apart, backwards or shared: what lies between the first and the last counts
+    for row, reach in ((20, 5 * 20 + 10), (0, 10), (-20, 10)):
+        s, g = _logits(logits=far), _lib.CeLogitsGrad(dout=FAKE + 4096, dout_row=row, dlogits=FAKE + 4096 + 4 * reach)
+        assert L.ce_process_logits_backward_workspace(C.byref(s), C.byref(g), C.byref(nbytes)) == 0
+        g.dlogits -= 4
+        assert L.ce_process_logits_backward_workspace(C.byref(s), C.byref(g), C.byref(nbytes)) == EINVAL
