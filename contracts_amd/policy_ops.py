@@ -34,7 +34,8 @@ def linear_scan(x, gate, state=None, done=None, reverse=False, out=None, state_o
     Forward in time h_t = a_t h_{t-1} + x_t from h_{-1} = state, `last` = the state after step T - 1; with `reverse`
     h_t = a_t h_{t+1} + x_t from h_T = state, `last` = h_0.  done[t, e] says that an episode ended with step t: nothing crosses the border
     between t and t + 1, in either direction (going forward, `last` is 0 where done[T - 1]).  So `last` is the `state` of the next
-    call: one of T = 1 moves a sampler's memory on, and a rollout may be scanned in pieces.
+    call: one of T = 1 moves a sampler's memory on, and a rollout may be scanned in pieces.  (A sampler that learns of done after the step clears
+    the state of the rows that ended itself: state.masked_fill_(done[:, None] != 0, 0).)
 
     x: [T, E, C] float32, bfloat16 or float16 (float64 without gradients).  gate: [T, E, H] of x's type or float32, H
     dividing C (channel c is under gate c // (C // H)); strides of 0 share it along time or rows; or a float, one constant.  A gate

@@ -198,3 +198,36 @@ def test_long_logits_of_more_than_two_to_the_23_rows(ops):
     from contracts_amd._lib import EngineError
     with pytest.raises(EngineError, match="2\\^24 rows"):
         ops.process_logits(l[:1].expand(1 << 24, V))
+
+
+@pytest.mark.parametrize("E,n", [(3, 2), (17, 3)])
+def test_a_samplers_memory_is_the_learners_across_episodes(ops, E, n):
+    """the documented loop: single steps in place, the rows of episodes that a step ended cleared behind it; the learner's scan of the same rollout,
+    cut by its done flags, sees the same memory at every step"""
+    from contracts_amd.engine import BatchedEnv
+    T, D = 23, 12
+    env = BatchedEnv("cleanup", E, n, contract="cleanup", horizon=5, auto_reset=True)
+    env.seed(seed0=5)
+    env.reset()
+    g = gen(E)
+    x, gate = torch.randn((T, E * n, D), generator=g, device="cuda"), torch.rand((T, E * n, D), generator=g, device="cuda")
+    acts = torch.randn((T, E, n, env.num_actions), generator=g, device="cuda")
+    state = torch.randn((E * n, D), generator=g, device="cuda")
+    state0, memory, done = state.clone(), [], torch.zeros((T, E), dtype=torch.uint8, device="cuda")
+    for t in range(T):
+        mem, _ = ops.linear_scan(x[t][None], gate[t][None], state=state, state_out=state)
+        memory.append(mem[0])
+        env.step_policy_device(acts[t].data_ptr(), "argmax")
+        env.synchronize()
+        ended = env.torch_tensors()["done"].bool().repeat_interleave(n)
+        state.masked_fill_(ended[:, None], 0)
+        done[t] = env.torch_tensors()["done"]
+    env.close()
+    assert int(done.sum()) == E * (T // 5)
+    want = oracle.scan(x, gate, state0, done.repeat_interleave(n, 1), False)
+    bound = oracle.rounded(want["y"], want["ybound"], F32)
+    oracle.close(torch.stack(memory), want["y"], bound, "sampler")
+    y, last = ops.linear_scan(x, gate, state=state0, done=done.repeat_interleave(n, 1))
+    oracle.close(y, want["y"], bound, "learner")
+    for s in (state, last):
+        oracle.close(s, want["last"], want["lastbound"] + np.abs(want["last"]) * oracle.U32, "state")
