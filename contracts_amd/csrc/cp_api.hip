@@ -95,7 +95,9 @@ int check_scan(const ce_scan* s) {
 //    4096 waves in all: [65537, 1, 1024] bfloat16, 16 heads: 78 with 128 chunks and 4 channels a lane, 168 with 16 chunks and 1 channel;
 //    [1000, 37, 360] float keeps whole at 1672 waves: 31 against 36.  Gradients: [1000, 37, 360] float, 9 heads: 54 with 8 chunks of pairs of
 //    channels, 60 whole with one; [1000, 64, 256] float 71 whole with one (2048 waves), 81 in chunks.
-void share(cp::ScanParams& p, int* vec, bool grad, bool halves, uint64_t columns, uint64_t (*blocks)(const cp::ScanParams&, uint64_t columns, int vec)) {
+//  * a state moved on in place keeps the time axis whole (`split` is false), with the lanes and waves that suit that: its chunks would read the incoming
+//    state while the last of them writes the outgoing one.
+void share(cp::ScanParams& p, int* vec, bool grad, bool halves, bool split, uint64_t columns, uint64_t (*blocks)(const cp::ScanParams&, uint64_t columns, int vec)) {
   p.chunks = p.waves = 1;
   if (p.T <= CE_SCAN_SAVED_STEPS) return;
   const int widest = *vec;
@@ -106,7 +108,7 @@ void share(cp::ScanParams& p, int* vec, bool grad, bool halves, uint64_t columns
   } else {
     while (*vec > 1 && blocks(p, columns, *vec) * p.waves < 4096) *vec /= 2;
   }
-  if (blocks(p, columns, *vec) * p.waves >= 1536 || p.T < CE_SCAN_SPLIT_STEPS) return;
+  if (blocks(p, columns, *vec) * p.waves >= 1536 || p.T < CE_SCAN_SPLIT_STEPS || !split) return;
   *vec = widest;
   if (grad) p.waves = 4;
   const uint64_t have = blocks(p, columns, widest) * p.waves, tile = p.waves * CE_SCAN_SAVED_STEPS;
@@ -142,7 +144,7 @@ void plan_scan(const ce_scan* s, const ce_scan_grad* g, Plan* o) {
   p.T = T;
   p.head = (uint32_t)head;
   const bool sums = g && o->mode == cp::kGateHead;
-  share(p, &vec, g != nullptr, b == 2, E * C, sums ? head_waves : flat_waves);
+  share(p, &vec, g != nullptr, b == 2, g || !s->last || s->last != s->state, E * C, sums ? head_waves : flat_waves);
   o->vec = vec;
   const bool rev = s->flags & CE_SCAN_REVERSE;
   const int64_t sign = rev ? -1 : 1, off = rev && T ? (int64_t)T - 1 : 0;
@@ -183,8 +185,6 @@ void plan_scan(const ce_scan* s, const ce_scan_grad* g, Plan* o) {
   }
   const uint32_t spanned = 62 / p.row_cols + 2;  // rows that 64 lanes can touch
   p.flags = !s->done ? cp::kFlagsNone : spanned <= 4 ? cp::kFlags4 : spanned <= 16 ? cp::kFlags16 : cp::kFlagsLane;
-  // the chunks of a split time axis read the incoming state while the last of them writes the outgoing one
-  if (!g && s->last && s->last == s->state) p.chunks = 1;
   if (p.chunks == 1) p.chunk = T;
 }
 

@@ -43,7 +43,7 @@ const char* ce_policy_error(void);
  * y is rounded once to its own type and the rounded value is not used again.  T = 0 hands the state on.
  * Types: x and y dtype; gate dtype or CE_F32; state and last float (CE_F64: double throughout, and no backward pass).
  * gate == NULL: the constant `decay`, finite in the state's type.  state / done / last / saved may be NULL (zeros / none ended / not wanted).
- * `last` may be `state` itself (a state moved on in place); no other overlap of outputs with inputs.  x_row and gate_row are not
+ * `last` may be `state` itself (a state moved on in place; the time axis is then never split over blocks, however few); no other overlap of outputs with inputs.  x_row and gate_row are not
  * negative, and the rows that 256 channels span, min(E - 1, 255 / C + 1) of them (none where C is a
  * multiple of 256 and heads a power of two of channels), lie within 2^28 elements of each other. */
 #define CE_SCAN_REVERSE 1u

@@ -231,3 +231,18 @@ def test_a_samplers_memory_is_the_learners_across_episodes(ops, E, n):
     oracle.close(y, want["y"], bound, "learner")
     for s in (state, last):
         oracle.close(s, want["last"], want["lastbound"] + np.abs(want["last"]) * oracle.U32, "state")
+
+
+@pytest.mark.parametrize("T,E,C,H", [(511, 2, 6, 2), (512, 1, 8, 4), (700, 3, 24, 4), (2051, 2, 10, 10), (5000, 8, 64, 1), (1000, 37, 360, 9), (600, 520, 256, 256)])
+@pytest.mark.parametrize("dt,gt", [(F32, F32), (BF16, F32), (F64, F64)])
+def test_a_long_scan_moves_a_state_on_in_place(ops, T, E, C, H, dt, gt):
+    """the bits of the call with a state_out of its own, cut into chunks as that is: it reads the incoming state while the outgoing one is written"""
+    if T * E * C > 1 << 24:
+        dt = gt = BF16
+    for reverse in (False, True):
+        x, gate, state, done = scan_inputs(T, E, C, H, dt, gt, 9)
+        y, last = ops.linear_scan(x, gate, state=state, done=done, reverse=reverse)
+        for _ in range(3):
+            s, out = state.clone(), torch.empty_like(x)
+            y2, s2 = ops.linear_scan(x, gate, state=s, done=done, reverse=reverse, out=out, state_out=s)
+            assert y2 is out and s2 is s and out.equal(y) and s.equal(last)
