@@ -246,3 +246,78 @@ def test_a_long_scan_moves_a_state_on_in_place(ops, T, E, C, H, dt, gt):
             s, out = state.clone(), torch.empty_like(x)
             y2, s2 = ops.linear_scan(x, gate, state=s, done=done, reverse=reverse, out=out, state_out=s)
             assert y2 is out and s2 is s and out.equal(y) and s.equal(last)
+
+
+@pytest.mark.parametrize("T,E,C,H", [(700, 3, 12, 4), (1100, 2, 130, 2), (530, 5, 6, 6)])
+@pytest.mark.parametrize("dt,gt", [(F32, F32), (BF16, F32), (F16, F16)])
+def test_a_split_scan_takes_strides_orders_and_shared_gates(ops, T, E, C, H, dt, gt):
+    """time axes long enough for chunks, with their gradients: batch-major and channel-first memory, slices of wider tensors, gates and done shared or turned"""
+    x, gate, state, done = scan_inputs(T, E, C, H, dt, gt, 6, done=0.03)
+    dy, dl = torch.randn((T, E, C), generator=gen(7), device="cuda").to(dt), torch.randn((E, C), generator=gen(8), device="cuda")
+    batch = lambda t: t.transpose(0, 1).contiguous().transpose(0, 1)  # noqa: E731
+    chan = lambda t: t.permute(2, 0, 1).contiguous().permute(1, 2, 0)  # noqa: E731
+
+    def wide(t, by=3):
+        w = torch.full((t.shape[0], t.shape[1] + 2, t.shape[2] + 2 * by), float("nan"), device="cuda", dtype=t.dtype)
+        w[:, 1:-1, by:-by] = t
+        return w[:, 1:-1, by:-by]
+
+    def check(xx, gg, reverse, tag):
+        """gg: a gate of [T, E, H], or a smaller one that is expanded to it; gradients come in its own shape"""
+        leaves = [t.detach().requires_grad_(True) for t in (xx, gg, state.t().contiguous().t())]
+        full = leaves[1].expand(T, E, H)
+        y, last = ops.linear_scan(leaves[0], full, state=leaves[2], done=done.t().contiguous().t(), reverse=reverse)
+        f = oracle.scan(x, full, state, done, reverse)
+        oracle.close(y, f["y"], oracle.rounded(f["y"], f["ybound"], dt), tag + " y")
+        oracle.close(last, f["last"], f["lastbound"] + np.abs(f["last"]) * oracle.U32, tag + " last")
+        b = oracle.scan_grad(f, dy, dl, H, reverse)
+        dx, dg, ds = torch.autograd.grad((y, last), leaves, (batch(dy), dl.t().contiguous().t()))
+        oracle.close(dx, b["dx"], oracle.rounded(b["dx"], b["dxbound"], dt), tag + " dx")
+        oracle.close(ds, b["dstate"], b["dstatebound"] + np.abs(b["dstate"]) * oracle.U32, tag + " dstate")
+        if gg.shape == (T, E, H):
+            oracle.close(dg, b["dgate"], oracle.rounded(b["dgate"], b["dgatebound"], gt), tag + " dgate")
+        elif gt == F32:  # torch adds the shared entries up in float, a rounding for every doubling at best, one a term at worst
+            axes, terms = tuple(i for i in range(2) if gg.shape[i] == 1 and (T, E)[i] > 1), np.abs(b["dgate"]) + b["dgatebound"]
+            oracle.close(dg, b["dgate"].sum(axes, keepdims=True), (b["dgatebound"] + T * E * oracle.U32 * terms).sum(axes, keepdims=True), tag + " dgate")
+
+    for reverse in (False, True):
+        for k, xx in enumerate((batch(x), chan(x), wide(x), wide(x, 4))):
+            check(xx, (batch(gate), wide(gate), chan(gate), gate)[k], reverse, "layout %d" % k)
+        for shape in ((1, 1, H), (1, E, H), (T, 1, H)):
+            check(batch(x), gate[:shape[0], :shape[1]].clone(), reverse, "gate %s" % (shape,))
+
+
+def test_gradients_follow_torchs_current_stream(ops):
+    """inputs and gradients that a side stream is still making: forward, backward and their scratch memory wait by stream order alone"""
+    x, gate, state, done = scan_inputs(3000, 1, 16, 4, F32, F32, 12)
+    l, tok, lengths, prompt, pen, u = logits_inputs(40, 3000, 50, F32, 4)
+    bias = torch.randn((2, 3000), generator=gen(1), device="cuda")
+    dy, dl, dz = torch.randn_like(x), torch.randn_like(state), torch.randn_like(l)
+    reward, value = torch.randn((300, 8, 2), dtype=F64, device="cuda"), torch.randn((300, 8, 2), device="cuda")
+
+    def work(made):
+        xx, dyy, ll, dzz, rr = made((x, dy, l, dz, reward))
+        leaves = [t.detach().requires_grad_(True) for t in (xx, gate, state, ll, bias)]
+        y, last = ops.linear_scan(leaves[0], leaves[1], state=leaves[2], done=done)
+        z = ops.process_logits(leaves[3], tokens=tok, lengths=lengths, prompt_lengths=prompt, bias=leaves[4], **pen)
+        return [y.detach(), last.detach(), z.detach(), *torch.autograd.grad((y, last, z), leaves, (dyy, dl, dzz)), *ops.advantages(rr, value)]
+
+    want = work(lambda ts: ts)
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    for _ in range(3):
+        empty = [torch.full_like(t, float("nan")) for t in (x, dy, l, dz, reward)]
+        torch.cuda.synchronize()
+
+        def late(ts):
+            big = torch.randn((4096, 4096), device="cuda")
+            for _ in range(30):
+                big = big @ big * 1e-2
+            for e, t in zip(empty, ts):
+                e.copy_(t + 0 * torch.nan_to_num(big[0, 0], 0, 0, 0))
+            return empty
+        with torch.cuda.stream(side):
+            got = work(late)
+            done_there = side.record_event()
+        done_there.synchronize()
+        assert all(a.equal(b) for a, b in zip(got, want))
