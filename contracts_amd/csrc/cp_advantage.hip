@@ -3,7 +3,7 @@
 // A_t = delta_t + gamma lam A_{t+1}: the recurrence of cp_scan.hip run against time, its input delta_t made on the way from reward,
 // value and done.  A lane owns one agent of one env (neighbouring lanes, neighbouring addresses), the W waves of a block share
 // its time axis in runs of kSteps steps.  double throughout: the engine's rewards are, and V_{t+1} - V_t cancels; bound by HBM all the
-// same: 64 planes of 16 384 envs x 8 agents in 34 us, 5.0 TB/s.  20 planes of 64 x 2 take 6.3 us, one run's chain of reads and the launch.
+// same: 64 planes of 16 384 envs x 8 agents in 32 us, 5.4 TB/s.  20 planes of 64 x 2 take 6.1 us, one run's chain of reads and the launch.
 #include "cp_common.h"
 
 namespace cp {

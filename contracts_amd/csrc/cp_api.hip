@@ -91,8 +91,9 @@ int check_scan(const ce_scan* s) {
 //  * else the waves of a block share the time axis (a second walk in registers), 8 of them, and lanes take fewer channels as long as that
 //    makes waves: [512, 256, 256] bfloat16 36 with 2 channels a lane, 43 with 4, 40 with 4 waves; the gradients' longer walks do better with 4
 //    waves where 2048 can be had: 75 against 82.
-//  * under 1536 waves that way, the time axis is cut into chunks too, which costs reading x and the gate twice, at least a tile each and
-//    4096 waves in all: [65537, 1, 1024] bfloat16, 16 heads: 78 with 128 chunks and 4 channels a lane, 168 with 16 chunks and 1 channel;
+//  * under 1536 waves that way, the time axis is cut into chunks too, which costs reading x and the gate twice, at least a tile each, up
+//    to 4096 waves in all, in whole tiles: [65537, 1, 1024] bfloat16, 16 heads: 77 with 103 chunks (of 640 steps: 128 chunks would be of 513) and 4 channels a
+//    lane, 168 with 16 chunks and 1 channel;
 //    [1000, 37, 360] float keeps whole at 1672 waves: 31 against 36.  Gradients: [1000, 37, 360] float, 9 heads: 54 with 8 chunks of pairs of
 //    channels, 60 whole with one; [1000, 64, 256] float 71 whole with one (2048 waves), 81 in chunks.
 //  * a state moved on in place keeps the time axis whole (`split` is false), with the lanes and waves that suit that: its chunks would read the incoming

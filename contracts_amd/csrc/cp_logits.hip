@@ -123,8 +123,8 @@ __device__ __forceinline__ float only(float z, uint32_t ok, int q) {
 // What does not wait for something else is read first (a block is a chain of reads: the fewer links, the better): scores, the first tokens of the
 // history whatever its length, the row's own numbers; then the mask, whose place one of these names.  (Scores taken apart where they are read, or
 // read behind a branch, cost a wait of their own: 36 us against 33 at 256 x 131072 bfloat16, 160 against 153 for both passes at 2048 x 32000.)
-// The table is 16 KB, 8 blocks a CU.  (Entries of 16 bits and runs of 8192 gain nothing: 29.7 us against 29.0 at 256 x 131072 bfloat16 with
-// histories of up to 2048, 6.1 against 4.7 at 1 x 50257 float; without a history the same pass takes 22, as a copy does.)
+// The table is 16 KB, 8 blocks a CU.  (Entries of 16 bits and runs of 8192 gain nothing: 2 % slower at 256 x 131072 bfloat16 with
+// histories of up to 2048, 30 % at 1 x 50257 float; the first takes 32 us now, the second 5.2, and the first without a history 22, as a copy does.)
 template <class X, class O, class K> __global__ __launch_bounds__(kBlock) void k_logits_run(ce_logits s, uint64_t row0, uint32_t runs) {
   constexpr int kGroups = kTile / kBlock / kLane, kFirst = 4;
   typedef Pack<X, kLane> Eight;
@@ -307,7 +307,7 @@ hipError_t launch_logits(const ce_logits& s, hipStream_t st) {
 // their sums in a fixed order.
 // The few scores that a repetition penalty scaled are put right behind that, one lane to a token of a history: a token that occurs twice
 // is written twice, with the same value.  (Marking them in LDS ahead of the walk, as the forward pass does, took 113 us where the walk
-// and this take 58 + 27, at 2048 x 32000 bfloat16 with histories of up to 512.)
+// and this take 62 + 24, at 2048 x 32000 bfloat16 with histories of up to 512.)
 constexpr int kCols = kBlock * kLane;
 
 struct GradShape {

@@ -7,7 +7,7 @@
 // writes y is the plain recurrence in float, whatever the cut.  Where E * C gives too few blocks for the 256 CUs, the time
 // axis is cut into chunks too: a first launch reduces every chunk to (P, H), and a chunk of the second folds those before it.
 // Bound by HBM: reads x and a, writes y, 2 flops an element.  [128, 4096, 128] bfloat16, a gate a channel, takes 75-80 us, 5.1-5.4 TB/s, the rate of
-// a large copy; [65537, 1, 1024] bfloat16 under 16 heads 27 + 52 (chunks, then the walk: what is left is the second
+// a large copy; [65537, 1, 1024] bfloat16 under 16 heads 27 + 50 (chunks, then the walk: what is left is the second
 // reading of x, and the chunks ahead that every block folds).  Addresses are a wave's base in scalar registers plus a lane's 32-bit
 // offset: with 64-bit addresses a lane the compiler kept one for every step, spilled, and the gradient kernel took 208 us where it takes 70
 // ([512, 256, 256] bfloat16).
