@@ -19,7 +19,8 @@ int refuse(const char* what, ...) {
   return CE_EINVAL;
 }
 
-// The call's device while it is made; the caller's own is current again afterwards.
+// The call's device while it is made; the caller's own is current again afterwards.  The thread's error state starts clean: what an earlier call of
+// another library left there must not be blamed on the launches that follow.
 struct OnDevice {
   int before = -1;
   hipError_t err;
@@ -27,6 +28,7 @@ struct OnDevice {
     err = hipGetDevice(&before);
     if (err == hipSuccess && before != device) err = hipSetDevice(device);
     else if (err == hipSuccess) before = -1;
+    (void)hipGetLastError();
   }
   ~OnDevice() {
     if (before >= 0) (void)hipSetDevice(before);

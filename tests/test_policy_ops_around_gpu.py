@@ -321,3 +321,22 @@ def test_gradients_follow_torchs_current_stream(ops):
             done_there = side.record_event()
         done_there.synchronize()
         assert all(a.equal(b) for a, b in zip(got, want))
+
+
+def test_another_librarys_error_is_not_blamed_on_a_call(ops):
+    """the runtime keeps a thread's last error until somebody asks: a null argument refused elsewhere says nothing about the launches that follow"""
+    import ctypes
+    runtime = ctypes.CDLL(next(line.split()[-1] for line in open("/proc/self/maps") if "libamdhip64.so" in line))
+    x, r, l = torch.randn((40, 3, 6), device="cuda"), torch.randn((40, 3, 2), device="cuda"), torch.randn((6, 10), device="cuda")
+    leaf, lleaf = x.clone().requires_grad_(True), l.clone().requires_grad_(True)
+    y, z = ops.linear_scan(leaf, 0.5)[0], ops.process_logits(lleaf)
+    dx, dl = torch.ones_like(y), torch.ones_like(z)
+    calls = [lambda: ops.linear_scan(x, 0.5)[0], lambda: ops.advantages(r, r)[0], lambda: ops.process_logits(l), lambda: torch.autograd.grad(y, leaf, dx, retain_graph=True)[0],
+             lambda: torch.autograd.grad(z, lleaf, dl, retain_graph=True)[0]]
+    for call in calls:
+        want = call()
+        torch.cuda.synchronize()
+        assert runtime.hipGetDevice(None) != 0  # refused on the host; nothing reaches the device
+        got = call()
+        runtime.hipGetLastError()  # a backward pass runs in a thread of torch's own: this one's error is still there, and equal() would be blamed
+        assert got.equal(want)
