@@ -60,9 +60,9 @@ def advantages(reward, value, last_value=None, done=None, gamma=0.99, lam=0.95, 
 
 
 def pack_mask(allowed):
-    """bool [..., V] -> the words of a packed mask, int32 [..., ceil(V / 32)]: bit v % 32 of word v // 32"""
+    """bool or uint8 [..., V] (nonzero = allowed) -> the words of a packed mask, int32 [..., ceil(V / 32)]: bit v % 32 of word v // 32"""
     V = allowed.shape[-1]
-    bits = torch.nn.functional.pad(allowed.to(torch.int64), (0, -V % 32)).unflatten(-1, (-1, 32))
+    bits = torch.nn.functional.pad((allowed != 0).to(torch.int64), (0, -V % 32)).unflatten(-1, (-1, 32))
     words = (bits << torch.arange(32, device=allowed.device)).sum(-1)
     return torch.where(words >= 2 ** 31, words - 2 ** 32, words).to(torch.int32)
 

@@ -255,3 +255,11 @@ def test_logits_gradients_do_not_overlap_what_they_are_made_of(L):
         assert L.ce_process_logits_backward_workspace(C.byref(s), C.byref(g), C.byref(nbytes)) == 0
         g.dlogits -= 4
         assert L.ce_process_logits_backward_workspace(C.byref(s), C.byref(g), C.byref(nbytes)) == EINVAL
+
+
+def test_pack_mask_takes_what_the_masks_of_bytes_take():
+    """nonzero = allowed, as process_logits reads a uint8 mask: a byte of 2 or 255 is one bit, its own"""
+    from contracts_amd import policy_ops as ops
+    m = torch.randint(0, 256, (3, 70), generator=torch.Generator().manual_seed(1)).to(torch.uint8)
+    m[:, ::3] = 0
+    assert ops.pack_mask(m).equal(ops.pack_mask(m != 0))
